@@ -154,6 +154,66 @@ NPU_B200_API int npu_b200_prefill_attention(const void* d_q, const void* d_k, co
                                             int keys, int max_seq, float scale, int causal,
                                             void* stream);
 
+/* ---------------------------------------------------------------------------
+ * Paged key-value cache.
+ *
+ * Keys (and values) of any number of sequences in a pool of fixed-size pages, so
+ * that a cache grows page by page and sequences share what they have in common
+ * (no counterpart in the reference, whose compiled programs hold one flat cache
+ * per sequence):
+ *
+ *   d_k_pages, d_v_pages [num_pages, kv_heads, page_size, head_dim] FP16, 16-byte
+ *                aligned; head_dim in {64, 128}; page_size a multiple of 8 in
+ *                [8, 65536]; num_pages x kv_heads x page_size < 2^31
+ *   d_page_table [batch, table_entries] int32: position j of sequence b is row
+ *                j % page_size of page d_page_table[b][j / page_size].  Entries of
+ *                positions that a call does not touch may hold anything (-1 where
+ *                npu_b200_page_update has none).
+ *
+ * An entry outside [0, num_pages) that a call does need sets the bounds bit of
+ * npu_b200_device_status, and the access is skipped (keys and values read as
+ * zero, new rows are dropped).
+ *
+ * window and sinks: with window > 0 the token at position p sees key j iff
+ * j <= p and (j > p - window or j < sinks): the last `window` keys, itself
+ * included, and the first `sinks`.  window == 0: every key up to p.  Pages that
+ * hold no visible key are not read; their entries may be -1.
+ * ------------------------------------------------------------------------- */
+
+/* Attention of one new token per sequence, at position d_seq_lens[b] - 1 (its
+ * own key and value are in the pages already: npu_b200_paged_append), head h with
+ * KV head h / (q_heads / kv_heads); the counterpart of npu_b200_flash_decode:
+ *
+ *   d_q, d_out [batch, q_heads, head_dim] FP16, 16-byte aligned; any group
+ *   d_seq_lens [batch] int32 keys per sequence, clamped to [0, table_entries x
+ *              page_size]; 0 keys gives a zero row
+ *   d_workspace npu_b200_paged_decode_workspace_size() bytes, 16-byte aligned, on
+ *              the current device; holds nothing between calls and needs no
+ *              clearing.  Calls that may overlap on the GPU need separate ones.
+ * FP32 scores, softmax statistics and accumulation, softmax weights rounded to
+ * FP16, the output rounded once; the work is split over the keys evenly over
+ * the SMs and joined in a fixed order, so the same inputs give the same bits.
+ * Launched as programmatic dependents of the stream's previous work, like
+ * npu_b200_flash_decode. */
+NPU_B200_API size_t npu_b200_paged_decode_workspace_size(int q_heads, int kv_heads, int head_dim);
+NPU_B200_API int npu_b200_paged_decode(const void* d_q, const void* d_k_pages,
+                                       const void* d_v_pages, const int32_t* d_page_table,
+                                       const int32_t* d_seq_lens, void* d_out, int batch,
+                                       int q_heads, int kv_heads, int head_dim, int num_pages,
+                                       int page_size, int table_entries, int window, int sinks,
+                                       float scale, void* d_workspace, size_t workspace_bytes,
+                                       void* stream);
+
+/* New rows of K and V into the pages: row i < d_lens[b] (NULL: every row) of
+ * sequence b to position d_starts[b] + i.  d_k, d_v [batch, kv_heads, rows,
+ * head_dim] FP16, 16-byte aligned; batch <= 65535.  Two rows that the tables send
+ * to one place leave either of them there. */
+NPU_B200_API int npu_b200_paged_append(const void* d_k, const void* d_v, void* d_k_pages,
+                                       void* d_v_pages, const int32_t* d_page_table,
+                                       const int32_t* d_starts, const int32_t* d_lens, int batch,
+                                       int kv_heads, int rows, int head_dim, int num_pages,
+                                       int page_size, int table_entries, void* stream);
+
 /* Linear layer on tcgen05 tensor cores:
  *   out[b, n] = act( sum_k x[b, k] * w[n, k] + bias[n] ),  FP32 accumulation.
  *

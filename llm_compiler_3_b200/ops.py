@@ -6,6 +6,7 @@ here runs a libnpu_b200 kernel and nothing else.  Inputs must be CUDA, FP16
 """
 from __future__ import annotations
 
+import contextlib
 import ctypes
 
 import torch
@@ -114,6 +115,104 @@ def prefill_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Ten
         kv_heads, head_dim, queries, int(keys), max_seq, float(scale), 1 if causal else 0,
         _stream()))
     return out
+
+
+# ---------------------------------------------------------------------------
+# Paged key-value cache (the layout and the rules are in include/npu_b200.h).
+#
+# These operators run on the device of their tensors, whichever is current, on
+# that device's current stream; scratch comes from torch's allocator at each
+# call, so calls on several streams and captured graphs share none.
+# ---------------------------------------------------------------------------
+def _device_of(name: str, t: torch.Tensor, **others: torch.Tensor | None):
+    """Context in which t's device is the current one; every tensor must be on it."""
+    for other, u in others.items():
+        if u is not None and u.device != t.device:
+            raise ValueError(f"{other} is on {u.device} but {name} on {t.device}")
+    if t.device.index == torch.cuda.current_device():
+        return contextlib.nullcontext()
+    return torch.cuda.device(t.device)
+
+
+def _require_pages(k_pages: torch.Tensor, v_pages: torch.Tensor, page_table: torch.Tensor,
+                   batch: int, head_dim: int) -> None:
+    _require(k_pages, "k_pages", ndim=4)
+    _require(v_pages, "v_pages", ndim=4)
+    _require(page_table, "page_table", dtype=torch.int32, ndim=2)
+    if v_pages.shape != k_pages.shape or k_pages.shape[3] != head_dim:
+        raise ValueError(f"k_pages {tuple(k_pages.shape)}, v_pages {tuple(v_pages.shape)} and "
+                         f"head_dim {head_dim} disagree")
+    if page_table.shape[0] != batch:
+        raise ValueError("page_table must have one row per sequence")
+
+
+def _require_counts(t: torch.Tensor, name: str, batch: int) -> None:
+    _require(t, name, dtype=torch.int32, ndim=1)
+    if t.shape[0] != batch:
+        raise ValueError(f"{name} must have one entry per sequence")
+
+
+def _output(out: torch.Tensor | None, shape, dtype: torch.dtype, device: torch.device,
+            name: str = "out") -> torch.Tensor:
+    if out is None:
+        return torch.empty(shape, dtype=dtype, device=device)
+    _require(out, name, dtype=dtype)
+    if out.shape != torch.Size(shape) or out.device != device:
+        raise ValueError(f"{name} must be {tuple(shape)} on {device}")
+    return out
+
+
+def paged_decode(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor,
+                 page_table: torch.Tensor, seq_lens: torch.Tensor, window: int = 0,
+                 sinks: int = 0, scale: float | None = None, out: torch.Tensor | None = None
+                 ) -> torch.Tensor:
+    """Attention of one new token per sequence over a paged cache: q [B, Hq, D], pages
+    [N, Hkv, P, D], page_table [B, E] int32, seq_lens [B] int32 (the new token included).
+
+    Returns out [B, Hq, D] FP16 = softmax(scale q K^T) V over keys [0, seq_lens[b]), with
+    window > 0 over the last `window` of them and the first `sinks`; zero without keys."""
+    _require(q, "q", ndim=3)
+    batch, q_heads, head_dim = q.shape
+    _require_pages(k_pages, v_pages, page_table, batch, head_dim)
+    _require_counts(seq_lens, "seq_lens", batch)
+    num_pages, kv_heads, page_size, _ = k_pages.shape
+    with _device_of("q", q, k_pages=k_pages, v_pages=v_pages, page_table=page_table,
+                    seq_lens=seq_lens):
+        out = _output(out, q.shape, q.dtype, q.device)
+        lib = _native.lib()
+        need = lib.npu_b200_paged_decode_workspace_size(q_heads, kv_heads, head_dim)
+        ws = torch.empty(need, dtype=torch.uint8, device=q.device)
+        _native.check(lib.npu_b200_paged_decode(
+            q.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(), page_table.data_ptr(),
+            seq_lens.data_ptr(), out.data_ptr(), batch, q_heads, kv_heads, head_dim, num_pages,
+            page_size, page_table.shape[1], int(window), int(sinks),
+            head_dim ** -0.5 if scale is None else float(scale), ws.data_ptr(), need, _stream()))
+    return out
+
+
+def paged_append(k: torch.Tensor, v: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor,
+                 page_table: torch.Tensor, starts: torch.Tensor,
+                 lens: torch.Tensor | None = None) -> None:
+    """New keys and values into the pages, in place: k, v [B, Hkv, M, D]; row i < lens[b]
+    (default: every row) of sequence b goes to position starts[b] + i."""
+    _require(k, "k", ndim=4)
+    _require(v, "v", ndim=4)
+    batch, kv_heads, rows, head_dim = k.shape
+    if v.shape != k.shape:
+        raise ValueError("k and v must have one shape")
+    _require_pages(k_pages, v_pages, page_table, batch, head_dim)
+    if k_pages.shape[1] != kv_heads:
+        raise ValueError(f"k has {kv_heads} heads but the pages {k_pages.shape[1]}")
+    _require_counts(starts, "starts", batch)
+    if lens is not None:
+        _require_counts(lens, "lens", batch)
+    num_pages, _, page_size, _ = k_pages.shape
+    with _device_of("k", k, v=v, k_pages=k_pages, v_pages=v_pages, page_table=page_table,
+                    starts=starts, lens=lens):
+        _native.check(_native.lib().npu_b200_paged_append(
+            k.data_ptr(), v.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(),
+            page_table.data_ptr(), starts.data_ptr(), 0 if lens is None else lens.data_ptr(),
+            batch, kv_heads, rows, head_dim, num_pages, page_size, page_table.shape[1], _stream()))
 
 
 def linear(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | None = None,

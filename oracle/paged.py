@@ -1,0 +1,84 @@
+"""64-bit CPU restatement of the paged-cache operators (test infrastructure only).
+
+Written from the definitions in ``include/npu_b200.h``: sequences are rebuilt
+from their pages one by one, every key is shown or hidden by the written rule,
+and softmax is taken in FP64.  ``attention_paged`` also returns, per output
+element, how far a kernel may be off that rounds only where the kernels do:
+
+  * each softmax weight to FP16 before the second product: a relative 2^-11
+    (below 2^-14, FP16's smallest normal number, an absolute 2^-25);
+  * scores in FP32: a dot product of D terms is off by at most (D + 4) 2^-23
+    times the sum of the terms' magnitudes (tensor cores may cut instead of
+    round, hence 2^-23), which moves each weight by that relative amount, and
+    the exponential by 2^-21;
+  * sums of n weights and n products in FP32: n 2^-23 each, relative to the
+    sum of the magnitudes;
+  * the output to FP16: 2^-11 of it (2^-25 below the normal numbers).
+"""
+from __future__ import annotations
+
+import torch
+
+__all__ = ["rows_of_pages", "attention_paged", "append_paged"]
+
+
+def rows_of_pages(pages: torch.Tensor, row: torch.Tensor, n: int) -> torch.Tensor:
+    """Positions [0, n) of one sequence: [Hkv, n, D].  Entries that are no page
+    (their positions must be hidden) give NaN."""
+    page_size = pages.shape[2]
+    parts = []
+    for e in range((n + page_size - 1) // page_size):
+        page = int(row[e])
+        ok = 0 <= page < pages.shape[0]
+        parts.append(pages[page] if ok else torch.full_like(pages[0], float("nan")))
+    if not parts:
+        return pages[0][:, :0]
+    return torch.cat(parts, 1)[:, :n]
+
+
+def attention_paged(q, k_pages, v_pages, table, seq_lens, q_lens=None, window=0, sinks=0,
+                    scale=None):
+    """q [B, Hq, M, D]; query i < q_lens[b] (default M) of sequence b is at position
+    seq_lens[b] - q_lens[b] + i; later rows are zero.  Returns (out, bound) in FP64."""
+    batch, heads, chunk, dim = q.shape
+    kv_heads = k_pages.shape[1]
+    scale = dim ** -0.5 if scale is None else scale
+    out = torch.zeros(q.shape, dtype=torch.float64)
+    bound = torch.zeros(q.shape, dtype=torch.float64)
+    for b in range(batch):
+        n = int(seq_lens[b])
+        m = chunk if q_lens is None else int(q_lens[b])
+        k = rows_of_pages(k_pages, table[b], n).double()
+        v = rows_of_pages(v_pages, table[b], n).double()
+        for i in range(m):
+            p = n - m + i
+            see = [j for j in range(n)
+                   if 0 <= j <= p and (window == 0 or j > p - window or j < sinks)]
+            if not see:
+                continue
+            for h in range(heads):
+                kk, vv = k[h * kv_heads // heads][see], v[h * kv_heads // heads][see]
+                qq = q[b, h, i].double()
+                w = torch.softmax(kk @ qq * scale, 0)
+                out[b, h, i] = w @ vv
+                mass = w @ vv.abs()
+                off = float((kk.abs() @ qq.abs()).max()) * abs(scale) * (dim + 4) * 2.0 ** -23
+                rel = 2.0 ** -11 + 2 * off + 2.0 ** -20 + 2 * len(see) * 2.0 ** -23
+                bound[b, h, i] = (2.0 ** -11 * out[b, h, i].abs() + 2.0 ** -25 + rel * mass
+                                  + len(see) * 2.0 ** -25 * vv.abs().max())
+    return out, bound
+
+
+def append_paged(k, k_pages, table, starts, lens=None):
+    """k [B, Hkv, M, D] into a copy of the pages; rows without a page are dropped."""
+    pages = k_pages.clone()
+    page_size = pages.shape[2]
+    for b in range(k.shape[0]):
+        for i in range(k.shape[2] if lens is None else int(lens[b])):
+            at = int(starts[b]) + i
+            if not 0 <= at < table.shape[1] * page_size:
+                continue
+            page = int(table[b, at // page_size])
+            if 0 <= page < pages.shape[0]:
+                pages[page, :, at % page_size] = k[b, :, i]
+    return pages
