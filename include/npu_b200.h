@@ -214,6 +214,94 @@ NPU_B200_API int npu_b200_paged_append(const void* d_k, const void* d_v, void* d
                                        int kv_heads, int rows, int head_dim, int num_pages,
                                        int page_size, int table_entries, void* stream);
 
+/* The page table of the next step: new row b takes over the first
+ * d_seq_lens[d_parents[b]] tokens of an old row (a parent outside [0, rows): no
+ * tokens), with pages for d_capacity[b] tokens in all (at least those it takes
+ * over).  This is admission (no parent), growth (its own parent, a larger
+ * capacity), forking (several rows with one parent), reordering of beams, and
+ * freeing (an old row that is nobody's parent) in one.  Old and new rows count
+ * from 1 to 8192.
+ *
+ *   Full pages are shared.  The last, partly filled page goes to the lowest new
+ *   row of its parent if nothing else holds it (count 1); every other child gets
+ *   a fresh page and an entry in d_copies, for npu_b200_page_copy.  Pages past the
+ *   tokens are fresh.  The old rows' holds end: their pages that no new row
+ *   shares, and that nobody outside the table holds, are free at once.
+ *   Fresh pages are the lowest free ones (count <= 0), in the order of rows and
+ *   entries.  Entries that are no page stay -1 and cost none.
+ *
+ *   d_page_table [rows, table_entries], d_seq_lens [rows] (clamped to what the
+ *     table reaches), d_parents, d_capacity [new_rows], d_page_refs [num_pages]:
+ *     how many rows (of this table and of others) hold each page; all int32
+ *   d_new_table [new_rows, table_entries] (-1 where there is no page), d_new_lens
+ *     [new_rows], d_new_refs [num_pages]: apart from the old ones, so that a step
+ *     that ran short of pages can be repeated from them
+ *   d_copies [2, new_rows]: the pages to copy from and to, packed at the front in
+ *     the rows' order, -1 after them
+ *   d_info [3]: free pages left, pages that were wanted and not there (their
+ *     entries are -1), copies */
+NPU_B200_API int npu_b200_page_update(const int32_t* d_page_table, const int32_t* d_seq_lens,
+                                      const int32_t* d_parents, const int32_t* d_capacity,
+                                      const int32_t* d_page_refs, int32_t* d_new_table,
+                                      int32_t* d_new_lens, int32_t* d_new_refs, int32_t* d_copies,
+                                      int32_t* d_info, int rows, int new_rows, int table_entries,
+                                      int page_size, int num_pages, void* stream);
+
+/* The pages in use (count > 0) to the front of the pool: with n of them, the k-th
+ * free page below n receives the k-th used page at or above n.
+ *
+ *   d_moves [2, max(1, num_pages / 2)]: from and to, packed, -1 after them
+ *   d_index [num_pages]: where each page is now (-1: free), for other tables
+ *   d_new_table: every entry through d_index (-1 for what is no page in use)
+ *   d_info [2]: n, moves
+ * The data follows with npu_b200_page_copy(d_moves, d_info + 1). */
+NPU_B200_API int npu_b200_page_compact(const int32_t* d_page_table, const int32_t* d_page_refs,
+                                       int32_t* d_new_table, int32_t* d_new_refs, int32_t* d_moves,
+                                       int32_t* d_index, int32_t* d_info, int rows,
+                                       int table_entries, int num_pages, void* stream);
+
+/* Copies pages in every slab of a pool [slabs, num_pages, page_bytes] (for
+ * example K and V of every layer): d_pages [2, n] int32, from and to; the first
+ * min(n, *d_count) of them, or all n without d_count.  Pairs of -1 are skipped, a
+ * pair that names no page sets the bounds bit.  page_bytes a multiple of 16.  No
+ * page that is written may be named twice. */
+NPU_B200_API int npu_b200_page_copy(void* d_pool, const int32_t* d_pages, const int32_t* d_count,
+                                    int n, int slabs, int num_pages, size_t page_bytes,
+                                    void* stream);
+
+/* Beam search, one step: of the beams x vocab continuations of each sequence
+ * (log-softmax of the beam's logits plus its score) the `width` best, best first,
+ * the lowest beam x vocab + token among equals; the beam counterpart of the
+ * ARGMAX epilogue.
+ *
+ *   d_logits [batch, beams, vocab] FP16 (logits_f32 == 0) or FP32, 16-byte aligned;
+ *     -inf bans a token, NaN counts as -inf, +inf as the type's largest number
+ *   d_scores [batch, beams] FP32; -inf (or NaN) takes a beam out
+ *   d_done   [batch, beams] bytes or NULL: a finished beam has one continuation,
+ *     the end token `eos` at its own score.  eos -1: no end token (d_done NULL)
+ *   d_out_scores, d_out_tokens, d_out_parents [batch, width]: parents are rows
+ *     batch x beams + beam, as npu_b200_page_update and npu_b200_beam_reorder take
+ *     them.  Where no continuation is left: -inf, -1, -1
+ *   d_out_done [batch, width] bytes or NULL: finished, now or before
+ *   beams and width in 1..32, batch x beams <= 65535, vocab <= 2^26
+ *   d_workspace npu_b200_beam_select_workspace_size() bytes, 16-byte aligned, on
+ *     the current device; holds nothing between calls
+ * Sums over the vocabulary are FP32 per stretch and FP64 across stretches; the
+ * candidates are compared in FP64. */
+NPU_B200_API size_t npu_b200_beam_select_workspace_size(int batch, int beams, int vocab, int width);
+NPU_B200_API int npu_b200_beam_select(const void* d_logits, int logits_f32, const float* d_scores,
+                                      const uint8_t* d_done, float* d_out_scores,
+                                      int32_t* d_out_tokens, int32_t* d_out_parents,
+                                      uint8_t* d_out_done, int batch, int beams, int vocab,
+                                      int width, int eos, void* d_workspace,
+                                      size_t workspace_bytes, void* stream);
+
+/* Rows of a per-beam state in their new order: out[r] = state[d_parents[r]], a zero
+ * row for -1 (a parent that is no row sets the bounds bit too).  state [rows] and
+ * out [new_rows], row_bytes each, apart from one another. */
+NPU_B200_API int npu_b200_beam_reorder(const void* d_state, const int32_t* d_parents, void* d_out,
+                                       int rows, int new_rows, size_t row_bytes, void* stream);
+
 /* Linear layer on tcgen05 tensor cores:
  *   out[b, n] = act( sum_k x[b, k] * w[n, k] + bias[n] ),  FP32 accumulation.
  *

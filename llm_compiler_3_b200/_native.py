@@ -62,6 +62,15 @@ _SIGNATURES = [
     ("npu_b200_paged_append", c_int,
      [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_int, c_int,
       c_int, c_int, c_int, c_int, c_void_p]),
+    ("npu_b200_page_update", c_int, [c_void_p] * 10 + [c_int] * 5 + [c_void_p]),
+    ("npu_b200_page_compact", c_int, [c_void_p] * 7 + [c_int] * 3 + [c_void_p]),
+    ("npu_b200_page_copy", c_int,
+     [c_void_p, c_void_p, c_void_p, c_int, c_int, c_int, c_size_t, c_void_p]),
+    ("npu_b200_beam_select_workspace_size", c_size_t, [c_int, c_int, c_int, c_int]),
+    ("npu_b200_beam_select", c_int,
+     [c_void_p, c_int] + [c_void_p] * 6 + [c_int] * 5 + [c_void_p, c_size_t, c_void_p]),
+    ("npu_b200_beam_reorder", c_int,
+     [c_void_p, c_void_p, c_void_p, c_int, c_int, c_size_t, c_void_p]),
     ("npu_b200_linear_workspace_size", c_size_t, [c_int, c_int, c_int]),
     ("npu_b200_linear", c_int,
      [c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_int, c_int, c_int, c_void_p, c_size_t,

@@ -215,6 +215,147 @@ def paged_append(k: torch.Tensor, v: torch.Tensor, k_pages: torch.Tensor, v_page
             batch, kv_heads, rows, head_dim, num_pages, page_size, page_table.shape[1], _stream()))
 
 
+def page_update(page_table: torch.Tensor, seq_lens: torch.Tensor, parents: torch.Tensor,
+                capacity: torch.Tensor, page_refs: torch.Tensor, page_size: int
+                ) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor, torch.Tensor, torch.Tensor]:
+    """The page table of the next step: row b continues old row parents[b] (-1: none) with
+    pages for capacity[b] tokens; old rows without a child are freed.
+
+    page_table [R, E], seq_lens [R], parents [R'], capacity [R'], page_refs [N], all int32.
+    Returns (table [R', E], lens [R'], refs [N], copies [2, R'], info [3]): pages to copy
+    (from, to; packed) for `page_copy`, and info = free pages left, pages short, copies.
+    The inputs stay as they are, so a step that ran short can be repeated."""
+    _require(page_table, "page_table", dtype=torch.int32, ndim=2)
+    _require(page_refs, "page_refs", dtype=torch.int32, ndim=1)
+    _require(parents, "parents", dtype=torch.int32, ndim=1)
+    rows, entries = page_table.shape
+    new_rows = parents.shape[0]
+    _require_counts(seq_lens, "seq_lens", rows)
+    _require_counts(capacity, "capacity", new_rows)
+    n = page_refs.shape[0]
+    with _device_of("page_table", page_table, seq_lens=seq_lens, parents=parents,
+                    capacity=capacity, page_refs=page_refs):
+        # One allocation for the five results, each at a 16-byte border.
+        sizes = [(new_rows * entries, (new_rows, entries)), (new_rows, (new_rows,)), (n, (n,)),
+                 (2 * new_rows, (2, new_rows)), (3, (3,))]
+        table, lens, refs, copies, info = _parts(sizes, page_table.device)
+        _native.check(_native.lib().npu_b200_page_update(
+            page_table.data_ptr(), seq_lens.data_ptr(), parents.data_ptr(), capacity.data_ptr(),
+            page_refs.data_ptr(), table.data_ptr(), lens.data_ptr(), refs.data_ptr(),
+            copies.data_ptr(), info.data_ptr(), rows, new_rows, entries, int(page_size), n,
+            _stream()))
+    return table, lens, refs, copies, info
+
+
+def page_compact(page_table: torch.Tensor, page_refs: torch.Tensor
+                 ) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor, torch.Tensor, torch.Tensor]:
+    """The pages in use to the front of the pool: page_table [R, E], page_refs [N] int32.
+
+    Returns (table, refs, moves [2, max(1, N // 2)], index [N], info [2]): pages to copy (from,
+    to; packed), where each page is now (-1: free), and info = pages in use, moves.  Move the
+    data with `page_copy(pool, moves, info[1:])` before the next use of the new table."""
+    _require(page_table, "page_table", dtype=torch.int32, ndim=2)
+    _require(page_refs, "page_refs", dtype=torch.int32, ndim=1)
+    rows, entries = page_table.shape
+    n = page_refs.shape[0]
+    most = max(1, n // 2)
+    with _device_of("page_table", page_table, page_refs=page_refs):
+        sizes = [(rows * entries, (rows, entries)), (n, (n,)), (2 * most, (2, most)), (n, (n,)),
+                 (2, (2,))]
+        table, refs, moves, index, info = _parts(sizes, page_table.device)
+        _native.check(_native.lib().npu_b200_page_compact(
+            page_table.data_ptr(), page_refs.data_ptr(), table.data_ptr(), refs.data_ptr(),
+            moves.data_ptr(), index.data_ptr(), info.data_ptr(), rows, entries, n, _stream()))
+    return table, refs, moves, index, info
+
+
+def _parts(sizes, device: torch.device) -> list[torch.Tensor]:
+    """int32 tensors of (words, shape), cut from one allocation at 16-byte borders."""
+    steps = [(words + 3) & ~3 for words, _ in sizes]
+    whole = torch.empty(sum(steps), dtype=torch.int32, device=device)
+    return [part[:words].view(shape) for part, (words, shape) in zip(whole.split(steps), sizes)]
+
+
+def page_copy(pool: torch.Tensor, pages: torch.Tensor, count: torch.Tensor | None = None) -> None:
+    """Copies pages in place, in every slab of a pool [slabs, N, ...] of any type (K and V of
+    every layer): pages [2, n] int32 (from, to), the first count[0] of them (default: all; -1
+    pairs are skipped).  No page that is written may be named twice."""
+    if not isinstance(pool, torch.Tensor) or not pool.is_cuda or not pool.is_contiguous():
+        raise ValueError("pool must be a contiguous CUDA tensor")
+    if pool.dim() < 3 or pool.numel() == 0:
+        raise ValueError(f"pool must be [slabs, pages, ...], got {tuple(pool.shape)}")
+    _require(pages, "pages", dtype=torch.int32, ndim=2)
+    if pages.shape[0] != 2:
+        raise ValueError("pages must be [2, n]: from and to")
+    if count is not None:
+        _require(count, "count", dtype=torch.int32, ndim=1)
+        if count.shape[0] < 1:
+            raise ValueError("count must hold a number")
+    slabs, n = pool.shape[:2]
+    with _device_of("pool", pool, pages=pages, count=count):
+        _native.check(_native.lib().npu_b200_page_copy(
+            pool.data_ptr(), pages.data_ptr(), 0 if count is None else count.data_ptr(),
+            pages.shape[1], slabs, n, pool.numel() // (slabs * n) * pool.element_size(), _stream()))
+
+
+def beam_select(logits: torch.Tensor, scores: torch.Tensor, width: int,
+                done: torch.Tensor | None = None, eos: int = -1
+                ) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor, torch.Tensor]:
+    """The `width` best continuations of each sequence's beams: logits [B, W, V] FP16 or FP32,
+    scores [B, W] FP32 (summed log-probabilities), done [B, W] bool (finished beams; needs the
+    end token `eos`).
+
+    Returns (scores [B, width] FP32, tokens, parents [B, width] int32, done [B, width] bool),
+    best first, the lowest beam x V + token among equals; parents are rows b x W + beam.  Where
+    nothing is left: -inf, -1, -1, False."""
+    if not isinstance(logits, torch.Tensor) or logits.dtype not in (torch.float16, torch.float32):
+        raise ValueError("logits must be a float16 or float32 tensor")
+    _require(logits, "logits", dtype=logits.dtype, ndim=3)
+    _require(scores, "scores", dtype=torch.float32, ndim=2)
+    batch, beams, vocab = logits.shape
+    if scores.shape != (batch, beams):
+        raise ValueError(f"scores must be {(batch, beams)}, got {tuple(scores.shape)}")
+    if done is not None:
+        _require(done, "done", dtype=torch.bool, ndim=2)
+        if done.shape != scores.shape:
+            raise ValueError("done must have the shape of scores")
+    width = int(width)
+    if width < 1:
+        raise ValueError(f"width must be positive, got {width}")
+    with _device_of("logits", logits, scores=scores, done=done):
+        lib = _native.lib()
+        out_scores = torch.empty(batch, width, dtype=torch.float32, device=logits.device)
+        tokens = torch.empty(batch, width, dtype=torch.int32, device=logits.device)
+        parents = torch.empty(batch, width, dtype=torch.int32, device=logits.device)
+        out_done = torch.empty(batch, width, dtype=torch.bool, device=logits.device)
+        need = lib.npu_b200_beam_select_workspace_size(batch, beams, vocab, width)
+        ws = torch.empty(need, dtype=torch.uint8, device=logits.device)
+        _native.check(lib.npu_b200_beam_select(
+            logits.data_ptr(), logits.dtype == torch.float32, scores.data_ptr(),
+            0 if done is None else done.data_ptr(), out_scores.data_ptr(), tokens.data_ptr(),
+            parents.data_ptr(), out_done.data_ptr(), batch, beams, vocab, width, int(eos),
+            ws.data_ptr(), need, _stream()))
+    return out_scores, tokens, parents, out_done
+
+
+def beam_reorder(state: torch.Tensor, parents: torch.Tensor, out: torch.Tensor | None = None
+                 ) -> torch.Tensor:
+    """Rows of a per-beam state [R, ...] of any type in their new order: out[r] =
+    state[parents[r]] for parents of any shape with R' numbers; -1 gives a zero row."""
+    if not isinstance(state, torch.Tensor) or not state.is_cuda or not state.is_contiguous():
+        raise ValueError("state must be a contiguous CUDA tensor")
+    if state.dim() < 1 or state.numel() == 0:
+        raise ValueError(f"state must be [rows, ...], got {tuple(state.shape)}")
+    _require(parents, "parents", dtype=torch.int32)
+    rows, new_rows = state.shape[0], parents.numel()
+    with _device_of("state", state, parents=parents, out=out):
+        out = _output(out, (new_rows, *state.shape[1:]), state.dtype, state.device)
+        _native.check(_native.lib().npu_b200_beam_reorder(
+            state.data_ptr(), parents.data_ptr(), out.data_ptr(), rows, new_rows,
+            state.numel() // rows * state.element_size(), _stream()))
+    return out
+
+
 def linear(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | None = None,
            relu: bool = False, out_dtype: torch.dtype = torch.float16,
            out: torch.Tensor | None = None) -> torch.Tensor:

@@ -17,3 +17,4 @@ the reference's own known-answer tests.
 from .decode import *  # noqa: F401,F403
 from .graph import run_graph_plan  # noqa: F401
 from .paged import *  # noqa: F401,F403
+from .beam import *  # noqa: F401,F403

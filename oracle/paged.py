@@ -19,7 +19,8 @@ from __future__ import annotations
 
 import torch
 
-__all__ = ["rows_of_pages", "attention_paged", "append_paged"]
+__all__ = ["rows_of_pages", "attention_paged", "append_paged", "page_update", "page_compact",
+           "page_copy"]
 
 
 def rows_of_pages(pages: torch.Tensor, row: torch.Tensor, n: int) -> torch.Tensor:
@@ -82,3 +83,88 @@ def append_paged(k, k_pages, table, starts, lens=None):
             if 0 <= page < pages.shape[0]:
                 pages[page, :, at % page_size] = k[b, :, i]
     return pages
+
+
+def page_update(table, lens, parents, capacity, refs, page_size):
+    """The next step's page table, row by row on Python numbers; returns the lists
+    (table, lens, refs, copies, info) of npu_b200_page_update."""
+    old = [[int(x) for x in row] for row in table]
+    rows, entries, n = len(old), len(old[0]), len(refs)
+    page = lambda x: 0 <= x < n  # noqa: E731
+    left = [int(x) for x in refs]
+    for row in old:
+        for x in row:
+            if page(x):
+                left[x] -= 1
+    new, new_lens, wants, seen = [], [], [], set()
+    for b, parent in enumerate(int(x) for x in parents):
+        row = [-1] * entries
+        length = 0
+        if 0 <= parent < rows:
+            length = min(max(int(lens[parent]), 0), entries * page_size)
+        cap = max(min(max(int(capacity[b]), 0), entries * page_size), length)
+        full, part = divmod(length, page_size)
+        for e in range(full):
+            if page(old[parent][e]):
+                row[e] = old[parent][e]
+                left[row[e]] += 1
+        start = full
+        if part:
+            start += 1
+            last = old[parent][full]
+            if page(last):
+                if parent not in seen and int(refs[last]) == 1:
+                    row[full] = last
+                    left[last] += 1
+                else:
+                    wants.append((b, full, last))
+        if 0 <= parent < rows:
+            seen.add(parent)
+        wants += [(b, e, None) for e in range(start, -(-cap // page_size))]
+        new.append(row)
+        new_lens.append(length)
+    left = [max(x, 0) for x in left]
+    free = [p for p in range(n) if left[p] == 0]
+    copies, short = [], 0
+    for b, e, source in wants:
+        if not free:
+            short += 1
+            continue
+        new[b][e] = free.pop(0)
+        left[new[b][e]] = 1
+        if source is not None:
+            copies.append((source, new[b][e]))
+    pad = len(new) - len(copies)
+    moves = [[s for s, _ in copies] + [-1] * pad, [d for _, d in copies] + [-1] * pad]
+    return new, new_lens, left, moves, [len(free), short, len(copies)]
+
+
+def page_compact(table, refs):
+    """The lists (table, refs, moves, index, info) of npu_b200_page_compact."""
+    n = len(refs)
+    live = [p for p in range(n) if int(refs[p]) > 0]
+    count = len(live)
+    holes = [p for p in range(count) if int(refs[p]) <= 0]
+    high = [p for p in live if p >= count]
+    index = [-1] * n
+    for p in live:
+        index[p] = p
+    for p, to in zip(high, holes):
+        index[p] = to
+    left = [0] * n
+    for p in live:
+        left[index[p]] = int(refs[p])
+    new = [[index[int(x)] if 0 <= int(x) < n else -1 for x in row] for row in table]
+    pad = [-1] * (max(1, n // 2) - len(high))
+    return new, left, [high + pad, holes + pad], index, [count, len(high)]
+
+
+def page_copy(pool, pages, count=None):
+    """pool [slabs, N, ...] with pages[0][i] copied to pages[1][i], as a new tensor."""
+    out = pool.clone()
+    n = len(pages[0]) if count is None else min(max(int(count), 0), len(pages[0]))
+    for i in range(n):
+        s, d = int(pages[0][i]), int(pages[1][i])
+        if 0 <= s < pool.shape[1] and 0 <= d < pool.shape[1]:
+            out[:, d] = pool[:, s]
+    return out
