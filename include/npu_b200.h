@@ -204,6 +204,27 @@ NPU_B200_API int npu_b200_paged_decode(const void* d_q, const void* d_k_pages,
                                        float scale, void* d_workspace, size_t workspace_bytes,
                                        void* stream);
 
+/* Attention of a chunk of new tokens per sequence, on tcgen05; the counterpart of
+ * npu_b200_prefill_attention: query i < d_q_lens[b] (NULL: all `queries`) of
+ * sequence b is at position d_seq_lens[b] - d_q_lens[b] + i, the chunk's own keys
+ * and values being in the pages already.  Causal, with the window and the sinks
+ * of every query's own position.
+ *
+ *   d_q, d_out [batch, q_heads, queries, head_dim] FP16, 16-byte aligned.  Rows past
+ *              d_q_lens[b], at a negative position, or without a visible key, are
+ *              zero
+ *   d_seq_lens [batch] int32 keys per sequence, the chunk included, clamped to
+ *              [0, table_entries x page_size]; d_q_lens [batch] int32, clamped to
+ *              [0, queries]
+ * Arithmetic as in npu_b200_paged_decode. */
+NPU_B200_API int npu_b200_paged_prefill(const void* d_q, const void* d_k_pages,
+                                        const void* d_v_pages, const int32_t* d_page_table,
+                                        const int32_t* d_seq_lens, const int32_t* d_q_lens,
+                                        void* d_out, int batch, int q_heads, int kv_heads,
+                                        int head_dim, int queries, int num_pages, int page_size,
+                                        int table_entries, int window, int sinks, float scale,
+                                        void* stream);
+
 /* New rows of K and V into the pages: row i < d_lens[b] (NULL: every row) of
  * sequence b to position d_starts[b] + i.  d_k, d_v [batch, kv_heads, rows,
  * head_dim] FP16, 16-byte aligned; batch <= 65535.  Two rows that the tables send

@@ -59,6 +59,7 @@ _SIGNATURES = [
     ("npu_b200_paged_decode", c_int,
      [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_int, c_int, c_int,
       c_int, c_int, c_int, c_int, c_int, c_float, c_void_p, c_size_t, c_void_p]),
+    ("npu_b200_paged_prefill", c_int, [c_void_p] * 7 + [c_int] * 10 + [c_float, c_void_p]),
     ("npu_b200_paged_append", c_int,
      [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_int, c_int,
       c_int, c_int, c_int, c_int, c_void_p]),

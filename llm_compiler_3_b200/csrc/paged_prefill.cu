@@ -1,0 +1,548 @@
+// Attention of a chunk of new tokens per sequence over a paged key-value cache.
+//
+// Query i < q_lens[b] of sequence b sits at position p = seq_lens[b] - q_lens[b] + i
+// and sees the keys of paged.cuh: causal, with an optional window and sinks.
+//   out[b, h, i] = sum_j softmax_j(scale q[b, h, i] . k[j]) v[j]
+// in one pass over the keys with a running maximum m, sum l and output O (FP32).
+// The weights are rounded to FP16 as the second product's operand (the values are
+// FP16 too), the output is rounded once.  Rows that see no key, and rows past
+// q_lens[b], are zero.
+//
+// Bound: the tensor cores, 4 D flops per visible (query, key) pair and head, and
+// next to them the exponentials: an SM does 16 a clock, so 128 x 128 of them take
+// as long as the tile's two products at D = 128.  Both run all the time only if two
+// query tiles take turns: while one tile's scores become weights, the tensor cores
+// do the other's P V and next Q K^T.
+//
+// One CTA per pair of query tiles; a tile is 128 rows, `hp` heads of one GQA group
+// x `bm` queries, so that few queries still fill the rows and share one pass over
+// K and V.
+//   warps 0-3, 4-7  softmax of tile 0 / 1: thread r has row r (TMEM lane r)
+//   warp 8          TMA: both Q tiles, then K and V tiles of 128 keys in one ring
+//                   (K0 V0 K1 V1 ...), one box per piece of a page, each lane one
+//   warp 9          MMA issue: S_t = Q_t K^T and O_t += P_t V
+//   warps 10-11     none (a register split goes by groups of four warps)
+// TMEM: S0, S1 (128 columns each), O0, O1 (D each); P_t, FP16, lies over the first
+// half of S_t.  The tensor pipe works in order, so S_t(j + 1), issued after
+// P_t(j) V, cannot overwrite weights that are still read, and its completion says
+// that O_t is up to date.  A row's maximum moves, and its O row is rescaled, only
+// when a tile's exceeds it by 2^8: weights stay below 256, exact enough in FP16.
+#include <math.h>
+
+#include <algorithm>
+
+#include "paged.cuh"
+
+namespace npu_b200 {
+
+void prefill_blocking(int queries, int group, int* bm, int* hp);  // prefill_attention.cu
+
+namespace {
+
+constexpr int kKeys = 128;        // keys per tile
+constexpr int kThreads = 384;
+// Registers: 384 threads launch with 168 each; the softmax threads, which hold a
+// row of scores, take over what the other four warps do not need
+// (256 x 216 + 128 x 72 = 384 x 168).
+constexpr int kRegsLaunch = 168, kRegsSoftmax = 216, kRegsOther = 72;
+static_assert(256 * kRegsSoftmax + 128 * kRegsOther <= kThreads * kRegsLaunch, "register split");
+constexpr uint32_t kTmemCols = 512;
+constexpr float kRescaleLog2 = 8.f;
+
+template <int D>
+struct PpShape {
+  static constexpr int kRegions = D / 64;             // 128-byte swizzle regions of a row
+  static constexpr int kRegionBytes = 128 * 128;      // 128 rows of one region
+  static constexpr int kTileBytes = kRegions * kRegionBytes;  // Q, K or V tile
+  static constexpr int kStages = D == 128 ? 5 : 8;    // K and V tiles in the ring
+  static constexpr int kRing = 2 * kTileBytes;
+  static constexpr int kBars = kRing + kStages * kTileBytes;
+  static constexpr int kNumBars = 1 + 2 * kStages + 6 + 1;
+  static constexpr int kSmem = kBars + kNumBars * 8 + 16 + 1024;
+};
+
+struct PpParams {
+  const int32_t* table;
+  const int32_t* seq_lens;
+  const int32_t* q_lens;  // or null: every query
+  __half* out;
+  int q_heads, kv_heads, queries, entries, page_size, box, num_pages, total_rows;
+  int bm, hp, q_blocks, window, sinks, negate;
+  float scale_log2;  // > 0
+};
+
+__device__ __forceinline__ void tmem_ld32(uint32_t taddr, uint32_t* r) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, "
+      "%13, %14, %15, %16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, "
+      "[%32];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
+        "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]),
+        "=r"(r[15]), "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]),
+        "=r"(r[22]), "=r"(r[23]), "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]),
+        "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+      : "r"(taddr));
+}
+__device__ __forceinline__ void tmem_st32(uint32_t taddr, const uint32_t* r) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, "
+      "%13, %14, %15, %16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31, "
+      "%32};" ::"r"(taddr),
+      "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]),
+      "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(r[16]),
+      "r"(r[17]), "r"(r[18]), "r"(r[19]), "r"(r[20]), "r"(r[21]), "r"(r[22]), "r"(r[23]), "r"(r[24]),
+      "r"(r[25]), "r"(r[26]), "r"(r[27]), "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31])
+      : "memory");
+}
+
+// (a.lo * b + c, a.hi * b + c) and sums of pairs: two FP32 lanes per instruction.
+__device__ __forceinline__ uint64_t pack2(float lo, float hi) {
+  return static_cast<uint64_t>(__float_as_uint(hi)) << 32 | __float_as_uint(lo);
+}
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t d;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
+  return d;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+  uint64_t d;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+  return d;
+}
+__device__ __forceinline__ float lo2(uint64_t a) { return __uint_as_float(static_cast<uint32_t>(a)); }
+__device__ __forceinline__ float hi2(uint64_t a) { return __uint_as_float(static_cast<uint32_t>(a >> 32)); }
+
+// What the two query tiles of a CTA cover.
+struct Span {
+  int seq_len, q_len, first_pos;  // first_pos: position of query 0 of the chunk
+  int lo, len, s;                 // keys that some of the CTA's queries see: [0, s) and [lo, len)
+  TileRange<kKeys> tiles;
+  __device__ __forceinline__ bool sees(int j) const { return j < len && (j >= lo || j < s); }
+  __device__ __forceinline__ bool sees_any(int j, int n) const { return j < len && (j + n > lo || j < s); }
+  __device__ __forceinline__ bool sees_all(int j, int n) const {
+    return j + n <= len && (j >= lo || j + n <= s);
+  }
+};
+
+template <int D>
+__global__ void __launch_bounds__(kThreads, 1)
+    paged_prefill_kernel(const __grid_constant__ CUtensorMap qmap,
+                         const __grid_constant__ CUtensorMap kmap,
+                         const __grid_constant__ CUtensorMap vmap, const PpParams p) {
+  using S = PpShape<D>;
+  constexpr int kStages = S::kStages;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) &
+                                             ~uintptr_t(1023));
+  const uint32_t sQ = smem_u32(smem), sRing = sQ + S::kRing;
+  uint64_t* q_full = reinterpret_cast<uint64_t*>(smem + S::kBars);
+  uint64_t* full = q_full + 1;         // [stages]
+  uint64_t* empty = full + kStages;    // [stages]
+  uint64_t* s_full = empty + kStages;  // [2]
+  uint64_t* p_full = s_full + 2;       // [2]
+  uint64_t* o_done = p_full + 2;       // [2]
+  uint64_t* drain = o_done + 2;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(drain + 1);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int group = p.q_heads / p.kv_heads, subgroups = group / p.hp;
+  const int n_units = p.q_blocks * subgroups;
+  const int hk = static_cast<int>(blockIdx.x) % p.kv_heads;
+  const int b = static_cast<int>(blockIdx.x) / p.kv_heads;
+  // Units (query block, head subgroup), last query blocks first; this CTA has
+  // units u0 (tile 0) and u0 + 1 (tile 1, if there is one).
+  const int u0 = 2 * static_cast<int>(blockIdx.y);
+  const bool has1 = u0 + 1 < n_units;
+  auto unit_m0 = [&](int u) { return (p.q_blocks - 1 - u / subgroups) * p.bm; };
+
+  pdl_launch_dependents();
+  pdl_wait();
+  Span span;
+  span.seq_len = min(max(p.seq_lens[b], 0), p.entries * p.page_size);
+  span.q_len = p.q_lens != nullptr ? min(max(p.q_lens[b], 0), p.queries) : p.queries;
+  span.first_pos = span.seq_len - span.q_len;
+  {
+    const int m_lo = unit_m0(has1 ? u0 + 1 : u0);
+    const int m_hi = min(unit_m0(u0) + p.bm, span.q_len);  // one past the last query
+    const int first = max(0, span.first_pos + m_lo);
+    span.len = m_hi > m_lo ? max(0, span.first_pos + m_hi) : 0;
+    span.lo = p.window > 0 ? max(0, first - p.window + 1) : 0;
+    span.s = min(p.sinks, span.lo);
+    span.tiles.set(span.lo, span.len, p.sinks);
+    if (span.len == 0) span.tiles.n = 0;
+  }
+  const int n_tiles = span.tiles.n;
+
+  if (threadIdx.x == 0) {
+    mbar_init(q_full, 1);
+    for (int s = 0; s < kStages; ++s) {
+      mbar_init(&full[s], 1);
+      mbar_init(&empty[s], 1);
+    }
+    for (int t = 0; t < 2; ++t) {
+      mbar_init(&s_full[t], 1);
+      mbar_init(&p_full[t], 128);
+      mbar_init(&o_done[t], 1);
+    }
+    mbar_init(drain, 1);
+    *abort_flag = 0;
+    fence_barrier_init();
+  }
+  if (warp == 9) {
+    tmem_alloc(tmem_slot, kTmemCols);
+    tmem_relinquish();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = *tmem_slot;
+  if (warp < 8)
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kRegsSoftmax));
+  else
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRegsOther));
+
+  if (warp == 8) {
+    // ---------------- TMA producer ----------------
+    if (n_tiles > 0) {
+      if (lane == 0) {
+        prefetch_tensormap(&qmap);
+        prefetch_tensormap(&kmap);
+        prefetch_tensormap(&vmap);
+        const int tiles_q = has1 ? 2 : 1;
+        mbar_arrive_expect_tx(q_full, static_cast<uint32_t>(tiles_q * p.hp * S::kRegions * p.bm * 128));
+        for (int t = 0; t < tiles_q; ++t) {
+          const int u = u0 + t, m0 = unit_m0(u), gs = u % subgroups;
+          for (int g = 0; g < p.hp; ++g) {
+            const int plane = b * p.q_heads + hk * group + gs * p.hp + g;
+            for (int a = 0; a < S::kRegions; ++a)
+              tma_load_3d(sQ + t * S::kTileBytes + a * S::kRegionBytes + g * p.bm * 128, &qmap, q_full,
+                          a * 64, m0, plane);
+          }
+        }
+      }
+      // Each lane loads one box: rows of one page, one 64-dim region.
+      const int combos = kKeys / p.box * S::kRegions;
+      const int my_region = lane % S::kRegions, my_row = lane / S::kRegions * p.box;
+      const bool mine = lane < combos;
+      auto look_up = [&](int j) {  // the page of this lane's box of tile j; -2: nothing visible
+        const int at = span.tiles.key0(j) + my_row;
+        if (!mine || !span.sees_any(at, p.box)) return -2;
+        return p.table[static_cast<size_t>(b) * p.entries + at / p.page_size];
+      };
+      int page = look_up(0);
+      bool ok = true;
+      int issued = 0;
+      for (int j = 0; ok && j < n_tiles; ++j) {
+        const int at = span.tiles.key0(j) + my_row;
+        int row = p.total_rows;  // past the pool: the box is filled with zeros
+        if (page >= 0 && page < p.num_pages)
+          row = (page * p.kv_heads + hk) * p.page_size + at % p.page_size;
+        else if (page != -2)
+          report_error(kDevErrBounds);
+        if (j + 1 < n_tiles) page = look_up(j + 1);
+        for (int kv = 0; kv < 2; ++kv) {
+          const int x = 2 * j + kv, s = x % kStages;
+          if (x >= kStages)
+            ok = __all_sync(0xffffffffu, wait_or_abort(&empty[s], ((x / kStages) - 1) & 1, abort_flag));
+          if (!ok) break;
+          if (lane == 0) mbar_arrive_expect_tx(&full[s], S::kTileBytes);
+          __syncwarp();
+          if (mine)
+            tma_load_3d(sRing + s * S::kTileBytes + my_region * S::kRegionBytes + my_row * 128,
+                        kv ? &vmap : &kmap, &full[s], my_region * 64, row, 0);
+          issued = x + 1;
+        }
+      }
+      if (!ok) {  // leave no copy in flight into this CTA's shared memory
+        *abort_flag = 1;
+        mbar_wait(q_full, 0, kDevErrTmaTimeout);
+        for (int x = max(0, issued - kStages); x < issued; ++x)
+          mbar_wait(&full[x % kStages], (x / kStages) & 1, kDevErrTmaTimeout);
+      }
+    }
+  } else if (warp == 9) {
+    // ---------------- MMA issuer (lane 0; the warp clears hidden rows of V) ----------------
+    if (n_tiles > 0) {
+      const uint32_t idesc_s = idesc_f16_f32(128, kKeys) | (p.negate ? 1u << 13 : 0u);
+      constexpr uint32_t idesc_pv = idesc_f16_f32(128, D) | kIdescBMajorMN;
+      const uint64_t dq = smem_desc_sw128(sQ), dk = smem_desc_sw128(sRing);
+      const uint64_t dv = smem_desc_sw128_mn(sRing, S::kRegionBytes, 1024);
+      auto wait = [&](uint64_t* bar, uint32_t phase) {
+        return __all_sync(0xffffffffu, lane == 0 ? spin_or_abort(bar, phase, abort_flag) : true);
+      };
+      auto issue_s = [&](int t, int x) {  // x: K's place in the ring's sequence
+        if (lane == 0) {
+          const uint64_t q = dq + (t * S::kTileBytes >> 4);
+          const uint64_t k = dk + ((x % kStages) * S::kTileBytes >> 4);
+#pragma unroll
+          for (int kk = 0; kk < D / 16; ++kk) {
+            const uint32_t off = ((kk >> 2) * S::kRegionBytes + (kk & 3) * 32) >> 4;
+            tc_mma_f16(tmem + t * kKeys, q + off, k + off, idesc_s, kk > 0 ? 1u : 0u);
+          }
+          tc_commit(&s_full[t]);
+        }
+      };
+      auto issue_pv = [&](int t, int x, bool first) {
+        if (lane == 0) {
+          const uint64_t v = dv + ((x % kStages) * S::kTileBytes >> 4);
+#pragma unroll
+          for (int kk = 0; kk < kKeys / 16; ++kk)
+            tc_mma_f16_tmem_a(tmem + 2 * kKeys + t * 128, tmem + t * kKeys + kk * 8, v + (kk * 2048 >> 4),
+                              idesc_pv, !first || kk > 0 ? 1u : 0u);
+        }
+      };
+      bool ok = wait(q_full, 0) && wait(&full[0], 0);
+      if (ok) {
+        tc_fence_after();
+        issue_s(0, 0);
+        issue_s(1, 0);
+        if (lane == 0) tc_commit(&empty[0]);
+      }
+      for (int j = 0; ok && j < n_tiles; ++j) {
+        const int xv = 2 * j + 1, xk = 2 * j + 2, sv = xv % kStages, sk = xk % kStages;
+        ok = wait(&full[sv], (xv / kStages) & 1);
+        if (!ok) break;
+        const int key0 = span.tiles.key0(j);
+        if (!span.sees_all(key0, kKeys)) {
+          // Rows that no query here sees may hold anything; their weights are 0,
+          // but 0 * NaN is NaN.
+          ok = __all_sync(0xffffffffu, wait_or_abort(&full[sv], (xv / kStages) & 1, abort_flag));
+          if (!ok) break;
+          for (int r = lane; r < kKeys; r += 32)
+            if (!span.sees(key0 + r))
+              for (int a = 0; a < S::kRegions; ++a)
+                for (int x = 0; x < 128; x += 16)
+                  *reinterpret_cast<uint4*>(smem + S::kRing + sv * S::kTileBytes + a * S::kRegionBytes +
+                                            r * 128 + x) = make_uint4(0, 0, 0, 0);
+          fence_proxy_async_smem();
+          __syncwarp();
+        }
+        for (int t = 0; t < 2; ++t) {
+          ok = wait(&p_full[t], j & 1);
+          if (!ok) break;
+          tc_fence_after();
+          issue_pv(t, xv, j == 0);
+          if (t == 1 && lane == 0) tc_commit(&empty[sv]);
+          if (j + 1 < n_tiles) {
+            if (t == 0) {
+              ok = wait(&full[sk], (xk / kStages) & 1);
+              if (!ok) break;
+              tc_fence_after();
+            }
+            issue_s(t, xk);
+            if (t == 1 && lane == 0) tc_commit(&empty[sk]);
+          } else if (lane == 0) {
+            tc_commit(&o_done[t]);
+          }
+        }
+      }
+      if (!ok) {  // no MMA may write TMEM after it is released
+        *abort_flag = 1;
+        if (lane == 0) {
+          tc_commit(drain);
+          mbar_wait(drain, 0, kDevErrMmaTimeout);
+        }
+        __syncwarp();
+      }
+    }
+  } else if (warp < 8) {
+    // ---------------- softmax warpgroups ----------------
+    const int tt = warp >> 2, r = threadIdx.x & 127;
+    const bool unit_ok = tt == 0 || has1;
+    const int u = u0 + tt;
+    const int m0 = unit_ok ? unit_m0(u) : 0, gs = u % subgroups;
+    const int g = r / p.bm, i = r % p.bm;
+    const bool row_ok = unit_ok && g < p.hp && m0 + i < p.queries;
+    // Keys of this row: j <= last and (j >= lo or j < sinks).
+    const int last = row_ok && m0 + i < span.q_len ? span.first_pos + m0 + i : -1;
+    const int lo = p.window > 0 ? max(0, last - p.window + 1) : 0;
+    const uint32_t t_lane = tmem + (static_cast<uint32_t>((warp & 3) * 32) << 16);
+    const uint32_t t_s = t_lane + tt * kKeys, t_o = t_lane + 2 * kKeys + tt * 128;
+    float m_run = -INFINITY, l_run = 0.f;
+    bool ok = true;
+    for (int j = 0; j < n_tiles; ++j) {
+      ok = __all_sync(0xffffffffu, wait_or_abort(&s_full[tt], j & 1, abort_flag));
+      if (!ok) break;
+      tc_fence_after();
+      uint32_t sr[kKeys];
+#pragma unroll
+      for (int c = 0; c < kKeys; c += 32) tmem_ld32(t_s + c, sr + c);
+      tmem_ld_wait();
+      const int key0 = span.tiles.key0(j);
+      if (!__all_sync(0xffffffffu, key0 + kKeys - 1 <= last && (key0 >= lo || key0 + kKeys <= p.sinks))) {
+#pragma unroll
+        for (int e = 0; e < kKeys; ++e) {
+          const int key = key0 + e;
+          if (key > last || (key < lo && key >= p.sinks)) sr[e] = 0xff800000u;  // -inf
+        }
+      }
+      float top[8];
+#pragma unroll
+      for (int e = 0; e < 8; ++e) top[e] = __uint_as_float(sr[e]);
+#pragma unroll
+      for (int c = 8; c < kKeys; c += 8)
+#pragma unroll
+        for (int e = 0; e < 8; ++e) top[e] = fmaxf(top[e], __uint_as_float(sr[c + e]));
+      const float mx = fmaxf(fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])),
+                             fmaxf(fmaxf(top[4], top[5]), fmaxf(top[6], top[7])));
+      const float m_tile = mx * p.scale_log2;
+      const bool grow = m_tile > m_run + kRescaleLog2;
+      if (__any_sync(0xffffffffu, grow)) {
+        float alpha = 1.f;
+        if (grow) {
+          alpha = m_run == -INFINITY ? 0.f : fast_exp2(m_run - m_tile);
+          l_run *= alpha;
+          m_run = m_tile;
+        }
+        if (j > 0) {  // rescale this warp's O rows: S_t(j) complete implies P_t(j - 1) V is
+#pragma unroll 1
+          for (int c = 0; c < D; c += 16) {
+            uint32_t o[16];
+            tmem_ld16(t_o + c, o);
+            tmem_ld_wait();
+#pragma unroll
+            for (int e = 0; e < 16; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * alpha);
+            tmem_st16(t_o + c, o);
+          }
+        }
+      }
+      const float m_use = m_run == -INFINITY ? 0.f : m_run;  // no key seen yet: all -inf
+      const uint64_t scale2 = pack2(p.scale_log2, p.scale_log2), minus2 = pack2(-m_use, -m_use);
+      uint64_t sum2[4] = {0, 0, 0, 0};
+#pragma unroll
+      for (int c = 0; c < kKeys; c += 64) {
+        uint32_t pk[32];
+#pragma unroll
+        for (int e = 0; e < 64; e += 2) {
+          const uint64_t s2 = static_cast<uint64_t>(sr[c + e + 1]) << 32 | sr[c + e];
+          const uint64_t x2 = fma2(s2, scale2, minus2);
+          const float w0 = fast_exp2(lo2(x2)), w1 = fast_exp2(hi2(x2));
+          sum2[(e >> 1) & 3] = add2(sum2[(e >> 1) & 3], pack2(w0, w1));
+          pk[e >> 1] = pack_half2(w0, w1);
+        }
+        tmem_st32(t_s + c / 2, pk);  // keys 2q, 2q + 1 in column q
+      }
+      tmem_st_wait();
+      tc_fence_before();
+      mbar_arrive(&p_full[tt]);
+      const uint64_t all2 = add2(add2(sum2[0], sum2[1]), add2(sum2[2], sum2[3]));
+      l_run += lo2(all2) + hi2(all2);
+    }
+    if (ok && n_tiles > 0)
+      ok = __all_sync(0xffffffffu, wait_or_abort(&o_done[tt], 0, abort_flag));
+    if (!ok) {
+      if (lane == 0) *abort_flag = 1;
+    } else {
+      tc_fence_after();
+      const bool any = n_tiles > 0 && l_run != 0.f;
+      const float inv = any ? 1.f / l_run : 0.f;
+      uint4* row = reinterpret_cast<uint4*>(
+          p.out + ((static_cast<size_t>(b) * p.q_heads + hk * group + gs * p.hp + g) * p.queries + m0 + i) * D);
+#pragma unroll 1
+      for (int c = 0; c < D; c += 16) {
+        uint32_t o[16];
+        if (n_tiles > 0) {
+          tmem_ld16(t_o + c, o);
+          tmem_ld_wait();
+        }
+        if (row_ok) {
+          float f[16];
+#pragma unroll
+          for (int e = 0; e < 16; ++e) f[e] = any ? __uint_as_float(o[e]) * inv : 0.f;
+          row[c / 8] = make_uint4(pack_half2(f[0], f[1]), pack_half2(f[2], f[3]), pack_half2(f[4], f[5]),
+                                  pack_half2(f[6], f[7]));
+          row[c / 8 + 1] = make_uint4(pack_half2(f[8], f[9]), pack_half2(f[10], f[11]),
+                                      pack_half2(f[12], f[13]), pack_half2(f[14], f[15]));
+        }
+      }
+    }
+  }
+
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 9) {
+    tc_fence_after();
+    tmem_dealloc(tmem, kTmemCols);
+  }
+}
+
+template <int D>
+int launch_pp(const CUtensorMap& qm, const CUtensorMap& km, const CUtensorMap& vm, const PpParams& p,
+              int batch, cudaStream_t stream) {
+  using S = PpShape<D>;
+  auto kern = paged_prefill_kernel<D>;
+  NPU_TRY_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, S::kSmem));
+  const int n_units = p.q_blocks * (p.q_heads / p.kv_heads / p.hp);
+  LaunchCfg cfg;
+  cfg.grid = dim3(batch * p.kv_heads, (n_units + 1) / 2);
+  cfg.block = dim3(kThreads);
+  cfg.smem = S::kSmem;
+  cfg.stream = stream;
+  cfg.pdl = true;
+  return launch(cfg, kern, qm, km, vm, p);
+}
+
+}  // namespace
+}  // namespace npu_b200
+
+extern "C" int npu_b200_paged_prefill(const void* d_q, const void* d_k_pages, const void* d_v_pages,
+                                      const int32_t* d_page_table, const int32_t* d_seq_lens,
+                                      const int32_t* d_q_lens, void* d_out, int batch, int q_heads,
+                                      int kv_heads, int head_dim, int queries, int num_pages,
+                                      int page_size, int table_entries, int window, int sinks,
+                                      float scale, void* stream) {
+  using namespace npu_b200;
+  clear_error();
+  NPU_REQUIRE(d_q && d_k_pages && d_v_pages && d_page_table && d_seq_lens && d_out,
+              "paged_prefill: null tensor pointer");
+  int rc = check_pages("paged_prefill", kv_heads, head_dim, num_pages, page_size, table_entries);
+  if (rc) return rc;
+  NPU_REQUIRE(batch >= 1 && static_cast<long long>(batch) * kv_heads < (1ll << 31),
+              "paged_prefill: batch %d x kv_heads %d out of range", batch, kv_heads);
+  NPU_REQUIRE(q_heads >= kv_heads && q_heads % kv_heads == 0,
+              "paged_prefill: q_heads %d is not a multiple of kv_heads %d", q_heads, kv_heads);
+  NPU_REQUIRE(queries >= 1, "paged_prefill: queries %d", queries);
+  NPU_REQUIRE(static_cast<long long>(batch) * q_heads < (1ll << 31),
+              "paged_prefill: batch %d x q_heads %d is too large", batch, q_heads);
+  NPU_REQUIRE(window >= 0 && sinks >= 0, "paged_prefill: window %d and sinks %d must not be negative",
+              window, sinks);
+  NPU_REQUIRE(std::isfinite(scale), "paged_prefill: scale is not finite");
+  NPU_REQUIRE(aligned16(d_q) && aligned16(d_k_pages) && aligned16(d_v_pages) && aligned16(d_out),
+              "paged_prefill: q, pages and out must be 16-byte aligned");
+  PpParams p;
+  p.table = d_page_table;
+  p.seq_lens = d_seq_lens;
+  p.q_lens = d_q_lens;
+  p.out = static_cast<__half*>(d_out);
+  p.q_heads = q_heads;
+  p.kv_heads = kv_heads;
+  p.queries = queries;
+  p.entries = table_entries;
+  p.page_size = page_size;
+  p.box = page_box(page_size, kKeys);
+  p.num_pages = num_pages;
+  const uint64_t rows = static_cast<uint64_t>(num_pages) * kv_heads * page_size;
+  p.total_rows = static_cast<int>(rows);
+  prefill_blocking(queries, q_heads / kv_heads, &p.bm, &p.hp);
+  p.q_blocks = (queries + p.bm - 1) / p.bm;
+  NPU_REQUIRE((static_cast<long long>(p.q_blocks) * (q_heads / kv_heads / p.hp) + 1) / 2 <= 65535,
+              "paged_prefill: %d queries make too many query blocks", queries);
+  p.window = window;
+  p.sinks = sinks;
+  // A negative scale negates Q inside the MMA; a scale of 0 is one so small that
+  // every visible key weighs the same, while -inf stays -inf.
+  p.negate = scale < 0.f;
+  p.scale_log2 = std::max(std::fabs(scale) * 1.4426950408889634f, 1e-30f);
+
+  CUtensorMap qm, km, vm;
+  rc = make_tensor_map_3d(&qm, d_q, head_dim, queries, static_cast<uint64_t>(batch) * q_heads,
+                          static_cast<uint64_t>(queries) * head_dim * 2, p.bm, 64);
+  if (rc) return rc;
+  rc = make_tensor_map_3d(&km, d_k_pages, head_dim, rows, 1, rows * head_dim * 2, p.box, 64);
+  if (rc) return rc;
+  rc = make_tensor_map_3d(&vm, d_v_pages, head_dim, rows, 1, rows * head_dim * 2, p.box, 64);
+  if (rc) return rc;
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  return head_dim == 128 ? launch_pp<128>(qm, km, vm, p, batch, s) : launch_pp<64>(qm, km, vm, p, batch, s);
+}

@@ -190,6 +190,34 @@ def paged_decode(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor,
     return out
 
 
+def paged_prefill(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor,
+                  page_table: torch.Tensor, seq_lens: torch.Tensor,
+                  q_lens: torch.Tensor | None = None, window: int = 0, sinks: int = 0,
+                  scale: float | None = None, out: torch.Tensor | None = None) -> torch.Tensor:
+    """Causal attention of a chunk of new tokens over a paged cache: q [B, Hq, M, D], the rest
+    as for `paged_decode`; query i < q_lens[b] (default M) of sequence b is at position
+    seq_lens[b] - q_lens[b] + i.
+
+    Returns out [B, Hq, M, D] FP16; rows past q_lens[b] or without a visible key are zero."""
+    _require(q, "q", ndim=4)
+    batch, q_heads, queries, head_dim = q.shape
+    _require_pages(k_pages, v_pages, page_table, batch, head_dim)
+    _require_counts(seq_lens, "seq_lens", batch)
+    if q_lens is not None:
+        _require_counts(q_lens, "q_lens", batch)
+    num_pages, kv_heads, page_size, _ = k_pages.shape
+    with _device_of("q", q, k_pages=k_pages, v_pages=v_pages, page_table=page_table,
+                    seq_lens=seq_lens, q_lens=q_lens):
+        out = _output(out, q.shape, q.dtype, q.device)
+        _native.check(_native.lib().npu_b200_paged_prefill(
+            q.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(), page_table.data_ptr(),
+            seq_lens.data_ptr(), 0 if q_lens is None else q_lens.data_ptr(), out.data_ptr(), batch,
+            q_heads, kv_heads, head_dim, queries, num_pages, page_size, page_table.shape[1],
+            int(window), int(sinks), head_dim ** -0.5 if scale is None else float(scale),
+            _stream()))
+    return out
+
+
 def paged_append(k: torch.Tensor, v: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor,
                  page_table: torch.Tensor, starts: torch.Tensor,
                  lens: torch.Tensor | None = None) -> None:

@@ -1,0 +1,204 @@
+"""Attention of a chunk of new tokens over a paged cache, against the 64-bit oracle
+(oracle/paged.py, which derives each element's bound; a weight's rounding is
+relative to a maximum that may lag by 2^8, so its absolute part, 2^-25 of the
+largest weight, only shrinks)."""
+import pytest
+import torch
+
+import oracle
+from conftest import seeded
+from test_paged import INF, NAN, check, ints, paged_cache
+
+
+def _prefill(q, k, v, table, lens, q_lens=None, **kw):
+    from llm_compiler_3_b200 import _native, ops
+    out = torch.full(q.shape, NAN, dtype=torch.float16, device="cuda")
+    ops.paged_prefill(q.cuda(), k.cuda(), v.cuda(), table.cuda(), ints(lens).cuda(),
+                      None if q_lens is None else ints(q_lens).cuda(), out=out, **kw)
+    torch.cuda.synchronize()
+    assert _native.device_status() == 0
+    return out.cpu()
+
+
+def check_prefill(q, k, v, table, lens, q_lens=None, **kw):
+    got = _prefill(q, k, v, table, lens, q_lens, **kw)
+    check(got, *oracle.attention_paged(q, k, v, table, lens, q_lens, **kw))
+    return got
+
+
+PREFILL_ARGS = dict(batch=2, q_heads=8, kv_heads=2, head_dim=128, queries=5, num_pages=9, page_size=16,
+                    entries=4, window=0, sinks=0, scale=0.1)
+
+
+@pytest.mark.parametrize("change,message", [
+    (dict(head_dim=96), "head_dim 96"), (dict(q_heads=7), "multiple of kv_heads"),
+    (dict(kv_heads=0), "kv_heads 0"), (dict(page_size=12), "page_size 12"),
+    (dict(num_pages=0), "0 pages"), (dict(num_pages=1 << 26), "too many rows"),
+    (dict(entries=0), "0 table entries"), (dict(batch=0), "batch 0"), (dict(queries=0), "queries 0"),
+    (dict(queries=1 << 26), "too many query blocks"),
+    (dict(window=-1), "window -1"), (dict(sinks=-1), "sinks -1"), (dict(scale=INF), "scale"),
+    (dict(scale=NAN), "scale"),
+])
+def test_refusals(change, message):
+    """Refused on the host, before any CUDA call."""
+    from llm_compiler_3_b200 import _native
+    a = dict(PREFILL_ARGS, **change)
+    p = 1 << 20
+
+    def call(ptrs):
+        return _native.lib().npu_b200_paged_prefill(
+            *ptrs, a["batch"], a["q_heads"], a["kv_heads"], a["head_dim"], a["queries"], a["num_pages"],
+            a["page_size"], a["entries"], a["window"], a["sinks"], a["scale"], None)
+
+    assert call([p] * 7) == -1
+    assert message.encode() in _native.lib().npu_b200_last_error()
+    a = dict(PREFILL_ARGS)
+    for i in (0, 1, 2, 3, 4, 6):
+        assert call([None if j == i else p for j in range(7)]) == -1
+    for i in (0, 1, 2, 6):
+        assert call([p + 8 if j == i else p for j in range(7)]) == -1
+
+
+# ---- on the GPU ------------------------------------------------------------------------------
+@pytest.mark.gpu
+@pytest.mark.parametrize("page", [8, 16, 24, 64, 128, 256])
+@pytest.mark.parametrize("dim", [64, 128])
+def test_page_sizes(cuda, page, dim):
+    """Pages smaller and larger than the 128-key tile; ragged chunks after ragged prefixes."""
+    lens, q_lens = [130, 40, 257, 7, 0], [17, 40, 1, 3, 0]
+    k, v, table = paged_cache(lens, 2, dim, page, seed=page)
+    check_prefill(seeded((5, 4, 40, dim), 3), k, v, table, lens, q_lens)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("heads,kv_heads", [(1, 1), (3, 1), (6, 2), (7, 1), (8, 1), (16, 1), (24, 2), (40, 1)])
+@pytest.mark.parametrize("queries", [1, 5, 33])
+def test_groups_and_few_queries(cuda, heads, kv_heads, queries):
+    """Any number of query heads to a key head, stacked in a tile or over several."""
+    lens = [70, queries]
+    k, v, table = paged_cache(lens, kv_heads, 64, 16, seed=heads)
+    check_prefill(seeded((2, heads, queries, 64), 4), k, v, table, lens)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("queries", [127, 128, 129, 256, 300])
+@pytest.mark.parametrize("dim", [64, 128])
+def test_query_tiles(cuda, queries, dim):
+    """Chunks around one and two query tiles, some rows at negative positions."""
+    lens = [queries + 5, queries // 2]
+    k, v, table = paged_cache(lens, 1, dim, 32, seed=queries)
+    check_prefill(seeded((2, 2, queries, dim), 5), k, v, table, lens)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("window,sinks", [(1, 0), (1, 1), (7, 0), (50, 33), (64, 100), (100, 3), (128, 128),
+                                          (129, 140), (200, 4), (2 ** 31 - 1, 2 ** 31 - 1)])
+def test_window(cuda, window, sinks):
+    """Windows and sinks on, inside and across tile borders; keys that no query sees hold
+    NaN, and the entries of pages without a visible key are no pages."""
+    lens, q_lens = [700, 64, 300, 1, 0, 133], [100, 64, 30, 1, 0, 5]
+    k, v, table = paged_cache(lens, 1, 64, 16, seed=window % 1000 + sinks % 1000)
+    shown = table.clone()
+    for b, (n, m) in enumerate(zip(lens, q_lens)):
+        seen = [j > n - m - window or j < sinks for j in range(n)]
+        for j in range(n):
+            if not seen[j]:
+                k[table[b, j // 16], :, j % 16] = NAN
+                v[table[b, j // 16], :, j % 16] = INF
+        for e in range((n + 15) // 16):
+            if not any(seen[e * 16:e * 16 + 16]):
+                shown[b, e] = -1
+    check_prefill(seeded((6, 2, 100, 64), 6), k, v, shown, lens, q_lens, window=window, sinks=sinks)
+
+
+@pytest.mark.gpu
+def test_window_of_a_long_chunk(cuda):
+    """Query tiles far apart: each reads its own tiles and the sinks'."""
+    lens, q_lens = [900], [700]
+    k, v, table = paged_cache(lens, 1, 128, 64, seed=31)
+    check_prefill(seeded((1, 1, 700, 128), 7), k, v, table, lens, q_lens, window=150, sinks=20)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dim", [64, 128])
+def test_scores_of_any_size(cuda, dim):
+    """Scores far apart (maxima that move), all equal, and negative scales."""
+    lens = [400, 300]
+    k, v, table = paged_cache(lens, 1, dim, 16, seed=9)
+    q = seeded((2, 4, 20, dim), 8, std=20.0)
+    check_prefill(q, k, v, table, lens)
+    check_prefill(q, k, v, table, lens, scale=-0.125)
+    check_prefill(q, k, v, table, lens, scale=0.0)
+    order = torch.arange(400).float()
+    for b, n in enumerate(lens):  # rising scores: the maximum moves at every tile
+        for j in range(n):
+            k[table[b, j // 16], :, j % 16] = order[j] / 100
+    check_prefill(torch.ones(2, 4, 20, dim).half(), k, v, table, lens, scale=0.5)
+
+
+@pytest.mark.gpu
+def test_agrees_with_the_contiguous_operator_and_with_decode(cuda):
+    """A prompt in pages is the prompt in a flat cache; its last row is a decode step."""
+    from llm_compiler_3_b200 import ops
+    n = 517
+    k, v, table = paged_cache([n], 2, 128, 32, seed=12)
+    q = seeded((1, 8, n, 128), 9)
+    got = _prefill(q, k, v, table, [n])
+    flat = [oracle.rows_of_pages(t, table[0], n)[None].contiguous().cuda() for t in (k, v)]
+    want = ops.prefill_attention(q.cuda(), *flat, causal=True).cpu()
+    assert float((got.float() - want.float()).abs().max()) < 1e-2
+    one = ops.paged_decode(q[:, :, -1].contiguous().cuda(), k.cuda(), v.cuda(), table.cuda(), ints([n]).cuda()).cpu()
+    check(got[:, :, -1:], *oracle.attention_paged(q[:, :, -1:], k, v, table, [n]))
+    check(one[:, :, None], *oracle.attention_paged(q[:, :, -1:], k, v, table, [n]))
+
+
+@pytest.mark.gpu
+def test_clamps_lengths_and_reports_bad_pages(cuda):
+    from llm_compiler_3_b200 import _native, ops
+    k, v, table = paged_cache([48, 48], 1, 64, 16, seed=10)
+    q = seeded((2, 2, 9, 64), 9)
+    assert torch.equal(_prefill(q, k, v, table, [1 << 30, -5], [100, 4]), _prefill(q, k, v, table, [48, 0], [9, 4]))
+    assert torch.count_nonzero(_prefill(q, k, v, table, [48, 48], [0, -3])) == 0
+    for page in (-1, k.shape[0], 2 ** 31 - 1, -2 ** 31):
+        bad = table.clone()
+        bad[1, 1] = page
+        out = ops.paged_prefill(q.cuda(), k.cuda(), v.cuda(), bad.cuda(), ints([48, 48]).cuda())
+        with pytest.raises(_native.NpuError, match="0x8"):
+            _native.device_status()
+        assert torch.equal(out[0].cpu(), _prefill(q, k, v, table, [48, 48])[0])
+
+
+@pytest.mark.gpu
+def test_on_streams_and_in_graphs(cuda):
+    from llm_compiler_3_b200 import ops
+    lens = [300, 200]
+    k, v, table = (t.cuda() for t in paged_cache(lens, 1, 128, 16, seed=13))
+    q, n = seeded((2, 4, 90, 128), 11).cuda(), ints(lens).cuda()
+    want = ops.paged_prefill(q, k, v, table, n)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = ops.paged_prefill(q, k, v, table, n)
+    streams, got = [torch.cuda.Stream() for _ in range(2)], []
+    torch.cuda.synchronize()
+    for i in range(10):
+        with torch.cuda.stream(streams[i % 2]):
+            got.append(ops.paged_prefill(q, k, v, table, n))
+            graph.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(out, want) and all(torch.equal(g, want) for g in got)
+    n.copy_(ints([95, 90]))
+    graph.replay()
+    assert torch.equal(out, ops.paged_prefill(q, k, v, table, n))
+
+
+@pytest.mark.gpu
+def test_checks_of_the_wrapper(cuda):
+    from llm_compiler_3_b200 import ops
+    k, v, table = (t.cuda() for t in paged_cache([20, 20], 2, 64, 16))
+    q, n = seeded((2, 4, 3, 64), 1).cuda(), ints([20, 20]).cuda()
+    good = dict(q=q, k_pages=k, v_pages=v, page_table=table, seq_lens=n)
+    for change in (dict(q=q.float()), dict(q=q[:, :, :, ::2]), dict(q=q[:1]), dict(q=q[:, :, 0]),
+                   dict(seq_lens=n[:1]), dict(q_lens=n[:1]), dict(q_lens=n.long()), dict(v_pages=v[:1]),
+                   dict(out=torch.empty_like(q)[:1]), dict(q_lens=n.cpu())):
+        with pytest.raises(ValueError):
+            ops.paged_prefill(**dict(good, **change))
