@@ -18,10 +18,10 @@
 // x `bm` queries, so that few queries still fill the rows and share one pass over
 // K and V.
 //   warps 0-3, 4-7  softmax of tile 0 / 1: thread r has row r (TMEM lane r)
-//   warp 8          TMA: both Q tiles, then K and V tiles of 128 keys in one ring
-//                   (K0 V0 K1 V1 ...), one box per piece of a page, each lane one
-//   warp 9          MMA issue: S_t = Q_t K^T and O_t += P_t V
-//   warps 10-11     none (a register split goes by groups of four warps)
+//   warp 8          TMA: both Q tiles, then K and V tiles in one ring (K0 V0 K1 V1
+//                   ...), one box per piece of a page, each lane one
+//   warp 9          MMA issue: O_t += P_t V, then the next S_t = Q_t K^T
+//   warp 10         clears the hidden rows of V tiles on a border
 // TMEM: S0, S1 (128 columns each), O0, O1 (D each); P_t, FP16, lies over the first
 // half of S_t.  The tensor pipe works in order, so S_t(j + 1), issued after
 // P_t(j) V, cannot overwrite weights that are still read, and its completion says
@@ -39,27 +39,24 @@ void prefill_blocking(int queries, int group, int* bm, int* hp);  // prefill_att
 
 namespace {
 
-constexpr int kKeys = 128;        // keys per tile
-constexpr int kThreads = 384;
-// Registers: 384 threads launch with 168 each; the softmax threads, which hold a
-// row of scores, take over what the other four warps do not need
-// (256 x 216 + 128 x 72 = 384 x 168).
-constexpr int kRegsLaunch = 168, kRegsSoftmax = 216, kRegsOther = 72;
-static_assert(256 * kRegsSoftmax + 128 * kRegsOther <= kThreads * kRegsLaunch, "register split");
+constexpr int KT = 128;           // keys per tile
+constexpr int kThreads = 352;
 constexpr uint32_t kTmemCols = 512;
 constexpr float kRescaleLog2 = 8.f;
 
 template <int D>
 struct PpShape {
-  static constexpr int kRegions = D / 64;             // 128-byte swizzle regions of a row
-  static constexpr int kRegionBytes = 128 * 128;      // 128 rows of one region
-  static constexpr int kTileBytes = kRegions * kRegionBytes;  // Q, K or V tile
-  static constexpr int kStages = D == 128 ? 5 : 8;    // K and V tiles in the ring
+  static constexpr int kRegions = D / 64;              // 128-byte swizzle regions of a row
+  static constexpr int kRegion = 128 * 128;            // 128 rows of one region
+  static constexpr int kTileBytes = kRegions * kRegion;  // a Q, K or V tile
+  static constexpr int kStages = D == 128 ? 5 : 10;    // K and V tiles in the ring
   static constexpr int kRing = 2 * kTileBytes;
   static constexpr int kBars = kRing + kStages * kTileBytes;
-  static constexpr int kNumBars = 1 + 2 * kStages + 6 + 1;
+  static constexpr int kNumBars = 1 + 3 * kStages + 6 + 1;
   static constexpr int kSmem = kBars + kNumBars * 8 + 16 + 1024;
+  static_assert(kSmem <= 232448, "shared memory");
 };
+constexpr int kS = 0, kO = 2 * KT;  // TMEM columns; O_t at kO + t D
 
 struct PpParams {
   const int32_t* table;
@@ -111,12 +108,17 @@ __device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
 }
 __device__ __forceinline__ float lo2(uint64_t a) { return __uint_as_float(static_cast<uint32_t>(a)); }
 __device__ __forceinline__ float hi2(uint64_t a) { return __uint_as_float(static_cast<uint32_t>(a >> 32)); }
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float d;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+  return d;
+}
 
 // What the two query tiles of a CTA cover.
 struct Span {
   int seq_len, q_len, first_pos;  // first_pos: position of query 0 of the chunk
   int lo, len, s;                 // keys that some of the CTA's queries see: [0, s) and [lo, len)
-  TileRange<kKeys> tiles;
+  TileRange<KT> tiles;
   __device__ __forceinline__ bool sees(int j) const { return j < len && (j >= lo || j < s); }
   __device__ __forceinline__ bool sees_any(int j, int n) const { return j < len && (j + n > lo || j < s); }
   __device__ __forceinline__ bool sees_all(int j, int n) const {
@@ -136,16 +138,17 @@ __global__ void __launch_bounds__(kThreads, 1)
                                              ~uintptr_t(1023));
   const uint32_t sQ = smem_u32(smem), sRing = sQ + S::kRing;
   uint64_t* q_full = reinterpret_cast<uint64_t*>(smem + S::kBars);
-  uint64_t* full = q_full + 1;         // [stages]
-  uint64_t* empty = full + kStages;    // [stages]
-  uint64_t* s_full = empty + kStages;  // [2]
-  uint64_t* p_full = s_full + 2;       // [2]
-  uint64_t* o_done = p_full + 2;       // [2]
+  uint64_t* full = q_full + 1;         // [stages] a K or V tile is there
+  uint64_t* raw = full + kStages;      // [stages] a V tile whose hidden rows are to be cleared is
+  uint64_t* empty = raw + kStages;     // [stages] the MMAs have read it
+  uint64_t* s_full = empty + kStages;  // [2] scores are there
+  uint64_t* p_full = s_full + 2;       // [2] weights are there
+  uint64_t* o_done = p_full + 2;       // [2] the last P V is done
   uint64_t* drain = o_done + 2;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(drain + 1);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
 
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
   const int group = p.q_heads / p.kv_heads, subgroups = group / p.hp;
   const int n_units = p.q_blocks * subgroups;
   const int hk = static_cast<int>(blockIdx.x) % p.kv_heads;
@@ -178,11 +181,12 @@ __global__ void __launch_bounds__(kThreads, 1)
     mbar_init(q_full, 1);
     for (int s = 0; s < kStages; ++s) {
       mbar_init(&full[s], 1);
+      mbar_init(&raw[s], 1);
       mbar_init(&empty[s], 1);
     }
     for (int t = 0; t < 2; ++t) {
       mbar_init(&s_full[t], 1);
-      mbar_init(&p_full[t], 128);
+      mbar_init(&p_full[t], 4);
       mbar_init(&o_done[t], 1);
     }
     mbar_init(drain, 1);
@@ -196,11 +200,16 @@ __global__ void __launch_bounds__(kThreads, 1)
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  const uint32_t tmem = *tmem_slot;
-  if (warp < 8)
-    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kRegsSoftmax));
-  else
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRegsOther));
+  const uint32_t tmem = __shfl_sync(0xffffffffu, *tmem_slot, 0);
+
+  // Phase of raw[x % stages] for the V tile at place x: how many border tiles used
+    // the stage before.
+  auto raw_phase = [&](int x) {
+    uint32_t n = 0;
+    for (int y = x - kStages; y > 0; y -= kStages)
+      if ((y & 1) && !span.sees_all(span.tiles.key0(y / 2), KT)) ++n;
+    return n & 1;
+  };
 
   if (warp == 8) {
     // ---------------- TMA producer ----------------
@@ -216,13 +225,13 @@ __global__ void __launch_bounds__(kThreads, 1)
           for (int g = 0; g < p.hp; ++g) {
             const int plane = b * p.q_heads + hk * group + gs * p.hp + g;
             for (int a = 0; a < S::kRegions; ++a)
-              tma_load_3d(sQ + t * S::kTileBytes + a * S::kRegionBytes + g * p.bm * 128, &qmap, q_full,
+              tma_load_3d(sQ + t * S::kTileBytes + a * S::kRegion + g * p.bm * 128, &qmap, q_full,
                           a * 64, m0, plane);
           }
         }
       }
       // Each lane loads one box: rows of one page, one 64-dim region.
-      const int combos = kKeys / p.box * S::kRegions;
+      const int combos = KT / p.box * S::kRegions;
       const int my_region = lane % S::kRegions, my_row = lane / S::kRegions * p.box;
       const bool mine = lane < combos;
       auto look_up = [&](int j) {  // the page of this lane's box of tile j; -2: nothing visible
@@ -246,107 +255,117 @@ __global__ void __launch_bounds__(kThreads, 1)
           if (x >= kStages)
             ok = __all_sync(0xffffffffu, wait_or_abort(&empty[s], ((x / kStages) - 1) & 1, abort_flag));
           if (!ok) break;
-          if (lane == 0) mbar_arrive_expect_tx(&full[s], S::kTileBytes);
+          uint64_t* bar = kv && !span.sees_all(span.tiles.key0(j), KT) ? &raw[s] : &full[s];
+          if (lane == 0) mbar_arrive_expect_tx(bar, S::kTileBytes);
           __syncwarp();
           if (mine)
-            tma_load_3d(sRing + s * S::kTileBytes + my_region * S::kRegionBytes + my_row * 128,
-                        kv ? &vmap : &kmap, &full[s], my_region * 64, row, 0);
+            tma_load_3d(sRing + s * S::kTileBytes + my_region * S::kRegion + my_row * 128,
+                        kv ? &vmap : &kmap, bar, my_region * 64, row, 0);
           issued = x + 1;
         }
       }
-      if (!ok) {  // leave no copy in flight into this CTA's shared memory
-        *abort_flag = 1;
-        mbar_wait(q_full, 0, kDevErrTmaTimeout);
-        for (int x = max(0, issued - kStages); x < issued; ++x)
-          mbar_wait(&full[x % kStages], (x / kStages) & 1, kDevErrTmaTimeout);
+      // Leave no copy in flight into this CTA's shared memory.
+      if (!ok) *abort_flag = 1;
+      mbar_wait(q_full, 0, kDevErrTmaTimeout);
+      for (int x = max(0, issued - kStages); x < issued; ++x) {
+        const int s = x % kStages;
+        const bool border = (x & 1) && !span.sees_all(span.tiles.key0(x / 2), KT);
+        mbar_wait(border ? &raw[s] : &full[s], border ? raw_phase(x) : (x / kStages) & 1, kDevErrTmaTimeout);
       }
     }
   } else if (warp == 9) {
-    // ---------------- MMA issuer (lane 0; the warp clears hidden rows of V) ----------------
-    if (n_tiles > 0) {
-      const uint32_t idesc_s = idesc_f16_f32(128, kKeys) | (p.negate ? 1u << 13 : 0u);
-      constexpr uint32_t idesc_pv = idesc_f16_f32(128, D) | kIdescBMajorMN;
-      const uint64_t dq = smem_desc_sw128(sQ), dk = smem_desc_sw128(sRing);
-      const uint64_t dv = smem_desc_sw128_mn(sRing, S::kRegionBytes, 1024);
-      auto wait = [&](uint64_t* bar, uint32_t phase) {
-        return __all_sync(0xffffffffu, lane == 0 ? spin_or_abort(bar, phase, abort_flag) : true);
-      };
-      auto issue_s = [&](int t, int x) {  // x: K's place in the ring's sequence
-        if (lane == 0) {
-          const uint64_t q = dq + (t * S::kTileBytes >> 4);
-          const uint64_t k = dk + ((x % kStages) * S::kTileBytes >> 4);
+    // ---------------- MMA issuer ----------------
+    // What timing it taught: the whole warp runs along and one elected lane issues,
+    // so that the compiler sees one value for all lanes and keeps descriptors in
+    // uniform registers (behind `lane == 0` each MMA took 92 cycles to issue, more
+    // than the 64 it runs); and little may stand between P_t's arrival and the first
+    // MMA, as instructions that run once in a thousand cycles are fetched anew each
+    // time: K and V are waited for before, and the next V's and K's places worked out.
+    const uint32_t idesc_s = idesc_f16_f32(128, KT) | (p.negate ? 1u << 13 : 0u);
+    constexpr uint32_t idesc_pv = idesc_f16_f32(128, D) | kIdescBMajorMN;
+    const uint64_t dq = smem_desc_sw128(sQ), dk = smem_desc_sw128(sRing);
+    const uint64_t dv = smem_desc_sw128_mn(sRing, S::kRegion, 1024);
+    auto wait = [&](uint64_t* bar, uint32_t phase) {
+      return __all_sync(0xffffffffu, spin_or_abort(bar, phase, abort_flag)) != 0;
+    };
+    auto issue_s = [&](int t, uint64_t k) {  // by the elected lane
+      const uint64_t q = dq + (t * S::kTileBytes >> 4);
 #pragma unroll
-          for (int kk = 0; kk < D / 16; ++kk) {
-            const uint32_t off = ((kk >> 2) * S::kRegionBytes + (kk & 3) * 32) >> 4;
-            tc_mma_f16(tmem + t * kKeys, q + off, k + off, idesc_s, kk > 0 ? 1u : 0u);
-          }
-          tc_commit(&s_full[t]);
-        }
-      };
-      auto issue_pv = [&](int t, int x, bool first) {
-        if (lane == 0) {
-          const uint64_t v = dv + ((x % kStages) * S::kTileBytes >> 4);
-#pragma unroll
-          for (int kk = 0; kk < kKeys / 16; ++kk)
-            tc_mma_f16_tmem_a(tmem + 2 * kKeys + t * 128, tmem + t * kKeys + kk * 8, v + (kk * 2048 >> 4),
-                              idesc_pv, !first || kk > 0 ? 1u : 0u);
-        }
-      };
-      bool ok = wait(q_full, 0) && wait(&full[0], 0);
-      if (ok) {
-        tc_fence_after();
-        issue_s(0, 0);
-        issue_s(1, 0);
-        if (lane == 0) tc_commit(&empty[0]);
+      for (int kk = 0; kk < D / 16; ++kk) {
+        const uint32_t off = ((kk >> 2) * S::kRegion + (kk & 3) * 32) >> 4;
+        tc_mma_f16(tmem + kS + t * KT, q + off, k + off, idesc_s, kk > 0 ? 1u : 0u);
       }
-      for (int j = 0; ok && j < n_tiles; ++j) {
-        const int xv = 2 * j + 1, xk = 2 * j + 2, sv = xv % kStages, sk = xk % kStages;
-        ok = wait(&full[sv], (xv / kStages) & 1);
+      tc_commit(&s_full[t]);
+    };
+    bool ok = n_tiles == 0 || (wait(q_full, 0) && wait(&full[0], 0));
+    if (ok && n_tiles > 0) {
+      tc_fence_after();
+      if (elect_one()) {
+        issue_s(0, dk);
+        issue_s(1, dk);
+        tc_commit(&empty[0]);
+      }
+    }
+    int sv = 1 % kStages, sk = 2 % kStages;      // stages of V(j) and K(j + 1)
+    uint32_t fv = 1 / kStages, fk = 2 / kStages;  // and their phases
+    for (int j = 0; ok && j < n_tiles; ++j) {
+      const bool more = j + 1 < n_tiles;
+      ok = wait(&full[sv], fv) && (!more || wait(&full[sk], fk));
+      if (!ok) break;
+      const uint64_t v0 = dv + (sv * S::kTileBytes >> 4), k0 = dk + (sk * S::kTileBytes >> 4);
+#pragma unroll
+      for (int t = 0; t < 2; ++t) {
+        ok = wait(&p_full[t], j & 1);
         if (!ok) break;
-        const int key0 = span.tiles.key0(j);
-        if (!span.sees_all(key0, kKeys)) {
-          // Rows that no query here sees may hold anything; their weights are 0,
-          // but 0 * NaN is NaN.
-          ok = __all_sync(0xffffffffu, wait_or_abort(&full[sv], (xv / kStages) & 1, abort_flag));
-          if (!ok) break;
-          for (int r = lane; r < kKeys; r += 32)
-            if (!span.sees(key0 + r))
-              for (int a = 0; a < S::kRegions; ++a)
-                for (int x = 0; x < 128; x += 16)
-                  *reinterpret_cast<uint4*>(smem + S::kRing + sv * S::kTileBytes + a * S::kRegionBytes +
-                                            r * 128 + x) = make_uint4(0, 0, 0, 0);
-          fence_proxy_async_smem();
-          __syncwarp();
-        }
-        for (int t = 0; t < 2; ++t) {
-          ok = wait(&p_full[t], j & 1);
-          if (!ok) break;
-          tc_fence_after();
-          issue_pv(t, xv, j == 0);
-          if (t == 1 && lane == 0) tc_commit(&empty[sv]);
-          if (j + 1 < n_tiles) {
-            if (t == 0) {
-              ok = wait(&full[sk], (xk / kStages) & 1);
-              if (!ok) break;
-              tc_fence_after();
-            }
-            issue_s(t, xk);
-            if (t == 1 && lane == 0) tc_commit(&empty[sk]);
-          } else if (lane == 0) {
+        tc_fence_after();
+        if (elect_one()) {
+#pragma unroll
+          for (int kk = 0; kk < KT / 16; ++kk)
+            tc_mma_f16_tmem_a(tmem + kO + t * D, tmem + kS + t * KT + kk * 8, v0 + (kk * 2048 >> 4),
+                              idesc_pv, j > 0 || kk > 0 ? 1u : 0u);
+          if (more)
+            issue_s(t, k0);
+          else
             tc_commit(&o_done[t]);
+          if (t == 1) {
+            tc_commit(&empty[sv]);
+            if (more) tc_commit(&empty[sk]);
           }
-        }
-      }
-      if (!ok) {  // no MMA may write TMEM after it is released
-        *abort_flag = 1;
-        if (lane == 0) {
-          tc_commit(drain);
-          mbar_wait(drain, 0, kDevErrMmaTimeout);
         }
         __syncwarp();
       }
+      sv += 2;
+      if (sv >= kStages) sv -= kStages, fv ^= 1;
+      sk += 2;
+      if (sk >= kStages) sk -= kStages, fk ^= 1;
     }
-  } else if (warp < 8) {
+    if (!ok) {  // no MMA may write TMEM after it is released
+      *abort_flag = 1;
+      if (elect_one()) {
+        tc_commit(drain);
+        mbar_wait(drain, 0, kDevErrMmaTimeout);
+      }
+      __syncwarp();
+    }
+  } else if (warp == 10) {
+    // ---------------- hidden rows of V ----------------
+    // Rows that no query here sees may hold anything; their weights are 0, but
+    // 0 * NaN is NaN.
+    for (int j = 0; j < n_tiles; ++j) {
+      const int key0 = span.tiles.key0(j), x = 2 * j + 1, s = x % kStages;
+      if (span.sees_all(key0, KT)) continue;
+      if (!__all_sync(0xffffffffu, wait_or_abort(&raw[s], raw_phase(x), abort_flag))) break;
+      for (int r = lane; r < KT; r += 32)
+        if (!span.sees(key0 + r))
+          for (int a = 0; a < S::kRegions; ++a)
+            for (int c = 0; c < 128; c += 16)
+              *reinterpret_cast<uint4*>(smem + S::kRing + s * S::kTileBytes + a * S::kRegion +
+                                        r * 128 + c) = make_uint4(0, 0, 0, 0);
+      fence_proxy_async_smem();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&full[s]);
+    }
+  } else {
     // ---------------- softmax warpgroups ----------------
     const int tt = warp >> 2, r = threadIdx.x & 127;
     const bool unit_ok = tt == 0 || has1;
@@ -358,34 +377,39 @@ __global__ void __launch_bounds__(kThreads, 1)
     const int last = row_ok && m0 + i < span.q_len ? span.first_pos + m0 + i : -1;
     const int lo = p.window > 0 ? max(0, last - p.window + 1) : 0;
     const uint32_t t_lane = tmem + (static_cast<uint32_t>((warp & 3) * 32) << 16);
-    const uint32_t t_s = t_lane + tt * kKeys, t_o = t_lane + 2 * kKeys + tt * 128;
+    const uint32_t t_s = t_lane + kS + tt * KT, t_o = t_lane + kO + tt * D;
+    auto wait = [&](uint64_t* bar, uint32_t phase) {
+      return __all_sync(0xffffffffu, wait_or_abort(bar, phase, abort_flag)) != 0;
+    };
     float m_run = -INFINITY, l_run = 0.f;
     bool ok = true;
     for (int j = 0; j < n_tiles; ++j) {
-      ok = __all_sync(0xffffffffu, wait_or_abort(&s_full[tt], j & 1, abort_flag));
+      ok = wait(&s_full[tt], j & 1);
       if (!ok) break;
       tc_fence_after();
-      uint32_t sr[kKeys];
+      uint32_t sr[KT];
 #pragma unroll
-      for (int c = 0; c < kKeys; c += 32) tmem_ld32(t_s + c, sr + c);
+      for (int c = 0; c < KT; c += 32) tmem_ld32(t_s + c, sr + c);
       tmem_ld_wait();
       const int key0 = span.tiles.key0(j);
-      if (!__all_sync(0xffffffffu, key0 + kKeys - 1 <= last && (key0 >= lo || key0 + kKeys <= p.sinks))) {
+      if (!__all_sync(0xffffffffu, key0 + KT - 1 <= last && (key0 >= lo || key0 + KT <= p.sinks))) {
 #pragma unroll
-        for (int e = 0; e < kKeys; ++e) {
+        for (int e = 0; e < KT; ++e) {
           const int key = key0 + e;
           if (key > last || (key < lo && key >= p.sinks)) sr[e] = 0xff800000u;  // -inf
         }
       }
-      float top[8];
+      float top[4];
 #pragma unroll
-      for (int e = 0; e < 8; ++e) top[e] = __uint_as_float(sr[e]);
+      for (int e = 0; e < 4; ++e) top[e] = __uint_as_float(sr[e]);
 #pragma unroll
-      for (int c = 8; c < kKeys; c += 8)
+      for (int c = 4; c < KT - 4; c += 8)
 #pragma unroll
-        for (int e = 0; e < 8; ++e) top[e] = fmaxf(top[e], __uint_as_float(sr[c + e]));
-      const float mx = fmaxf(fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])),
-                             fmaxf(fmaxf(top[4], top[5]), fmaxf(top[6], top[7])));
+        for (int e = 0; e < 4; ++e)
+          top[e] = max3(top[e], __uint_as_float(sr[c + e]), __uint_as_float(sr[c + 4 + e]));
+#pragma unroll
+      for (int e = 0; e < 4; ++e) top[e] = fmaxf(top[e], __uint_as_float(sr[KT - 4 + e]));
+      const float mx = fmaxf(max3(top[0], top[1], top[2]), top[3]);
       const float m_tile = mx * p.scale_log2;
       const bool grow = m_tile > m_run + kRescaleLog2;
       if (__any_sync(0xffffffffu, grow)) {
@@ -395,7 +419,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           l_run *= alpha;
           m_run = m_tile;
         }
-        if (j > 0) {  // rescale this warp's O rows: S_t(j) complete implies P_t(j - 1) V is
+        if (j > 0) {  // rescale this warp's O rows: with S_t(j) done, so is P_t(j - 1) V
 #pragma unroll 1
           for (int c = 0; c < D; c += 16) {
             uint32_t o[16];
@@ -411,8 +435,8 @@ __global__ void __launch_bounds__(kThreads, 1)
       const uint64_t scale2 = pack2(p.scale_log2, p.scale_log2), minus2 = pack2(-m_use, -m_use);
       uint64_t sum2[4] = {0, 0, 0, 0};
 #pragma unroll
-      for (int c = 0; c < kKeys; c += 64) {
-        uint32_t pk[32];
+      for (int c = 0; c < KT; c += 64) {
+        uint32_t pk[32];  // keys 2q, 2q + 1 in column q
 #pragma unroll
         for (int e = 0; e < 64; e += 2) {
           const uint64_t s2 = static_cast<uint64_t>(sr[c + e + 1]) << 32 | sr[c + e];
@@ -421,16 +445,16 @@ __global__ void __launch_bounds__(kThreads, 1)
           sum2[(e >> 1) & 3] = add2(sum2[(e >> 1) & 3], pack2(w0, w1));
           pk[e >> 1] = pack_half2(w0, w1);
         }
-        tmem_st32(t_s + c / 2, pk);  // keys 2q, 2q + 1 in column q
+        tmem_st32(t_s + c / 2, pk);
       }
       tmem_st_wait();
       tc_fence_before();
-      mbar_arrive(&p_full[tt]);
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&p_full[tt]);
       const uint64_t all2 = add2(add2(sum2[0], sum2[1]), add2(sum2[2], sum2[3]));
       l_run += lo2(all2) + hi2(all2);
     }
-    if (ok && n_tiles > 0)
-      ok = __all_sync(0xffffffffu, wait_or_abort(&o_done[tt], 0, abort_flag));
+    if (ok && n_tiles > 0) ok = wait(&o_done[tt], 0);
     if (!ok) {
       if (lane == 0) *abort_flag = 1;
     } else {
@@ -520,7 +544,7 @@ extern "C" int npu_b200_paged_prefill(const void* d_q, const void* d_k_pages, co
   p.queries = queries;
   p.entries = table_entries;
   p.page_size = page_size;
-  p.box = page_box(page_size, kKeys);
+  p.box = page_box(page_size, KT);
   p.num_pages = num_pages;
   const uint64_t rows = static_cast<uint64_t>(num_pages) * kv_heads * page_size;
   p.total_rows = static_cast<int>(rows);
@@ -544,5 +568,6 @@ extern "C" int npu_b200_paged_prefill(const void* d_q, const void* d_k_pages, co
   rc = make_tensor_map_3d(&vm, d_v_pages, head_dim, rows, 1, rows * head_dim * 2, p.box, 64);
   if (rc) return rc;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
-  return head_dim == 128 ? launch_pp<128>(qm, km, vm, p, batch, s) : launch_pp<64>(qm, km, vm, p, batch, s);
+  return head_dim == 128 ? launch_pp<128>(qm, km, vm, p, batch, s)
+                         : launch_pp<64>(qm, km, vm, p, batch, s);
 }
