@@ -304,7 +304,7 @@ NPU_B200_API int npu_b200_page_copy(void* d_pool, const int32_t* d_pages, const 
  *     batch x beams + beam, as npu_b200_page_update and npu_b200_beam_reorder take
  *     them.  Where no continuation is left: -inf, -1, -1
  *   d_out_done [batch, width] bytes or NULL: finished, now or before
- *   beams and width in 1..32, batch x beams <= 65535, vocab <= 2^26
+ *   beams and width in 1..32, batch x beams <= 65535, vocab <= 2^24
  *   d_workspace npu_b200_beam_select_workspace_size() bytes, 16-byte aligned, on
  *     the current device; holds nothing between calls
  * Sums over the vocabulary are FP32 per stretch and FP64 across stretches; the

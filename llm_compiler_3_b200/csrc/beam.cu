@@ -8,11 +8,13 @@
 //
 // Bound: one pass over the logits (HBM); next to it the exponentials, of which
 // an SM does 16 a clock against the ~12 FP16 logits a clock that HBM brings it.
-// So one pass does both: each warp streams a stretch of a row, 16 bytes per lane,
-// keeps per lane the running maximum and sum (rescaled once per 8 logits), and
-// holds its `width` best logits sorted across its lanes.  After the first few
-// words hardly any logit passes the warp's worst kept one, so the selection costs
-// one comparison per 8 logits.  A second, dependent launch joins the stretches.
+// So one pass does both: each warp streams its part of a row, 16 bytes per lane,
+// keeps the sum relative to its running maximum, and holds its `width` best logits
+// sorted across its lanes.  A logit is looked at only if it is a new maximum or
+// reaches a floor that `width` others are known to reach: at first the width-th
+// largest of the CTA's lanes' maxima over their first words, then the worst kept one
+// of any warp.  So maximum and selection cost one comparison per 8 logits and a few
+// insertions (with floors that each warp knew alone they cost twice the rest).  A second, dependent launch joins the stretches.
 //
 // Which of two candidates is larger decides whole beams, so what follows the
 // stretches (the sum over them, its logarithm, the candidates' worth) is in FP64;
@@ -20,6 +22,8 @@
 // some 1e-7 off.
 #include <float.h>
 #include <limits.h>
+
+#include <algorithm>
 
 #include "common.cuh"
 #include "host.hpp"
@@ -29,6 +33,8 @@ namespace {
 
 constexpr int kMaxWidth = 32;   // candidates kept: one per lane
 constexpr int kMaxBeams = 32;   // beams of a sequence: one per lane in the join
+constexpr int kMaxSplits = 128; // stretches of a row
+constexpr int kStaged = 512;    // entries of a row's lists that the join keeps in shared memory
 constexpr int kSelThreads = 256;
 constexpr int kSelWarps = kSelThreads / 32;
 constexpr float kLog2e = 1.4426950408889634f;
@@ -78,16 +84,86 @@ struct Best {
     floor = __shfl_sync(0xffffffffu, val, width - 1);
     floor_idx = __shfl_sync(0xffffffffu, idx, width - 1);
   }
-  // Each lane may offer one.
-  __device__ __forceinline__ void offer(float v, int i, bool has, int width) {
-    unsigned mask = __ballot_sync(0xffffffffu, has && takes(v, i));
+  // Each lane offers one.
+  __device__ __forceinline__ void offer(float v, int i, int width) {
+    unsigned mask = __ballot_sync(0xffffffffu, takes(v, i));
     while (mask) {
       const int src = __ffs(mask) - 1;
       put(__shfl_sync(0xffffffffu, v, src), __shfl_sync(0xffffffffu, i, src), width);
-      mask = __ballot_sync(0xffffffffu, has && takes(v, i)) & ~((2u << src) - 1);
+      mask = __ballot_sync(0xffffffffu, takes(v, i)) & ~((2u << src) - 1);
     }
   }
 };
+
+// Whole numbers in the order of the floating ones (-0 as 0).
+__device__ __forceinline__ uint32_t order_of(float v) {
+  const uint32_t b = __float_as_uint(v + 0.f);
+  return b ^ (static_cast<uint32_t>(static_cast<int32_t>(b) >> 31) | 0x80000000u);
+}
+__device__ __forceinline__ float of_order(uint32_t k) {
+  return __uint_as_float(k & 0x80000000u ? k ^ 0x80000000u : ~k);
+}
+
+// The `width` largest of the lanes' values in falling order (equal ones each):
+// lane k < width returns the k-th.
+__device__ __forceinline__ float best_of_lanes(float v, int width) {
+  const int lane = threadIdx.x & 31;
+  uint32_t k = order_of(v), mine = order_of(-INFINITY);
+  for (int i = 0; i < width; ++i) {
+    const uint32_t top = __reduce_max_sync(0xffffffffu, k);
+    const unsigned who = __ballot_sync(0xffffffffu, k == top);
+    if (lane == __ffs(who) - 1) k = 0;
+    if (lane == i) mine = top;
+  }
+  return of_order(mine);
+}
+
+// The `width` best of `lists` lists in falling order, one to a lane (list l of lane
+// l, l + 32, ...): `width` times the best head is taken.  val(l, i) and idx(l, i) are
+// read as the heads move; a list ends at -inf or at `width`.  Lane k returns the k-th.
+template <typename Val, typename Idx>
+__device__ __forceinline__ void merge_lists(int lists, int width, Val val, Idx idx, float* out_v,
+                                            int* out_i) {
+  const int lane = threadIdx.x & 31;
+  float v = -INFINITY;
+  int t = INT_MAX, from = 0;  // this lane's best head
+  int at[kMaxSplits / 32] = {};
+  auto refill = [&]() {
+    v = -INFINITY;
+    t = INT_MAX;
+#pragma unroll
+    for (int u = 0; u < kMaxSplits / 32; ++u) {
+      const int l = lane + 32 * u;
+      if (l < lists && at[u] < width) {
+        const float hv = val(l, at[u]);
+        const int hi = idx(l, at[u]);
+        if (hv > v || (hv == v && hi < t)) {
+          v = hv;
+          t = hi;
+          from = u;
+        }
+      }
+    }
+  };
+  refill();
+  *out_v = -INFINITY;
+  *out_i = INT_MAX;
+  for (int k = 0; k < width; ++k) {
+    const uint32_t key = order_of(v);
+    const uint32_t top = __reduce_max_sync(0xffffffffu, key);
+    const int low = __reduce_min_sync(0xffffffffu, key == top ? t : INT_MAX);
+    if (lane == k) {
+      *out_v = of_order(top);
+      *out_i = low;
+    }
+    if (key == top && t == low && v > -INFINITY) {
+#pragma unroll
+      for (int u = 0; u < kMaxSplits / 32; ++u)
+        if (u == from) ++at[u];
+      refill();
+    }
+  }
+}
 
 // NaN counts as -inf, +inf as the largest number of the type.
 __device__ __forceinline__ void widen(const uint4& w, float (&x)[8], const __half*) {
@@ -143,12 +219,15 @@ __device__ __forceinline__ uint4 shifted(const uint4& a, const uint4& b, int hal
 
 // Block (s, row): stretch s of row `row`, a piece per warp.
 template <typename T>
-__global__ void __launch_bounds__(kSelThreads) beam_stretch_kernel(const BeamParams p) {
+__global__ void __launch_bounds__(kSelThreads, 4) beam_stretch_kernel(const BeamParams p) {
   constexpr int L = 16 / sizeof(T);  // logits of a word
   __shared__ float s_val[kSelWarps][32], s_max[kSelWarps], s_sum[kSelWarps];
   __shared__ int s_idx[kSelWarps][32];
+  __shared__ uint32_t s_floor;  // order_of() of what `width` logits of the row reach
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const long long row = blockIdx.y;
+  if (threadIdx.x == 0) s_floor = 0;
+  __syncthreads();
   pdl_launch_dependents();
   pdl_wait();
   if (p.done != nullptr && p.done[row]) return;  // the join does not look at its stretches
@@ -161,67 +240,98 @@ __global__ void __launch_bounds__(kSelThreads) beam_stretch_kernel(const BeamPar
   const int words = (p.vocab + L - 1) / L;
   const int w_begin = min(static_cast<int>(blockIdx.x) * p.words, words);
   const int w_end = min(w_begin + p.words, words);
-  const int each = ((w_end - w_begin + kSelWarps - 1) / kSelWarps + 31) & ~31;
-  const int my_begin = min(w_begin + warp * each, w_end), my_end = min(my_begin + each, w_end);
 
   Best best;
-  float m = -FLT_MAX, sum = 0.f;
+  float m = -FLT_MAX, sum = 0.f;  // of the warp, and the lane's share
   constexpr int kAhead = 4;
-  for (int w0 = my_begin; w0 < my_end; w0 += 32 * kAhead) {
+  constexpr int kTurn = 32 * kAhead;  // words that a warp loads together
+  const int turns = (w_end - w_begin + kSelWarps * kTurn - 1) / (kSelWarps * kTurn);
+  for (int turn = 0; turn < turns; ++turn) {  // every warp takes every turn
+    const int w0 = w_begin + (turn * kSelWarps + warp) * kTurn;
+    // A turn inside the stretch, the row and the tensor needs no checks.
+    const bool inside = w0 + kTurn <= w_end && (w0 + kTurn) * L <= p.vocab;
     uint4 raw[kAhead];
+    if (inside) {
+      const uint4* src = reinterpret_cast<const uint4*>(logits) + first + w0 + lane;
 #pragma unroll
-    for (int u = 0; u < kAhead; ++u) {
-      const int w = min(w0 + u * 32 + lane, my_end - 1);
-      raw[u] = tensor_word(logits, first + w, p.total);
+      for (int u = 0; u < kAhead; ++u) raw[u] = __ldg(src + u * 32);
+    } else {
+#pragma unroll
+      for (int u = 0; u < kAhead; ++u)
+        raw[u] = tensor_word(logits, first + min(w0 + u * 32 + lane, w_end - 1), p.total);
     }
     if (lead != 0) {
 #pragma unroll
-      for (int u = 0; u < kAhead; ++u) {
-        const int w = min(w0 + u * 32 + lane, my_end - 1);
-        raw[u] = shifted(raw[u], tensor_word(logits, first + w + 1, p.total),
+      for (int u = 0; u < kAhead; ++u)
+        raw[u] = shifted(raw[u], tensor_word(logits, first + min(w0 + u * 32 + lane, w_end - 1) + 1, p.total),
                          lead * static_cast<int>(sizeof(T)) / 2);
-      }
     }
-#pragma unroll
-    for (int u = 0; u < kAhead; ++u) {
-      const int w = w0 + u * 32 + lane;
-      const int t0 = w * L;  // token of the word's first logit
-      float x[L];
+    auto logits_of = [&](int u, float(&x)[L]) {
       widen(raw[u], x, logits);
-      if (w >= my_end || t0 + L > p.vocab) {
+      if (!inside) {
+        const int n = w0 + u * 32 + lane < w_end ? p.vocab - (w0 + u * 32 + lane) * L : 0;
 #pragma unroll
         for (int i = 0; i < L; ++i)
-          if (w >= my_end || t0 + i >= p.vocab) x[i] = -INFINITY;
+          if (i >= n) x[i] = -INFINITY;
       }
-      float top = x[0];
+      float top = max3(x[0], x[1], max3(x[2], x[3], x[L - 1]));
+      if (L == 8) top = max3(top, x[4 % L], max3(x[5 % L], x[6 % L], top));
+      return top;
+    };
+    if (turn == 0) {
+      float top = -INFINITY;
 #pragma unroll
-      for (int i = 1; i < L; ++i) top = fmaxf(top, x[i]);
-      const float m_new = fmaxf(m, top);
-      float s = 0.f;
-#pragma unroll
-      for (int i = 0; i < L; ++i) s += fast_exp2((x[i] - m_new) * kLog2e);
-      sum = sum * fast_exp2((m - m_new) * kLog2e) + s;
-      m = m_new;
-      if (__any_sync(0xffffffffu, top >= best.floor && top > -INFINITY)) {
-#pragma unroll
-        for (int i = 0; i < L; ++i) best.offer(x[i], t0 + i, true, p.width);
+      for (int u = 0; u < kAhead; ++u) {
+        float x[L];
+        top = fmaxf(top, logits_of(u, x));
       }
+      m = fmaxf(m, of_order(__reduce_max_sync(0xffffffffu, order_of(top))));
+      s_val[warp][lane] = best_of_lanes(top, p.width);
+      __syncthreads();
+      if (warp == 0) {  // the warps' lists into one: its last is the first floor
+        float val;
+        int idx;
+        merge_lists(kSelWarps, p.width, [&](int l, int i) { return s_val[l][i]; },
+                    [&](int l, int) { return l; }, &val, &idx);
+        val = __shfl_sync(0xffffffffu, val, p.width - 1);
+        if (lane == 0) s_floor = order_of(val);
+      }
+      __syncthreads();
+    }
+    float floor = of_order(max(order_of(best.floor), *const_cast<volatile uint32_t*>(&s_floor)));
+#pragma unroll
+    for (int u = 0; u < kAhead; ++u) {
+      float x[L];
+      const float top = logits_of(u, x);
+      if (__any_sync(0xffffffffu, top >= floor || top > m)) {
+        const float m_new = fmaxf(m, of_order(__reduce_max_sync(0xffffffffu, order_of(top))));
+        sum *= fast_exp2((m - m_new) * kLog2e);
+        m = m_new;
+        const int t0 = (w0 + u * 32 + lane) * L;  // token of the word's first logit
+#pragma unroll
+        for (int i = 0; i < L; ++i) best.offer(x[i] >= floor ? x[i] : -INFINITY, t0 + i, p.width);
+        if (best.floor > floor) {
+          floor = best.floor;
+          if (lane == 0) atomicMax(&s_floor, order_of(floor));
+        }
+      }
+      const uint64_t minus2 = pack2(-m, -m), log2e2 = pack2(kLog2e, kLog2e);
+      uint64_t s2 = 0;
+#pragma unroll
+      for (int i = 0; i < L; i += 2) {
+        const uint64_t d2 = mul2(add2(pack2(x[i], x[i + 1]), minus2), log2e2);
+        s2 = add2(s2, pack2(fast_exp2(lo2(d2)), fast_exp2(hi2(d2))));
+      }
+      sum += lo2(s2) + hi2(s2);
     }
   }
-  // The lanes' maxima and sums, then the warps'.
-  const float m_warp = [&] {
-    float v = m;
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, o));
-    return v;
-  }();
-  sum *= fast_exp2((m - m_warp) * kLog2e);
+  // The lanes' sums, then the warps'.
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
   s_val[warp][lane] = best.val;
   s_idx[warp][lane] = best.idx;
   if (lane == 0) {
-    s_max[warp] = m_warp;
+    s_max[warp] = m;
     s_sum[warp] = sum;
   }
   __syncthreads();
@@ -231,16 +341,18 @@ __global__ void __launch_bounds__(kSelThreads) beam_stretch_kernel(const BeamPar
   for (int w = 0; w < kSelWarps; ++w) m_all = fmaxf(m_all, s_max[w]);
 #pragma unroll
   for (int w = 0; w < kSelWarps; ++w) sum_all += s_sum[w] * fast_exp2((s_max[w] - m_all) * kLog2e);
-  for (int w = 1; w < kSelWarps; ++w)
-    best.offer(s_val[w][lane], s_idx[w][lane], lane < p.width, p.width);
+  float val;
+  int idx;
+  merge_lists(kSelWarps, p.width, [&](int l, int i) { return s_val[l][i]; },
+              [&](int l, int i) { return s_idx[l][i]; }, &val, &idx);
   const long long at = row * p.splits + blockIdx.x;
   if (lane == 0) {
     p.part_max[at] = m_all;
     p.part_sum[at] = sum_all;
   }
   if (lane < p.width) {
-    p.part_val[at * p.width + lane] = best.val;
-    p.part_idx[at * p.width + lane] = best.idx;
+    p.part_val[at * p.width + lane] = val;
+    p.part_idx[at * p.width + lane] = idx;
   }
 }
 
@@ -249,6 +361,8 @@ __global__ void __launch_bounds__(kSelThreads) beam_stretch_kernel(const BeamPar
 __global__ void __launch_bounds__(kSelThreads) beam_join_kernel(const BeamParams p) {
   __shared__ double s_worth[kMaxBeams][kMaxWidth];
   __shared__ int s_token[kMaxBeams][kMaxWidth];
+  __shared__ float s_val[kSelWarps][kStaged];
+  __shared__ int s_idx[kSelWarps][kStaged];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const long long seq = blockIdx.x;
   pdl_launch_dependents();
@@ -264,7 +378,17 @@ __global__ void __launch_bounds__(kSelThreads) beam_join_kernel(const BeamParams
         token = p.eos;
       }
     } else {
-      Best best;
+      const int n = p.splits * p.width;
+      const float* val = p.part_val + row * n;
+      const int* idx = p.part_idx + row * n;
+      if (n <= kStaged) {
+        for (int i = lane; i < n; i += 32) {
+          s_val[warp][i] = val[i];
+          s_idx[warp][i] = idx[i];
+        }
+        val = s_val[warp];
+        idx = s_idx[warp];
+      }
       float m = -FLT_MAX;
       for (int s = lane; s < p.splits; s += 32) m = fmaxf(m, p.part_max[row * p.splits + s]);
 #pragma unroll
@@ -276,17 +400,12 @@ __global__ void __launch_bounds__(kSelThreads) beam_join_kernel(const BeamParams
       }
 #pragma unroll
       for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-      const int n = p.splits * p.width;
-      for (int i0 = 0; i0 < n; i0 += 32) {
-        const int i = i0 + lane;
-        const float v = i < n ? p.part_val[row * n + i] : -INFINITY;
-        const int t = i < n ? p.part_idx[row * n + i] : INT_MAX;
-        best.offer(v, t, i < n, p.width);
-      }
-      if (lane < p.width && best.val > -INFINITY) {
-        worth = ((static_cast<double>(best.val) - static_cast<double>(m)) - log(sum)) + score;
-        token = best.idx;
-      }
+      __syncwarp();
+      float best;
+      merge_lists(p.splits, p.width, [&](int l, int i) { return val[l * p.width + i]; },
+                  [&](int l, int i) { return idx[l * p.width + i]; }, &best, &token);
+      if (best > -INFINITY)
+        worth = ((static_cast<double>(best) - static_cast<double>(m)) - log(sum)) + score;
     }
     if (!(worth > -INFINITY)) worth = -INFINITY;  // NaN scores choose nothing
     s_worth[w][lane] = worth;
@@ -297,23 +416,22 @@ __global__ void __launch_bounds__(kSelThreads) beam_join_kernel(const BeamParams
   int head = 0;  // lane w: the next candidate of beam w
   for (int k = 0; k < p.width; ++k) {
     double worth = -INFINITY;
-    int beam = INT_MAX, token = INT_MAX;
+    int token = INT_MAX;
     if (lane < p.beams && head < p.width) {
       worth = s_worth[lane][head];
       token = s_token[lane][head];
-      beam = lane;
     }
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) {
-      const double ow = __shfl_xor_sync(0xffffffffu, worth, o);
-      const int ob = __shfl_xor_sync(0xffffffffu, beam, o);
-      const int ot = __shfl_xor_sync(0xffffffffu, token, o);
-      if (ow > worth || (ow == worth && ob < beam)) {
-        worth = ow;
-        beam = ob;
-        token = ot;
-      }
-    }
+    // The largest, the lowest lane (beam) among equals: FP64 in the order of whole
+    // numbers, half by half.
+    const long long bits = __double_as_longlong(worth + 0.0);
+    const unsigned long long key = bits ^ ((bits >> 63) | (1ll << 63));
+    const uint32_t high = static_cast<uint32_t>(key >> 32);
+    const uint32_t top = __reduce_max_sync(0xffffffffu, high);
+    const uint32_t low = high == top ? static_cast<uint32_t>(key) : 0u;
+    const uint32_t top_low = __reduce_max_sync(0xffffffffu, low);
+    const int beam = __ffs(__ballot_sync(0xffffffffu, high == top && low == top_low)) - 1;
+    worth = __shfl_sync(0xffffffffu, worth, beam);
+    token = __shfl_sync(0xffffffffu, token, beam);
     const bool none = worth == -INFINITY;
     if (!none && lane == beam) ++head;
     if (lane == 0) {
@@ -369,14 +487,14 @@ int launch_reorder(ReorderParams p, long long row_bytes, cudaStream_t stream) {
 }
 
 // Stretches of a row: enough CTAs to fill the SMs a few times over, none shorter
-// than one turn of its warps, none over 2^17 logits (a lane then adds at most 64
+// than half a turn of its warps, none over 2^17 logits (a lane then adds at most 64
 // words' sums in FP32).
 int beam_splits(long long rows, int vocab) {
   const long long want = (8ll * sm_count() + rows - 1) / rows;
-  const long long most = (vocab + kSelThreads * 32 - 1) / (kSelThreads * 32);
+  const long long most = (vocab + kSelThreads * 16 - 1) / (kSelThreads * 16);
   const long long least = (vocab + (1 << 17) - 1) / (1 << 17);
-  const long long s = want < most ? want : most;
-  return static_cast<int>(s < least ? least : s);
+  const long long s = std::max(std::min(want, most), least);
+  return static_cast<int>(std::min<long long>(s, kMaxSplits));
 }
 
 size_t beam_workspace(int batch, int beams, int vocab, int width) {
@@ -404,7 +522,7 @@ extern "C" int npu_b200_beam_select(const void* d_logits, int logits_f32, const 
               "beam_select: null tensor pointer");
   NPU_REQUIRE(beams >= 1 && beams <= kMaxBeams, "beam_select: beams %d not in [1, %d]", beams, kMaxBeams);
   NPU_REQUIRE(width >= 1 && width <= kMaxWidth, "beam_select: width %d not in [1, %d]", width, kMaxWidth);
-  NPU_REQUIRE(vocab >= 1 && vocab <= 1 << 26, "beam_select: vocab %d not in [1, 2^26]", vocab);
+  NPU_REQUIRE(vocab >= 1 && vocab <= 1 << 24, "beam_select: vocab %d not in [1, 2^24]", vocab);
   NPU_REQUIRE(batch >= 1 && static_cast<long long>(batch) * beams <= 65535,
               "beam_select: batch %d x beams %d not in [1, 65535]", batch, beams);
   NPU_REQUIRE(eos >= -1 && eos < vocab, "beam_select: end token %d not in [-1, %d)", eos, vocab);

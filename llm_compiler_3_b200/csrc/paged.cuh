@@ -30,6 +30,20 @@ struct TileRange {
   __device__ __forceinline__ int key0(int i) const { return (i < n_sink ? i : w0 + i - n_sink) * T; }
 };
 
+// Quotients by a number known at launch, d in [2, 2^31): with 2^l >= d > 2^(l-1) and
+// m = floor(2^(31+l) / d) + 1, n / d = (n m) >> (31 + l) for every n < 2^31.
+struct Divisor {
+  uint32_t m, shift;
+  static Divisor of(uint32_t d) {
+    uint32_t l = 1;
+    while ((1ull << l) < d) ++l;
+    return {static_cast<uint32_t>((1ull << (31 + l)) / d + 1), l - 1};
+  }
+  __device__ __forceinline__ int quotient(int n) const {
+    return static_cast<int>(__umulhi(static_cast<uint32_t>(n), m) >> shift);
+  }
+};
+
 // Rows of the largest TMA box that never crosses a page: the largest power of
 // two that divides P, at most `tile`.
 inline int page_box(int page_size, int tile) {

@@ -26,6 +26,9 @@
 // query heads as the N columns: one pass over K and V serves the whole group.
 #include <math.h>
 
+#include <algorithm>
+#include <type_traits>
+
 #include "paged.cuh"
 
 namespace npu_b200 {
@@ -34,6 +37,7 @@ namespace {
 constexpr int kTile = 32;   // keys per warp stage
 constexpr int kWarps = 4;
 constexpr int kMinTiles = 4;  // of a CTA's stretch: one per warp
+constexpr float kRescaleLog2 = 8.f;
 
 template <int D, int NB>
 struct PdShape {
@@ -59,6 +63,7 @@ struct PdParams {
   int batch, q_heads, kv_heads, group, chunks;  // chunks: blocks of 8 NB query heads per KV head
   int entries, page_size, box, num_pages, total_rows;
   int window, sinks, pitch;
+  Divisor by_page;
   float scale_log2;
 };
 
@@ -83,22 +88,47 @@ struct Keys {
   }
 };
 
-// A place in the line of tiles: tile i of unit u of sequence b.
+// A place in the line of tiles: tile i of (sequence b, KV head h, block c of its
+// query heads).
 struct Place {
-  int b, u, i;
+  int b, h, c, i;
   Keys keys;
-  __device__ __forceinline__ void forward(const PdParams& p, int step, int units) {
+  __device__ __forceinline__ void forward(const PdParams& p, int step) {
     i += step;
     while (i >= keys.tiles.n) {
       i -= keys.tiles.n;
-      if (++u == units) {
-        u = 0;
-        if (++b >= p.batch) return;
-        keys.set(p, b);
-      }
+      if (++c < p.chunks) continue;
+      c = 0;
+      if (++h < p.kv_heads) continue;
+      h = 0;
+      if (++b >= p.batch) return;
+      keys.set(p, b);
     }
   }
 };
+
+// ldmatrix at a constant distance from an address.
+template <int OFF>
+__device__ __forceinline__ void ldmatrix_x4_at(uint32_t (&r)[4], uint32_t addr) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4 + %5];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+               : "r"(addr), "n"(OFF));
+}
+template <int OFF>
+__device__ __forceinline__ void ldmatrix_x4_trans_at(uint32_t (&r)[4], uint32_t addr) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0, %1, %2, %3}, [%4 + %5];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+               : "r"(addr), "n"(OFF));
+}
+
+// A loop whose index is a constant in its body.
+template <int N, int I = 0, typename F>
+__device__ __forceinline__ void unrolled(F&& f) {
+  if constexpr (I < N) {
+    f(std::integral_constant<int, I>{});
+    unrolled<N, I + 1>(f);
+  }
+}
 
 template <int D, int NB>
 __global__ void __launch_bounds__(kWarps * 32, 1)
@@ -182,8 +212,10 @@ __global__ void __launch_bounds__(kWarps * 32, 1)
   at.keys.set(p, at.b);
   {
     const long long rem = t0 - s_base;
-    at.u = static_cast<int>(rem / at.keys.tiles.n);
-    at.i = static_cast<int>(rem - static_cast<long long>(at.u) * at.keys.tiles.n);
+    const int unit = static_cast<int>(rem / at.keys.tiles.n);
+    at.i = static_cast<int>(rem - static_cast<long long>(unit) * at.keys.tiles.n);
+    at.h = unit / p.chunks;
+    at.c = unit - at.h * p.chunks;
   }
   const int n_mine = static_cast<int>(t1 - t0);
   const int my_tiles = n_mine > warp ? (n_mine - warp + kWarps - 1) / kWarps : 0;
@@ -194,45 +226,59 @@ __global__ void __launch_bounds__(kWarps * 32, 1)
   const int my_box = lane / (S::kRegions * 2), my_region = (lane >> 1) % S::kRegions;
   const bool my_v = lane & 1;
   Place ahead = at;
-  ahead.forward(p, warp, units);
-  int page = -1;  // of this lane's box of the tile at `ahead`; -2: no visible key in it
+  ahead.forward(p, warp);
+  // This lane's box of the tile at `ahead`: its page (-2: no visible key in it), and
+  // its row from the page's first.
+  int page = -2, row_in_page = 0;
+  const int page_rows = p.kv_heads * p.page_size;
   auto look_up = [&]() {
-    if (lane >= combos || ahead.b >= p.batch) return;
     const int j = ahead.keys.tiles.key0(ahead.i) + my_box * p.box;
-    page = ahead.keys.sees_any(j, p.box)
-               ? p.table[static_cast<size_t>(ahead.b) * p.entries + j / p.page_size]
-               : -2;
+    const int entry = p.by_page.quotient(j);
+    row_in_page = ahead.h * p.page_size + j - entry * p.page_size;
+    page = -2;
+    if (lane < combos && ahead.keys.sees_any(j, p.box))
+      page = p.table[static_cast<size_t>(ahead.b) * p.entries + entry];
   };
-  auto issue = [&](int k) {
-    const int st = k % S::kStages;
+  auto issue = [&](int k, int st) {
     if (lane == 0) mbar_arrive_expect_tx(&my_bars[st], S::kStageBytes);
     __syncwarp();
     if (lane < combos) {
-      const int j = ahead.keys.tiles.key0(ahead.i) + my_box * p.box;
       int row = p.total_rows;  // past the pool: the box is filled with zeros
       if (page >= 0 && page < p.num_pages)
-        row = (page * p.kv_heads + ahead.u / p.chunks) * p.page_size + j % p.page_size;
+        row = page * page_rows + row_in_page;
       else if (page != -2)
         report_error(kDevErrBounds);
       uint8_t* dst = my_stages + st * S::kStageBytes + (my_v ? S::kTileBytes : 0) +
                      my_region * S::kRegionBytes + my_box * p.box * 128;
       tma_load_2d(dst, my_v ? &vmap : &kmap, &my_bars[st], my_region * 64, row);
     }
-    ahead.forward(p, kWarps, units);
-    if (k + 1 < my_tiles) look_up();
+    if (k + 1 < my_tiles) {
+      ahead.forward(p, kWarps);
+      look_up();
+    }
   };
   if (my_tiles > 0) look_up();
   int issued = 0;
-  for (; issued < my_tiles && issued < S::kStages; ++issued) issue(issued);
+  for (; issued < my_tiles && issued < S::kStages; ++issued) issue(issued, issued);
+
+  // This lane's part of the ldmatrix addresses: chunk x of row r lies at x ^ (r % 8).
+  uint32_t k_at[4], v_at[4];
+#pragma unroll
+  for (int x = 0; x < 4; ++x) {
+    const int k_row = lane & 15, v_row = (lane & 7) + ((lane >> 4) << 3);
+    k_at[x] = k_row * 128 + (((2 * x + (lane >> 4)) ^ (k_row & 7)) << 4);
+    v_at[x] = v_row * 128 + (((2 * x + ((lane >> 3) & 1)) ^ (v_row & 7)) << 4);
+  }
 
   // ---- the stretch, unit by unit ----
-  int k = 0;  // this warp's next tile
+  int k = 0;  // this warp's next tile, in stage `st` at its `phase`-th turn
+  int st = 0;
+  uint32_t phase = 0;
   bool bad = false;
   for (int done = 0; done < n_mine;) {
     const int here = min(at.keys.tiles.n - at.i, n_mine - done);  // tiles of this unit
-    const int h = at.u / p.chunks, chunk = at.u - h * p.chunks;
-    const int heads = min(S::kHeads, p.group - chunk * S::kHeads);
-    const size_t q_row = static_cast<size_t>(at.b) * p.q_heads + h * p.group + chunk * S::kHeads;
+    const int heads = min(S::kHeads, p.group - at.c * S::kHeads);
+    const size_t q_row = static_cast<size_t>(at.b) * p.q_heads + at.h * p.group + at.c * S::kHeads;
 
     // Q^T fragments: column n = query head n of the block, zero past it.
     uint32_t qf[NB][KSTEPS][2];
@@ -256,15 +302,14 @@ __global__ void __launch_bounds__(kWarps * 32, 1)
     }
 
     for (; !bad && k * kWarps + warp < done + here; ++k) {
-      const int st = k % S::kStages;
-      if (!mbar_wait(&my_bars[st], (k / S::kStages) & 1, kDevErrTmaTimeout)) {
+      if (!mbar_wait(&my_bars[st], phase, kDevErrTmaTimeout)) {
         bad = true;
         break;
       }
       const int key0 = at.keys.tiles.key0(at.i + k * kWarps + warp - done);
       const bool whole = at.keys.sees_all(key0, kTile);
       uint8_t* kst = my_stages + st * S::kStageBytes;
-      const uint32_t kbase = smem_u32(kst), vbase = smem_u32(kst + S::kTileBytes);
+      const uint32_t kbase = smem_u32(kst), vbase = kbase + S::kTileBytes;
       if (!whole) {
         // A hidden row may hold anything; its weight is 0, but 0 * NaN is NaN.
         if (!at.keys.sees(key0 + lane)) {
@@ -278,49 +323,63 @@ __global__ void __launch_bounds__(kWarps * 32, 1)
       }
 
       // scores S^T[key, head] of two 16-key blocks
-      float sv[2][NB][4];
-#pragma unroll
-      for (int mt = 0; mt < 2; ++mt) {
-#pragma unroll
-        for (int nb = 0; nb < NB; ++nb) sv[mt][nb][0] = sv[mt][nb][1] = sv[mt][nb][2] = sv[mt][nb][3] = 0.f;
-        const int row = mt * 16 + (lane & 15);
-#pragma unroll
-        for (int s = 0; s < KSTEPS; ++s) {
-          const int ch = 2 * s + (lane >> 4);
-          uint32_t a0, a1, a2, a3;
-          ldmatrix_x4(a0, a1, a2, a3,
-                      kbase + (ch >> 3) * S::kRegionBytes + row * 128 + (((ch & 7) ^ (row & 7)) << 4));
+      float sv[2][NB][4] = {};
+      unrolled<2>([&](auto mt) {
+        unrolled<KSTEPS>([&](auto s) {
+          uint32_t a[4];
+          ldmatrix_x4_at<(s / 4) * S::kRegionBytes + mt * 2048>(a, kbase + k_at[s % 4]);
 #pragma unroll
           for (int nb = 0; nb < NB; ++nb)
-            mma_16816(sv[mt][nb], a0, a1, a2, a3, qf[nb][s][0], qf[nb][s][1]);
-        }
-      }
-      // online softmax, in the base-2 logarithm's domain
-      uint32_t pb[2][NB][2];
+            mma_16816(sv[mt][nb], a[0], a[1], a[2], a[3], qf[nb][s][0], qf[nb][s][1]);
+        });
+      });
+      // Online softmax, in the base-2 logarithm's domain.  A column's maximum moves only
+      // when a score exceeds it by 2^8 (weights stay below 256, exact enough in FP16):
+      // then, and only then, the lanes of a column compare notes and O is rescaled.
+      bool grows = false;
 #pragma unroll
-      for (int nb = 0; nb < NB; ++nb) {
-        float top[2] = {-INFINITY, -INFINITY};
+      for (int mt = 0; mt < 2; ++mt)
 #pragma unroll
-        for (int mt = 0; mt < 2; ++mt)
+        for (int nb = 0; nb < NB; ++nb)
 #pragma unroll
           for (int r = 0; r < 4; ++r) {
             float v = sv[mt][nb][r] * p.scale_log2;
             if (!whole && !at.keys.sees(key0 + mt * 16 + g + ((r & 2) ? 8 : 0))) v = -INFINITY;
             sv[mt][nb][r] = v;
-            top[r & 1] = fmaxf(top[r & 1], v);
+            grows |= v > m_run[nb][r & 1] + kRescaleLog2;
           }
-        float m_use[2], alpha[2];
+      if (__any_sync(0xffffffffu, grows)) {
 #pragma unroll
-        for (int j = 0; j < 2; ++j) {
-          top[j] = fmaxf(top[j], __shfl_xor_sync(0xffffffffu, top[j], 4));
-          top[j] = fmaxf(top[j], __shfl_xor_sync(0xffffffffu, top[j], 8));
-          top[j] = fmaxf(top[j], __shfl_xor_sync(0xffffffffu, top[j], 16));
-          const float m_new = fmaxf(m_run[nb][j], top[j]);
-          m_use[j] = m_new == -INFINITY ? 0.f : m_new;
-          alpha[j] = fast_exp2(m_run[nb][j] - m_use[j]);
-          m_run[nb][j] = m_new;
-          l_run[nb][j] *= alpha[j];
+        for (int nb = 0; nb < NB; ++nb) {
+          float alpha[2];
+#pragma unroll
+          for (int j = 0; j < 2; ++j) {
+            float top = fmaxf(fmaxf(sv[0][nb][j], sv[0][nb][2 + j]), fmaxf(sv[1][nb][j], sv[1][nb][2 + j]));
+            top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 4));
+            top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 8));
+            top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 16));
+            alpha[j] = 1.f;
+            if (top > m_run[nb][j] + kRescaleLog2) {
+              alpha[j] = m_run[nb][j] == -INFINITY ? 0.f : fast_exp2(m_run[nb][j] - top);
+              m_run[nb][j] = top;
+              l_run[nb][j] *= alpha[j];
+            }
+          }
+#pragma unroll
+          for (int d = 0; d < DBLK; ++d) {
+            o[nb][d][0] *= alpha[0];
+            o[nb][d][1] *= alpha[1];
+            o[nb][d][2] *= alpha[0];
+            o[nb][d][3] *= alpha[1];
+          }
         }
+      }
+      uint32_t pb[2][NB][2];
+#pragma unroll
+      for (int nb = 0; nb < NB; ++nb) {
+        float m_use[2];  // no key seen yet: all scores are -inf
+#pragma unroll
+        for (int j = 0; j < 2; ++j) m_use[j] = m_run[nb][j] == -INFINITY ? 0.f : m_run[nb][j];
 #pragma unroll
         for (int mt = 0; mt < 2; ++mt) {
           float w[4];
@@ -332,34 +391,25 @@ __global__ void __launch_bounds__(kWarps * 32, 1)
           pb[mt][nb][0] = movmatrix_trans(pack_half2(w[0], w[1]));
           pb[mt][nb][1] = movmatrix_trans(pack_half2(w[2], w[3]));
         }
-#pragma unroll
-        for (int d = 0; d < DBLK; ++d) {
-          o[nb][d][0] *= alpha[0];
-          o[nb][d][1] *= alpha[1];
-          o[nb][d][2] *= alpha[0];
-          o[nb][d][3] *= alpha[1];
-        }
       }
       // O^T[dim, head] += V^T P^T
-#pragma unroll
-      for (int mt = 0; mt < 2; ++mt) {
-        const int q4 = lane >> 3;
-        const int row = mt * 16 + (lane & 7) + ((q4 >> 1) << 3);
-#pragma unroll
-        for (int d = 0; d < DBLK; ++d) {
-          const int ch = 2 * d + (q4 & 1);
-          uint32_t a0, a1, a2, a3;
-          ldmatrix_x4_trans(a0, a1, a2, a3,
-                            vbase + (ch >> 3) * S::kRegionBytes + row * 128 + (((ch & 7) ^ (row & 7)) << 4));
+      unrolled<2>([&](auto mt) {
+        unrolled<DBLK>([&](auto d) {
+          uint32_t a[4];
+          ldmatrix_x4_trans_at<(d / 4) * S::kRegionBytes + mt * 2048>(a, vbase + v_at[d % 4]);
 #pragma unroll
           for (int nb = 0; nb < NB; ++nb)
-            mma_16816(o[nb][d], a0, a1, a2, a3, pb[mt][nb][0], pb[mt][nb][1]);
-        }
-      }
+            mma_16816(o[nb][d], a[0], a[1], a[2], a[3], pb[mt][nb][0], pb[mt][nb][1]);
+        });
+      });
       __syncwarp();
       if (issued < my_tiles) {
         fence_proxy_async_smem();  // this stage's reads and zero-fill precede the next TMA write
-        issue(issued++);
+        issue(issued++, st);
+      }
+      if (++st == S::kStages) {
+        st = 0;
+        phase ^= 1;
       }
     }
 
@@ -435,7 +485,7 @@ __global__ void __launch_bounds__(kWarps * 32, 1)
       p.joins[blockIdx.x] = make_int4(1 + others, static_cast<int>(q_row), heads, done == 0 ? 0 : 1);
     }
     done += here;
-    at.forward(p, here, units);
+    at.forward(p, here);
     __syncthreads();  // the join buffer is free again
   }
   if (bad) {  // leave no copy in flight into this CTA's shared memory
@@ -563,6 +613,7 @@ extern "C" int npu_b200_paged_decode(const void* d_q, const void* d_k_pages, con
   p.chunks = (p.group + heads - 1) / heads;
   p.entries = table_entries;
   p.page_size = page_size;
+  p.by_page = Divisor::of(page_size);
   p.box = box;
   p.num_pages = num_pages;
   p.total_rows = static_cast<int>(rows);

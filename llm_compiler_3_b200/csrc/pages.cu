@@ -25,34 +25,35 @@ constexpr int kAtOnce = 4;      // groups of 32 pages whose counts a warp loads 
 // Exclusive prefix of `v` over the CTA's threads and the CTA's total.
 __device__ __forceinline__ long long block_scan(long long v, long long* s_warp, long long* total) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  long long x = v;
+  auto inclusive = [&](long long x) {
 #pragma unroll
-  for (int o = 1; o < 32; o <<= 1) {
-    const long long y = __shfl_up_sync(0xffffffffu, x, o);
-    if (lane >= o) x += y;
-  }
-  __syncthreads();
+    for (int o = 1; o < 32; o <<= 1) {
+      const long long y = __shfl_up_sync(0xffffffffu, x, o);
+      if (lane >= o) x += y;
+    }
+    return x;
+  };
+  const long long x = inclusive(v);
   if (lane == 31) s_warp[warp] = x;
   __syncthreads();
-  long long before = 0, all = 0;
-  for (int w = 0; w < kWarpsPerCta; ++w) {
-    const long long y = s_warp[w];
-    if (w < warp) before += y;
-    all += y;
-  }
-  *total = all;
-  return before + x - v;
+  const long long upto = inclusive(s_warp[lane]);  // every warp scans the 32 warps' sums
+  *total = __shfl_sync(0xffffffffu, upto, 31);
+  return x - v + (warp > 0 ? __shfl_sync(0xffffffffu, upto, warp - 1) : 0);
 }
 
-// Sum over the CTA's threads (whole in every thread).
+// Sum over the CTA's warps of `v`, one value per warp; in every thread.  s_warp keeps
+// the warps' values.
 __device__ __forceinline__ int block_sum(int v, int* s_warp) {
-  v = __reduce_add_sync(0xffffffffu, v);
+  const int lane = threadIdx.x & 31;
+  if (lane == 0) s_warp[threadIdx.x >> 5] = v;
   __syncthreads();
-  if ((threadIdx.x & 31) == 0) s_warp[threadIdx.x >> 5] = v;
-  __syncthreads();
-  int all = 0;
-  for (int w = 0; w < kWarpsPerCta; ++w) all += s_warp[w];
-  return all;
+  return __reduce_add_sync(0xffffffffu, s_warp[lane]);
+}
+
+// Sum of the values of the warps before this one.
+__device__ __forceinline__ int warps_before(const int* s_warp) {
+  const int lane = threadIdx.x & 31;
+  return __reduce_add_sync(0xffffffffu, lane < static_cast<int>(threadIdx.x >> 5) ? s_warp[lane] : 0);
 }
 
 // Every CTA's `mine` into s_all[kCtas] of every CTA (needs a cluster barrier
@@ -85,24 +86,13 @@ struct UpdateParams {
   int rows, new_rows, entries, page_size, num_pages;
 };
 
-// One new row: what it keeps of its parent.
+// One new row, in shared memory: what it keeps of its parent.
 struct Row {
-  int parent, len, full, part, held, last;  // last: the partial page, or -1
-  __device__ __forceinline__ Row(const UpdateParams& p, int b) {
-    const int reach = p.entries * p.page_size;
-    parent = p.parents[b];
-    if (parent < 0 || parent >= p.rows) parent = -1;
-    len = parent < 0 ? 0 : min(max(p.lens[parent], 0), reach);
-    const int cap = max(min(max(p.capacity[b], 0), reach), len);
-    full = len / p.page_size;
-    part = len - full * p.page_size;
-    held = (cap + p.page_size - 1) / p.page_size;
-    last = -1;
-    if (part > 0) {
-      last = p.table[static_cast<size_t>(parent) * p.entries + full];
-      if (last < 0 || last >= p.num_pages) last = -1;
-    }
-  }
+  int parent;  // or -1
+  int len;     // tokens
+  int last;    // the partly filled page, or -1
+  int need;    // fresh pages of the rows before
+  int copy;    // 2 x the copying rows before, + 1 if this one copies its last page
 };
 
 // Grid: one cluster.  Phases, a cluster barrier after each of the first three:
@@ -113,14 +103,14 @@ struct Row {
 //   4. the k-th free page goes to the k-th need
 __global__ void __launch_bounds__(kThreads) page_update_kernel(const UpdateParams p) {
   extern __shared__ int32_t smem_i[];
-  int32_t* first = smem_i;                   // [rows] lowest new row of each old one
-  int32_t* need = first + p.rows;            // [new_rows + 1] fresh pages of the rows before
-  int32_t* copy = need + p.new_rows + 1;     // [new_rows] 2 x copying rows before, + 1 if this copies
+  int32_t* first = smem_i;                             // [rows] lowest new row of each old one
+  Row* row = reinterpret_cast<Row*>(first + p.rows);   // [new_rows]
   __shared__ long long s_scan[kWarpsPerCta];
-  __shared__ int s_sum[kWarpsPerCta], s_free[kCtas], s_warp_free[kWarpsPerCta], s_copies;
+  __shared__ int s_sum[kWarpsPerCta], s_free[kCtas], s_copies;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int rank = static_cast<int>(cluster_ctarank());
   const int all_threads = kCtas * kThreads, me = rank * kThreads + tid;
+  const int reach = p.entries * p.page_size;
   pdl_launch_dependents();
   pdl_wait();
 
@@ -128,31 +118,49 @@ __global__ void __launch_bounds__(kThreads) page_update_kernel(const UpdateParam
   for (int r = tid; r < p.rows; r += kThreads) first[r] = INT_MAX;
   if (tid == 0) s_copies = 0;
   __syncthreads();
-  for (int b = tid; b < p.new_rows; b += kThreads) {
-    const int parent = p.parents[b];
-    if (parent >= 0 && parent < p.rows) atomicMin(&first[parent], b);
+  const int each = (p.new_rows + kThreads - 1) / kThreads;
+  const int b0 = min(tid * each, p.new_rows), b1 = min(b0 + each, p.new_rows);
+  for (int b = b0; b < b1; ++b) {
+    Row r;
+    r.parent = p.parents[b];
+    const int cap = min(max(p.capacity[b], 0), reach);
+    r.len = 0;
+    r.last = -1;
+    r.copy = 0;
+    if (r.parent >= 0 && r.parent < p.rows) {
+      atomicMin(&first[r.parent], b);
+      r.len = min(max(p.lens[r.parent], 0), reach);
+    } else {
+      r.parent = -1;
+    }
+    const int full = r.len / p.page_size, part = r.len - full * p.page_size;
+    if (part > 0) {
+      r.last = p.table[static_cast<size_t>(r.parent) * p.entries + full];
+      if (r.last >= 0 && r.last < p.num_pages)
+        r.copy = p.refs[r.last] != 1;  // held elsewhere too
+      else
+        r.last = -1;
+    }
+    r.need = (max(cap, r.len) + p.page_size - 1) / p.page_size - full - (part > 0);
+    row[b] = r;
   }
   __syncthreads();
-  {
-    const int each = (p.new_rows + kThreads - 1) / kThreads;
-    const int b0 = min(tid * each, p.new_rows), b1 = min(b0 + each, p.new_rows);
-    long long mine = 0;  // needs, and copying rows in the upper half
-    auto of_row = [&](int b) {
-      const Row r(p, b);
-      const bool copies = r.last >= 0 && !(first[r.parent] == b && p.refs[r.last] == 1);
-      return static_cast<long long>(r.held - r.full - (r.part > 0) + copies) |
-             (copies ? 1ll << 32 : 0ll);
-    };
-    for (int b = b0; b < b1; ++b) mine += of_row(b);
-    long long total, at = block_scan(mine, s_scan, &total);
-    for (int b = b0; b < b1; ++b) {
-      const long long n = of_row(b);
-      need[b] = static_cast<int>(at & 0xffffffffll);
-      copy[b] = static_cast<int>(at >> 32) * 2 + static_cast<int>(n >> 32);
-      at += n;
-    }
-    if (tid == 0) need[p.new_rows] = static_cast<int>(total & 0xffffffffll);
+  long long mine = 0;  // needs, and copying rows in the upper half
+  for (int b = b0; b < b1; ++b) {
+    Row& r = row[b];
+    if (r.last >= 0 && first[r.parent] != b) r.copy = 1;
+    r.need += r.copy;
+    mine += static_cast<long long>(r.copy) << 32 | r.need;
   }
+  long long total, at_row = block_scan(mine, s_scan, &total);
+  for (int b = b0; b < b1; ++b) {
+    Row& r = row[b];
+    const long long n = static_cast<long long>(r.copy) << 32 | r.need;
+    r.need = static_cast<int>(at_row & 0xffffffffll);
+    r.copy |= static_cast<int>(at_row >> 32) * 2;
+    at_row += n;
+  }
+  const int wanted = static_cast<int>(total & 0xffffffffll);
   cluster_sync_all();
 
   // One warp per piece of a row, so that few long rows spread over the cluster too.
@@ -170,12 +178,13 @@ __global__ void __launch_bounds__(kThreads) page_update_kernel(const UpdateParam
   for (long long w = my_warp; w < p.new_rows * pieces; w += warps) {
     const int b = static_cast<int>(w / pieces);
     const int e0 = static_cast<int>(w - b * pieces) * kRowPiece;
-    const Row r(p, b);
-    const bool keeps = r.last >= 0 && !(copy[b] & 1);
+    const Row r = row[b];
+    const int full = r.len / p.page_size;
+    const bool keeps = r.last >= 0 && !(r.copy & 1);
 #pragma unroll 4
     for (int e = e0 + lane; e < min(e0 + kRowPiece, p.entries); e += 32) {
       int page = -1;
-      if (e < r.full || (e == r.full && keeps)) {
+      if (e < full || (e == full && keeps)) {
         page = p.table[static_cast<size_t>(r.parent) * p.entries + e];
         if (page < 0 || page >= p.num_pages) page = -1;
         if (page >= 0) atomicAdd(&p.new_refs[page], 1);
@@ -194,10 +203,7 @@ __global__ void __launch_bounds__(kThreads) page_update_kernel(const UpdateParam
     if (n < 0) p.new_refs[i] = 0;
     free_here += n <= 0;
   }
-  free_here = __reduce_add_sync(0xffffffffu, free_here);
-  if (lane == 0) s_warp_free[warp] = free_here;
-  const int cta_free = block_sum(lane == 0 ? free_here : 0, s_sum);
-  cluster_share(cta_free, s_free);
+  cluster_share(block_sum(__reduce_add_sync(0xffffffffu, free_here), s_sum), s_free);
   cluster_sync_all();
 
   int at = 0, n_free = 0;
@@ -205,8 +211,7 @@ __global__ void __launch_bounds__(kThreads) page_update_kernel(const UpdateParam
     if (c < rank) at += s_free[c];
     n_free += s_free[c];
   }
-  for (int w = 0; w < warp; ++w) at += s_warp_free[w];
-  const int wanted = need[p.new_rows];
+  at += warps_before(s_sum);
   for (int i0 = pages.begin; i0 < pages.end && at < wanted; i0 += 32 * kAtOnce) {
     int refs[kAtOnce];
 #pragma unroll
@@ -221,26 +226,26 @@ __global__ void __launch_bounds__(kThreads) page_update_kernel(const UpdateParam
       const int k = at + __popc(mask & ((1u << lane) - 1));
       at += __popc(mask);
       if (!free || k >= wanted) continue;
-      int lo = 0, hi = p.new_rows;  // the row b with need[b] <= k < need[b + 1]
+      int lo = 0, hi = p.new_rows;  // the last row b with need <= k
       while (hi - lo > 1) {
         const int mid = (lo + hi) >> 1;
-        if (need[mid] <= k) lo = mid; else hi = mid;
+        if (row[mid].need <= k) lo = mid; else hi = mid;
       }
-      const Row r(p, lo);
-      const bool copies = copy[lo] & 1;
-      const int j = k - need[lo];
-      const int e = r.full + j + (r.part > 0 && !copies);
+      const Row r = row[lo];
+      const bool copies = r.copy & 1;
+      const int j = k - r.need, full = r.len / p.page_size;
+      const int e = full + j + (r.len > full * p.page_size && !copies);
       p.new_table[static_cast<size_t>(lo) * p.entries + e] = page;
       p.new_refs[page] = 1;
       if (copies && j == 0) {
-        p.copies[copy[lo] >> 1] = r.last;
-        p.copies[p.new_rows + (copy[lo] >> 1)] = page;
+        p.copies[r.copy >> 1] = r.last;
+        p.copies[p.new_rows + (r.copy >> 1)] = page;
       }
     }
   }
   if (rank == 0) {  // the rows whose copy got its page are the first ones that copy
     for (int b = tid; b < p.new_rows; b += kThreads)
-      if ((copy[b] & 1) && need[b] < n_free) atomicMax(&s_copies, (copy[b] >> 1) + 1);
+      if ((row[b].copy & 1) && row[b].need < n_free) atomicMax(&s_copies, (row[b].copy >> 1) + 1);
     __syncthreads();
     for (int i = s_copies + tid; i < p.new_rows; i += kThreads)
       p.copies[i] = p.copies[p.new_rows + i] = -1;
@@ -273,20 +278,18 @@ __global__ void __launch_bounds__(kThreads) page_compact_kernel(const CompactPar
 
   int mine = 0;
   for (int i = pages.begin + lane; i < pages.end; i += 32) mine += p.refs[i] > 0;
-  mine = __reduce_add_sync(0xffffffffu, mine);
-  if (lane == 0) s_warp[warp] = mine;
-  cluster_share(block_sum(lane == 0 ? mine : 0, s_sum), s_live);
+  cluster_share(block_sum(__reduce_add_sync(0xffffffffu, mine), s_warp), s_live);
   cluster_sync_all();
   int at = 0, n = 0;  // live pages before this warp's, and all
   for (int c = 0; c < kCtas; ++c) {
     if (c < rank) at += s_live[c];
     n += s_live[c];
   }
-  for (int w = 0; w < warp; ++w) at += s_warp[w];
+  at += warps_before(s_warp);
 
   int low = 0;  // live pages below n
   for (int i = pages.begin + lane; i < min(pages.end, n); i += 32) low += p.refs[i] > 0;
-  cluster_share(block_sum(low, s_sum), s_low);
+  cluster_share(block_sum(__reduce_add_sync(0xffffffffu, low), s_sum), s_low);
   cluster_sync_all();
   low = 0;
   for (int c = 0; c < kCtas; ++c) low += s_low[c];
@@ -425,9 +428,9 @@ extern "C" int npu_b200_page_update(const int32_t* d_page_table, const int32_t* 
   UpdateParams p = {d_page_table, d_seq_lens, d_parents, d_capacity, d_page_refs,
                     d_new_table, d_new_lens, d_new_refs, d_copies, d_info,
                     rows, new_rows, table_entries, page_size, num_pages};
-  const size_t smem = (static_cast<size_t>(rows) + 2 * static_cast<size_t>(new_rows) + 1) * 4;
+  const size_t smem = static_cast<size_t>(rows) * 4 + static_cast<size_t>(new_rows) * sizeof(Row);
   NPU_TRY_CUDA(cudaFuncSetAttribute(page_update_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                    (3 * kMaxRows + 1) * 4));
+                                    kMaxRows * static_cast<int>(4 + sizeof(Row))));
   LaunchCfg cfg;
   cfg.grid = dim3(kCtas);
   cfg.block = dim3(kThreads);

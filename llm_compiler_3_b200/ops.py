@@ -124,21 +124,33 @@ def prefill_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Ten
 # that device's current stream; scratch comes from torch's allocator at each
 # call, so calls on several streams and captured graphs share none.
 # ---------------------------------------------------------------------------
-def _device_of(name: str, t: torch.Tensor, **others: torch.Tensor | None):
-    """Context in which t's device is the current one; every tensor must be on it."""
-    for other, u in others.items():
-        if u is not None and u.device != t.device:
-            raise ValueError(f"{other} is on {u.device} but {name} on {t.device}")
-    if t.device.index == torch.cuda.current_device():
-        return contextlib.nullcontext()
-    return torch.cuda.device(t.device)
+_HERE = contextlib.nullcontext()
 
 
-def _require_pages(k_pages: torch.Tensor, v_pages: torch.Tensor, page_table: torch.Tensor,
-                   batch: int, head_dim: int) -> None:
-    _require(k_pages, "k_pages", ndim=4)
-    _require(v_pages, "v_pages", ndim=4)
-    _require(page_table, "page_table", dtype=torch.int32, ndim=2)
+def _on(index: int):
+    """Context in which the device of that index is the current one."""
+    return _HERE if index == torch.cuda.current_device() else torch.cuda.device(index)
+
+
+def _device_index(t: torch.Tensor, name: str) -> int:
+    if not isinstance(t, torch.Tensor) or not t.is_cuda:
+        raise ValueError(f"{name} must be a CUDA tensor")
+    return t.get_device()
+
+
+def _require_on(index: int, t: torch.Tensor, name: str, dtype: torch.dtype = torch.float16,
+                ndim: int | None = None) -> None:
+    """_require, on the device of that index."""
+    _require(t, name, dtype, ndim)
+    if t.get_device() != index:
+        raise ValueError(f"{name} is on {t.device}, not on cuda:{index}")
+
+
+def _require_pages(index: int, k_pages: torch.Tensor, v_pages: torch.Tensor,
+                   page_table: torch.Tensor, batch: int, head_dim: int) -> None:
+    _require_on(index, k_pages, "k_pages", ndim=4)
+    _require_on(index, v_pages, "v_pages", ndim=4)
+    _require_on(index, page_table, "page_table", torch.int32, 2)
     if v_pages.shape != k_pages.shape or k_pages.shape[3] != head_dim:
         raise ValueError(f"k_pages {tuple(k_pages.shape)}, v_pages {tuple(v_pages.shape)} and "
                          f"head_dim {head_dim} disagree")
@@ -146,20 +158,25 @@ def _require_pages(k_pages: torch.Tensor, v_pages: torch.Tensor, page_table: tor
         raise ValueError("page_table must have one row per sequence")
 
 
-def _require_counts(t: torch.Tensor, name: str, batch: int) -> None:
-    _require(t, name, dtype=torch.int32, ndim=1)
+def _require_counts(index: int, t: torch.Tensor, name: str, batch: int) -> None:
+    _require_on(index, t, name, torch.int32, 1)
     if t.shape[0] != batch:
         raise ValueError(f"{name} must have one entry per sequence")
 
 
-def _output(out: torch.Tensor | None, shape, dtype: torch.dtype, device: torch.device,
-            name: str = "out") -> torch.Tensor:
+def _output_like(like: torch.Tensor, out: torch.Tensor | None, index: int) -> torch.Tensor:
     if out is None:
-        return torch.empty(shape, dtype=dtype, device=device)
-    _require(out, name, dtype=dtype)
-    if out.shape != torch.Size(shape) or out.device != device:
-        raise ValueError(f"{name} must be {tuple(shape)} on {device}")
+        return torch.empty_like(like)
+    _require_on(index, out, "out", like.dtype)
+    if out.shape != like.shape:
+        raise ValueError(f"out must be {tuple(like.shape)}, got {tuple(out.shape)}")
     return out
+
+
+def _raw_stream(index: int) -> int:
+    """The current stream of a device as a number (torch.cuda.current_stream() builds an
+    object around it, which takes longer than a launch)."""
+    return torch._C._cuda_getCurrentRawStream(index)
 
 
 def paged_decode(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor,
@@ -171,22 +188,22 @@ def paged_decode(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor,
 
     Returns out [B, Hq, D] FP16 = softmax(scale q K^T) V over keys [0, seq_lens[b]), with
     window > 0 over the last `window` of them and the first `sinks`; zero without keys."""
+    index = _device_index(q, "q")
     _require(q, "q", ndim=3)
     batch, q_heads, head_dim = q.shape
-    _require_pages(k_pages, v_pages, page_table, batch, head_dim)
-    _require_counts(seq_lens, "seq_lens", batch)
+    _require_pages(index, k_pages, v_pages, page_table, batch, head_dim)
+    _require_counts(index, seq_lens, "seq_lens", batch)
     num_pages, kv_heads, page_size, _ = k_pages.shape
-    with _device_of("q", q, k_pages=k_pages, v_pages=v_pages, page_table=page_table,
-                    seq_lens=seq_lens):
-        out = _output(out, q.shape, q.dtype, q.device)
+    with _on(index):
+        out = _output_like(q, out, index)
         lib = _native.lib()
         need = lib.npu_b200_paged_decode_workspace_size(q_heads, kv_heads, head_dim)
         ws = torch.empty(need, dtype=torch.uint8, device=q.device)
         _native.check(lib.npu_b200_paged_decode(
             q.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(), page_table.data_ptr(),
             seq_lens.data_ptr(), out.data_ptr(), batch, q_heads, kv_heads, head_dim, num_pages,
-            page_size, page_table.shape[1], int(window), int(sinks),
-            head_dim ** -0.5 if scale is None else float(scale), ws.data_ptr(), need, _stream()))
+            page_size, page_table.shape[1], window, sinks,
+            head_dim ** -0.5 if scale is None else scale, ws.data_ptr(), need, _raw_stream(index)))
     return out
 
 
@@ -199,22 +216,21 @@ def paged_prefill(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor,
     seq_lens[b] - q_lens[b] + i.
 
     Returns out [B, Hq, M, D] FP16; rows past q_lens[b] or without a visible key are zero."""
+    index = _device_index(q, "q")
     _require(q, "q", ndim=4)
     batch, q_heads, queries, head_dim = q.shape
-    _require_pages(k_pages, v_pages, page_table, batch, head_dim)
-    _require_counts(seq_lens, "seq_lens", batch)
+    _require_pages(index, k_pages, v_pages, page_table, batch, head_dim)
+    _require_counts(index, seq_lens, "seq_lens", batch)
     if q_lens is not None:
-        _require_counts(q_lens, "q_lens", batch)
+        _require_counts(index, q_lens, "q_lens", batch)
     num_pages, kv_heads, page_size, _ = k_pages.shape
-    with _device_of("q", q, k_pages=k_pages, v_pages=v_pages, page_table=page_table,
-                    seq_lens=seq_lens, q_lens=q_lens):
-        out = _output(out, q.shape, q.dtype, q.device)
+    with _on(index):
+        out = _output_like(q, out, index)
         _native.check(_native.lib().npu_b200_paged_prefill(
             q.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(), page_table.data_ptr(),
             seq_lens.data_ptr(), 0 if q_lens is None else q_lens.data_ptr(), out.data_ptr(), batch,
             q_heads, kv_heads, head_dim, queries, num_pages, page_size, page_table.shape[1],
-            int(window), int(sinks), head_dim ** -0.5 if scale is None else float(scale),
-            _stream()))
+            window, sinks, head_dim ** -0.5 if scale is None else scale, _raw_stream(index)))
     return out
 
 
@@ -223,24 +239,25 @@ def paged_append(k: torch.Tensor, v: torch.Tensor, k_pages: torch.Tensor, v_page
                  lens: torch.Tensor | None = None) -> None:
     """New keys and values into the pages, in place: k, v [B, Hkv, M, D]; row i < lens[b]
     (default: every row) of sequence b goes to position starts[b] + i."""
+    index = _device_index(k, "k")
     _require(k, "k", ndim=4)
-    _require(v, "v", ndim=4)
+    _require_on(index, v, "v", ndim=4)
     batch, kv_heads, rows, head_dim = k.shape
     if v.shape != k.shape:
         raise ValueError("k and v must have one shape")
-    _require_pages(k_pages, v_pages, page_table, batch, head_dim)
-    if k_pages.shape[1] != kv_heads:
-        raise ValueError(f"k has {kv_heads} heads but the pages {k_pages.shape[1]}")
-    _require_counts(starts, "starts", batch)
+    _require_pages(index, k_pages, v_pages, page_table, batch, head_dim)
+    num_pages, heads, page_size, _ = k_pages.shape
+    if heads != kv_heads:
+        raise ValueError(f"k has {kv_heads} heads but the pages {heads}")
+    _require_counts(index, starts, "starts", batch)
     if lens is not None:
-        _require_counts(lens, "lens", batch)
-    num_pages, _, page_size, _ = k_pages.shape
-    with _device_of("k", k, v=v, k_pages=k_pages, v_pages=v_pages, page_table=page_table,
-                    starts=starts, lens=lens):
+        _require_counts(index, lens, "lens", batch)
+    with _on(index):
         _native.check(_native.lib().npu_b200_paged_append(
             k.data_ptr(), v.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(),
             page_table.data_ptr(), starts.data_ptr(), 0 if lens is None else lens.data_ptr(),
-            batch, kv_heads, rows, head_dim, num_pages, page_size, page_table.shape[1], _stream()))
+            batch, kv_heads, rows, head_dim, num_pages, page_size, page_table.shape[1],
+            _raw_stream(index)))
 
 
 def page_update(page_table: torch.Tensor, seq_lens: torch.Tensor, parents: torch.Tensor,
@@ -253,25 +270,24 @@ def page_update(page_table: torch.Tensor, seq_lens: torch.Tensor, parents: torch
     Returns (table [R', E], lens [R'], refs [N], copies [2, R'], info [3]): pages to copy
     (from, to; packed) for `page_copy`, and info = free pages left, pages short, copies.
     The inputs stay as they are, so a step that ran short can be repeated."""
-    _require(page_table, "page_table", dtype=torch.int32, ndim=2)
-    _require(page_refs, "page_refs", dtype=torch.int32, ndim=1)
-    _require(parents, "parents", dtype=torch.int32, ndim=1)
+    index = _device_index(page_table, "page_table")
+    _require(page_table, "page_table", torch.int32, 2)
+    _require_on(index, page_refs, "page_refs", torch.int32, 1)
+    _require_on(index, parents, "parents", torch.int32, 1)
     rows, entries = page_table.shape
-    new_rows = parents.shape[0]
-    _require_counts(seq_lens, "seq_lens", rows)
-    _require_counts(capacity, "capacity", new_rows)
-    n = page_refs.shape[0]
-    with _device_of("page_table", page_table, seq_lens=seq_lens, parents=parents,
-                    capacity=capacity, page_refs=page_refs):
-        # One allocation for the five results, each at a 16-byte border.
-        sizes = [(new_rows * entries, (new_rows, entries)), (new_rows, (new_rows,)), (n, (n,)),
-                 (2 * new_rows, (2, new_rows)), (3, (3,))]
-        table, lens, refs, copies, info = _parts(sizes, page_table.device)
+    new_rows, n = parents.shape[0], page_refs.shape[0]
+    _require_counts(index, seq_lens, "seq_lens", rows)
+    _require_counts(index, capacity, "capacity", new_rows)
+    with _on(index):
+        table = torch.empty_like(page_table) if new_rows == rows else page_table.new_empty(
+            (new_rows, entries))
+        lens, refs = torch.empty_like(parents), torch.empty_like(page_refs)
+        copies, info = page_refs.new_empty((2, new_rows)), page_refs.new_empty(3)
         _native.check(_native.lib().npu_b200_page_update(
             page_table.data_ptr(), seq_lens.data_ptr(), parents.data_ptr(), capacity.data_ptr(),
             page_refs.data_ptr(), table.data_ptr(), lens.data_ptr(), refs.data_ptr(),
-            copies.data_ptr(), info.data_ptr(), rows, new_rows, entries, int(page_size), n,
-            _stream()))
+            copies.data_ptr(), info.data_ptr(), rows, new_rows, entries, page_size, n,
+            _raw_stream(index)))
     return table, lens, refs, copies, info
 
 
@@ -282,48 +298,42 @@ def page_compact(page_table: torch.Tensor, page_refs: torch.Tensor
     Returns (table, refs, moves [2, max(1, N // 2)], index [N], info [2]): pages to copy (from,
     to; packed), where each page is now (-1: free), and info = pages in use, moves.  Move the
     data with `page_copy(pool, moves, info[1:])` before the next use of the new table."""
-    _require(page_table, "page_table", dtype=torch.int32, ndim=2)
-    _require(page_refs, "page_refs", dtype=torch.int32, ndim=1)
+    index = _device_index(page_table, "page_table")
+    _require(page_table, "page_table", torch.int32, 2)
+    _require_on(index, page_refs, "page_refs", torch.int32, 1)
     rows, entries = page_table.shape
     n = page_refs.shape[0]
-    most = max(1, n // 2)
-    with _device_of("page_table", page_table, page_refs=page_refs):
-        sizes = [(rows * entries, (rows, entries)), (n, (n,)), (2 * most, (2, most)), (n, (n,)),
-                 (2, (2,))]
-        table, refs, moves, index, info = _parts(sizes, page_table.device)
+    with _on(index):
+        table, refs = torch.empty_like(page_table), torch.empty_like(page_refs)
+        where = torch.empty_like(page_refs)
+        moves, info = page_refs.new_empty((2, max(1, n // 2))), page_refs.new_empty(2)
         _native.check(_native.lib().npu_b200_page_compact(
             page_table.data_ptr(), page_refs.data_ptr(), table.data_ptr(), refs.data_ptr(),
-            moves.data_ptr(), index.data_ptr(), info.data_ptr(), rows, entries, n, _stream()))
-    return table, refs, moves, index, info
-
-
-def _parts(sizes, device: torch.device) -> list[torch.Tensor]:
-    """int32 tensors of (words, shape), cut from one allocation at 16-byte borders."""
-    steps = [(words + 3) & ~3 for words, _ in sizes]
-    whole = torch.empty(sum(steps), dtype=torch.int32, device=device)
-    return [part[:words].view(shape) for part, (words, shape) in zip(whole.split(steps), sizes)]
+            moves.data_ptr(), where.data_ptr(), info.data_ptr(), rows, entries, n,
+            _raw_stream(index)))
+    return table, refs, moves, where, info
 
 
 def page_copy(pool: torch.Tensor, pages: torch.Tensor, count: torch.Tensor | None = None) -> None:
     """Copies pages in place, in every slab of a pool [slabs, N, ...] of any type (K and V of
     every layer): pages [2, n] int32 (from, to), the first count[0] of them (default: all; -1
     pairs are skipped).  No page that is written may be named twice."""
-    if not isinstance(pool, torch.Tensor) or not pool.is_cuda or not pool.is_contiguous():
-        raise ValueError("pool must be a contiguous CUDA tensor")
-    if pool.dim() < 3 or pool.numel() == 0:
-        raise ValueError(f"pool must be [slabs, pages, ...], got {tuple(pool.shape)}")
-    _require(pages, "pages", dtype=torch.int32, ndim=2)
+    index = _device_index(pool, "pool")
+    if not pool.is_contiguous() or pool.dim() < 3 or pool.numel() == 0:
+        raise ValueError(f"pool must be a contiguous [slabs, pages, ...], got {tuple(pool.shape)}")
+    _require_on(index, pages, "pages", torch.int32, 2)
     if pages.shape[0] != 2:
         raise ValueError("pages must be [2, n]: from and to")
     if count is not None:
-        _require(count, "count", dtype=torch.int32, ndim=1)
+        _require_on(index, count, "count", torch.int32, 1)
         if count.shape[0] < 1:
             raise ValueError("count must hold a number")
     slabs, n = pool.shape[:2]
-    with _device_of("pool", pool, pages=pages, count=count):
+    with _on(index):
         _native.check(_native.lib().npu_b200_page_copy(
             pool.data_ptr(), pages.data_ptr(), 0 if count is None else count.data_ptr(),
-            pages.shape[1], slabs, n, pool.numel() // (slabs * n) * pool.element_size(), _stream()))
+            pages.shape[1], slabs, n, pool.numel() // (slabs * n) * pool.element_size(),
+            _raw_stream(index)))
 
 
 def beam_select(logits: torch.Tensor, scores: torch.Tensor, width: int,
@@ -336,33 +346,33 @@ def beam_select(logits: torch.Tensor, scores: torch.Tensor, width: int,
     Returns (scores [B, width] FP32, tokens, parents [B, width] int32, done [B, width] bool),
     best first, the lowest beam x V + token among equals; parents are rows b x W + beam.  Where
     nothing is left: -inf, -1, -1, False."""
-    if not isinstance(logits, torch.Tensor) or logits.dtype not in (torch.float16, torch.float32):
-        raise ValueError("logits must be a float16 or float32 tensor")
-    _require(logits, "logits", dtype=logits.dtype, ndim=3)
-    _require(scores, "scores", dtype=torch.float32, ndim=2)
+    index = _device_index(logits, "logits")
+    if logits.dtype not in (torch.float16, torch.float32):
+        raise ValueError(f"logits must be float16 or float32, got {logits.dtype}")
+    _require(logits, "logits", logits.dtype, 3)
+    _require_on(index, scores, "scores", torch.float32, 2)
     batch, beams, vocab = logits.shape
     if scores.shape != (batch, beams):
         raise ValueError(f"scores must be {(batch, beams)}, got {tuple(scores.shape)}")
     if done is not None:
-        _require(done, "done", dtype=torch.bool, ndim=2)
+        _require_on(index, done, "done", torch.bool, 2)
         if done.shape != scores.shape:
             raise ValueError("done must have the shape of scores")
-    width = int(width)
     if width < 1:
         raise ValueError(f"width must be positive, got {width}")
-    with _device_of("logits", logits, scores=scores, done=done):
+    with _on(index):
         lib = _native.lib()
-        out_scores = torch.empty(batch, width, dtype=torch.float32, device=logits.device)
-        tokens = torch.empty(batch, width, dtype=torch.int32, device=logits.device)
-        parents = torch.empty(batch, width, dtype=torch.int32, device=logits.device)
-        out_done = torch.empty(batch, width, dtype=torch.bool, device=logits.device)
+        out_scores = scores.new_empty((batch, width))
+        tokens = torch.empty_like(out_scores, dtype=torch.int32)
+        parents = torch.empty_like(tokens)
+        out_done = torch.empty_like(out_scores, dtype=torch.bool)
         need = lib.npu_b200_beam_select_workspace_size(batch, beams, vocab, width)
         ws = torch.empty(need, dtype=torch.uint8, device=logits.device)
         _native.check(lib.npu_b200_beam_select(
-            logits.data_ptr(), logits.dtype == torch.float32, scores.data_ptr(),
+            logits.data_ptr(), logits.dtype is torch.float32, scores.data_ptr(),
             0 if done is None else done.data_ptr(), out_scores.data_ptr(), tokens.data_ptr(),
-            parents.data_ptr(), out_done.data_ptr(), batch, beams, vocab, width, int(eos),
-            ws.data_ptr(), need, _stream()))
+            parents.data_ptr(), out_done.data_ptr(), batch, beams, vocab, width, eos,
+            ws.data_ptr(), need, _raw_stream(index)))
     return out_scores, tokens, parents, out_done
 
 
@@ -370,17 +380,22 @@ def beam_reorder(state: torch.Tensor, parents: torch.Tensor, out: torch.Tensor |
                  ) -> torch.Tensor:
     """Rows of a per-beam state [R, ...] of any type in their new order: out[r] =
     state[parents[r]] for parents of any shape with R' numbers; -1 gives a zero row."""
-    if not isinstance(state, torch.Tensor) or not state.is_cuda or not state.is_contiguous():
-        raise ValueError("state must be a contiguous CUDA tensor")
-    if state.dim() < 1 or state.numel() == 0:
-        raise ValueError(f"state must be [rows, ...], got {tuple(state.shape)}")
-    _require(parents, "parents", dtype=torch.int32)
+    index = _device_index(state, "state")
+    if not state.is_contiguous() or state.dim() < 1 or state.numel() == 0:
+        raise ValueError(f"state must be a contiguous [rows, ...], got {tuple(state.shape)}")
+    _require_on(index, parents, "parents", torch.int32)
     rows, new_rows = state.shape[0], parents.numel()
-    with _device_of("state", state, parents=parents, out=out):
-        out = _output(out, (new_rows, *state.shape[1:]), state.dtype, state.device)
+    with _on(index):
+        if out is None:
+            out = torch.empty_like(state) if new_rows == rows else state.new_empty(
+                (new_rows, *state.shape[1:]))
+        else:
+            _require_on(index, out, "out", state.dtype)
+            if out.shape != (new_rows, *state.shape[1:]):
+                raise ValueError(f"out must be {(new_rows, *state.shape[1:])}, got {tuple(out.shape)}")
         _native.check(_native.lib().npu_b200_beam_reorder(
             state.data_ptr(), parents.data_ptr(), out.data_ptr(), rows, new_rows,
-            state.numel() // rows * state.element_size(), _stream()))
+            state.numel() // rows * state.element_size(), _raw_stream(index)))
     return out
 
 

@@ -243,3 +243,13 @@ def test_wrapper_checks_and_graphs(cuda):
         want = ops.beam_select(logits, scores, 4, done, 2)
         assert all(torch.equal(a, b) for a, b in zip(got, want))
         assert torch.equal(rows, logits.view(6, 500)[want[2].view(-1).long()])
+
+
+@pytest.mark.gpu
+def test_zeros_of_both_signs_tie(cuda):
+    logits = torch.full((1, 2, 600), -1.0, dtype=torch.float16)
+    logits[0, :, 5::90] = -0.0
+    logits[0, :, 7::90] = 0.0
+    got = _select(logits, torch.zeros(1, 2), 14)
+    assert got[1].tolist() == [sorted(list(range(5, 600, 90)) + list(range(7, 600, 90)))]
+    assert got[2].tolist() == [[0] * 14]
