@@ -9,17 +9,18 @@
 // Bound: one pass over the logits (HBM); next to it the exponentials, of which
 // an SM does 16 a clock against the ~12 FP16 logits a clock that HBM brings it.
 // So one pass does both: each warp streams its part of a row, 16 bytes per lane,
-// keeps the sum relative to its running maximum, and holds its `width` best logits
-// sorted across its lanes.  A logit is looked at only if it is a new maximum or
-// reaches a floor that `width` others are known to reach: at first the width-th
-// largest of the CTA's lanes' maxima over their first words, then the worst kept one
-// of any warp.  So maximum and selection cost one comparison per 8 logits and a few
-// insertions (with floors that each warp knew alone they cost twice the rest).  A second, dependent launch joins the stretches.
+// keeps the sum relative to its running maximum, and lists the logits that reach a
+// floor which `width` logits of the CTA are known to reach: the width-th largest of
+// its lanes' maxima over their first words, then, each time twice as much has been
+// read, the width-th best candidate.  That leaves some width x log2(length / 4096)
+// candidates of a stretch, so the selection costs one comparison per 8 logits (sorted
+// lists that each warp kept for itself cost twice the rest).  A warp whose list runs
+// full, on rising logits, keeps its `width` best and raises the floor.  A second, dependent launch joins the stretches.
 //
 // Which of two candidates is larger decides whole beams, so what follows the
 // stretches (the sum over them, its logarithm, the candidates' worth) is in FP64;
-// within a stretch the FP32 sum of up to 2^-22-exact exponentials leaves ln S
-// some 1e-7 off.
+// within a stretch the FP32 sum of exponentials exact to 2^-22 leaves ln S some 1e-7
+// off.
 #include <float.h>
 #include <limits.h>
 
@@ -37,7 +38,11 @@ constexpr int kMaxSplits = 128; // stretches of a row
 constexpr int kStaged = 512;    // entries of a row's lists that the join keeps in shared memory
 constexpr int kSelThreads = 256;
 constexpr int kSelWarps = kSelThreads / 32;
+constexpr int kList = 320;      // candidates of a warp; one word of each lane adds at most 256
 constexpr float kLog2e = 1.4426950408889634f;
+constexpr float kLog2eLow = static_cast<float>(1.4426950408889634 - static_cast<double>(kLog2e));
+constexpr double kLn2 = 0.69314718055994530942;
+constexpr float kNothing = -FLT_MAX;  // the maximum and the reference before any logit above -inf
 
 struct BeamParams {
   const void* logits;
@@ -47,52 +52,14 @@ struct BeamParams {
   int32_t* out_tokens;
   int32_t* out_parents;
   uint8_t* out_done;    // or null
-  // Stretch s of row r: maximum, sum, and the best logits with their tokens.
-  float* part_max;      // [rows][splits]
+  // Stretch s of row r: reference, sum, and the best logits with their tokens.
+  float* part_ref;      // [rows][splits]
   float* part_sum;
   float* part_val;      // [rows][splits][width]
   int32_t* part_idx;
   int beams, vocab, width, splits, words;  // words: 16-byte words of a stretch
-  int eos;
+  int eos, f32;
   long long total;      // logits of the tensor
-};
-
-// The best logits of a warp, in falling order across its lanes: larger first,
-// lower token among equals.  Lanes past `width` hold what fell out.
-struct Best {
-  float val = -INFINITY;
-  int idx = INT_MAX;
-  float floor = -INFINITY;  // the worst kept: lane width - 1, in every lane
-  int floor_idx = INT_MAX;
-  __device__ __forceinline__ bool takes(float v, int i) const {
-    return v > floor || (v == floor && i < floor_idx && v > -INFINITY);
-  }
-  // One candidate, the same in every lane.
-  __device__ __forceinline__ void put(float v, int i, int width) {
-    const int lane = threadIdx.x & 31;
-    const bool before = val > v || (val == v && idx < i);
-    const int at = __popc(__ballot_sync(0xffffffffu, before));
-    const float up_v = __shfl_up_sync(0xffffffffu, val, 1);
-    const int up_i = __shfl_up_sync(0xffffffffu, idx, 1);
-    if (lane > at) {
-      val = up_v;
-      idx = up_i;
-    } else if (lane == at) {
-      val = v;
-      idx = i;
-    }
-    floor = __shfl_sync(0xffffffffu, val, width - 1);
-    floor_idx = __shfl_sync(0xffffffffu, idx, width - 1);
-  }
-  // Each lane offers one.
-  __device__ __forceinline__ void offer(float v, int i, int width) {
-    unsigned mask = __ballot_sync(0xffffffffu, takes(v, i));
-    while (mask) {
-      const int src = __ffs(mask) - 1;
-      put(__shfl_sync(0xffffffffu, v, src), __shfl_sync(0xffffffffu, i, src), width);
-      mask = __ballot_sync(0xffffffffu, takes(v, i)) & ~((2u << src) - 1);
-    }
-  }
 };
 
 // Whole numbers in the order of the floating ones (-0 as 0).
@@ -116,6 +83,45 @@ __device__ __forceinline__ float best_of_lanes(float v, int width) {
     if (lane == i) mine = top;
   }
   return of_order(mine);
+}
+
+// One warp's candidates.
+struct Candidates {
+  float val[kList];
+  int idx[kList];
+  int n;
+};
+
+// The `width` best of the lists' candidates, larger first, lower token among equals:
+// lane k returns the k-th.  Each turn takes the best that comes after the last one.
+__device__ __forceinline__ void take_best(const Candidates* lists, int count, int width, float* out_v,
+                                          int* out_i) {
+  const int lane = threadIdx.x & 31;
+  uint32_t last = 0xffffffffu;
+  int last_i = -1;
+  *out_v = -INFINITY;
+  *out_i = INT_MAX;
+  for (int k = 0; k < width; ++k) {
+    uint32_t best = 0;
+    int best_i = INT_MAX;
+    for (int l = 0; l < count; ++l)
+      for (int e = lane; e < lists[l].n; e += 32) {
+        const uint32_t v = order_of(lists[l].val[e]);
+        const int i = lists[l].idx[e];
+        const bool after = v < last || (v == last && i > last_i);
+        if (after && (v > best || (v == best && i < best_i))) {
+          best = v;
+          best_i = i;
+        }
+      }
+    last = __reduce_max_sync(0xffffffffu, best);
+    if (last == 0) break;  // no more
+    last_i = __reduce_min_sync(0xffffffffu, best == last ? best_i : INT_MAX);
+    if (lane == k) {
+      *out_v = of_order(last);
+      *out_i = last_i;
+    }
+  }
 }
 
 // The `width` best of `lists` lists in falling order, one to a lane (list l of lane
@@ -165,22 +171,87 @@ __device__ __forceinline__ void merge_lists(int lists, int width, Val val, Idx i
   }
 }
 
+// What differs between FP16 and FP32 logits.  Sums are relative to a reference: for
+// FP16 a power of two 2^r, so that e^x / 2^r = 2^(x log2 e - r) takes two FMAs whose
+// roundings are relative to the result, and a new reference costs no rounding; for
+// FP32, whose x log2 e may overflow, e^m.
 // NaN counts as -inf, +inf as the largest number of the type.
-__device__ __forceinline__ void widen(const uint4& w, float (&x)[8], const __half*) {
-  const uint32_t u[4] = {w.x, w.y, w.z, w.w};
-  const __half2 low = __half2half2(__ushort_as_half(0xfc00)), high = __half2half2(__ushort_as_half(0x7bff));
+template <typename T>
+struct Kind;
+template <>
+struct Kind<__half> {
+  static constexpr int kLogits = 8;
+  static constexpr float kMost = 65504.f;
+  // The largest logit of a word, NaN if there is one.
+  static __device__ __forceinline__ float top(const uint4& w) {
+    const uint32_t u[4] = {w.x, w.y, w.z, w.w};
+    __half2 h[4];
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const float2 f = __half22float2(__hmin2(__hmax2(*reinterpret_cast<const __half2*>(&u[i]), low), high));
-    x[2 * i] = f.x;
-    x[2 * i + 1] = f.y;
+    for (int i = 0; i < 4; ++i) h[i] = *reinterpret_cast<const __half2*>(&u[i]);
+    const __half2 t = __hmax2_nan(__hmax2_nan(h[0], h[1]), __hmax2_nan(h[2], h[3]));
+    return __half2float(__hmax_nan(__low2half(t), __high2half(t)));
   }
-}
-__device__ __forceinline__ void widen(const uint4& w, float (&x)[4], const float*) {
-  const uint32_t u[4] = {w.x, w.y, w.z, w.w};
+  // The word with its first n logits made ordinary, and -inf after them.
+  static __device__ __forceinline__ uint4 clean(const uint4& w, int n) {
+    uint32_t u[4] = {w.x, w.y, w.z, w.w};
+    const __half2 low = __half2half2(__ushort_as_half(0xfc00)), high = __half2half2(__ushort_as_half(0x7bff));
 #pragma unroll
-  for (int i = 0; i < 4; ++i) x[i] = fminf(fmaxf(__uint_as_float(u[i]), -INFINITY), FLT_MAX);
-}
+    for (int i = 0; i < 4; ++i) {
+      const __half2 h = __hmin2(__hmax2(*reinterpret_cast<const __half2*>(&u[i]), low), high);
+      u[i] = *reinterpret_cast<const uint32_t*>(&h);
+      if (2 * i + 1 >= n) u[i] = 2 * i >= n ? 0xfc00fc00u : (u[i] & 0xffffu) | 0xfc000000u;
+    }
+    return make_uint4(u[0], u[1], u[2], u[3]);
+  }
+  static __device__ __forceinline__ void widen(const uint4& w, float (&x)[8]) {
+    const uint32_t u[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&u[i]));
+      x[2 * i] = f.x;
+      x[2 * i + 1] = f.y;
+    }
+  }
+  static __device__ __forceinline__ float reference(float m) { return ceilf(m * kLog2e); }
+  // The exponents (base 2) of x0, x1 relative to the reference.
+  static __device__ __forceinline__ uint64_t exponents(float x0, float x1, float ref) {
+    const uint64_t x = pack2(x0, x1);
+    return fma2(x, pack2(kLog2eLow, kLog2eLow), fma2(x, pack2(kLog2e, kLog2e), pack2(-ref, -ref)));
+  }
+  static __device__ __forceinline__ float ratio(float from, float to) { return fast_exp2(from - to); }
+};
+template <>
+struct Kind<float> {
+  static constexpr int kLogits = 4;
+  static constexpr float kMost = FLT_MAX;
+  static __device__ __forceinline__ float top(const uint4& w) {
+    float a, b;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(a) : "f"(__uint_as_float(w.x)), "f"(__uint_as_float(w.y)));
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(b) : "f"(__uint_as_float(w.z)), "f"(__uint_as_float(w.w)));
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(a) : "f"(a), "f"(b));
+    return a;
+  }
+  static __device__ __forceinline__ uint4 clean(const uint4& w, int n) {
+    uint32_t u[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      u[i] = i >= n ? 0xff800000u
+                    : __float_as_uint(fminf(fmaxf(__uint_as_float(u[i]), -INFINITY), kMost));
+    return make_uint4(u[0], u[1], u[2], u[3]);
+  }
+  static __device__ __forceinline__ void widen(const uint4& w, float (&x)[4]) {
+    const uint32_t u[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) x[i] = __uint_as_float(u[i]);
+  }
+  static __device__ __forceinline__ float reference(float m) { return m; }
+  static __device__ __forceinline__ uint64_t exponents(float x0, float x1, float ref) {
+    return mul2(add2(pack2(x0, x1), pack2(-ref, -ref)), pack2(kLog2e, kLog2e));
+  }
+  static __device__ __forceinline__ float ratio(float from, float to) {
+    return fast_exp2((from - to) * kLog2e);
+  }
+};
 
 // The 16-byte word `w` of a tensor of `total` logits; the last one may reach past
 // its end and is then put together one by one, zero behind it.
@@ -217,17 +288,134 @@ __device__ __forceinline__ uint4 shifted(const uint4& a, const uint4& b, int hal
   return make_uint4(u[0], u[1], u[2], u[3]);
 }
 
+__device__ __forceinline__ float warp_max(float v) {
+  return of_order(__reduce_max_sync(0xffffffffu, order_of(v)));
+}
+
+// This thread's candidate among all of the CTA's lists (false: it has none), and how
+// many come before it.
+__device__ __forceinline__ bool rank_of_mine(const Candidates* lists, float* val, int* idx, int* before) {
+  int own = 0, e = threadIdx.x;  // number e of list `own`
+  while (own < kSelWarps && e >= lists[own].n) e -= lists[own++].n;
+  if (own == kSelWarps) return false;
+  *val = lists[own].val[e];
+  *idx = lists[own].idx[e];
+  const uint32_t v = order_of(*val);
+  int n = 0;
+  for (int w = 0; w < kSelWarps; ++w)
+#pragma unroll 4
+    for (int k = 0; k < lists[w].n; ++k) {
+      const uint32_t o = order_of(lists[w].val[k]);
+      n += o > v || (o == v && lists[w].idx[k] < *idx);
+    }
+  *before = n;
+  return true;
+}
+__device__ __forceinline__ int candidates(const Candidates* lists) {
+  int n = 0;
+#pragma unroll
+  for (int w = 0; w < kSelWarps; ++w) n += lists[w].n;
+  return n;
+}
+
+// What a warp carries along its part of a stretch: its maximum and reference, the
+// lane's share of the sum; no logit below `floor` is a candidate, none below `gate`
+// a candidate or a new maximum.
+struct Running {
+  float m = kNothing, ref = 0.f, sum = 0.f;
+  float floor = -INFINITY, gate = -INFINITY;
+};
+
+// One turn of a warp: the lane's words w, w + 32, ...  Nearly always nothing in them
+// reaches the gate (one vote), and what is left is a straight run of exponentials.
+template <typename T, int N>
+__device__ __forceinline__ void take_turn(uint4 (&raw)[N], int w, int width, Candidates& list,
+                                          uint32_t* s_floor, Running& r) {
+  using Kd = Kind<T>;
+  constexpr int L = Kd::kLogits;
+  const int lane = threadIdx.x & 31;
+  float top[N];
+  bool pass = false;
+#pragma unroll
+  for (int u = 0; u < N; ++u) {
+    top[u] = Kd::top(raw[u]);
+    pass |= !(top[u] < r.gate);
+  }
+  if (__any_sync(0xffffffffu, pass)) {
+    float most = -INFINITY;
+#pragma unroll
+    for (int u = 0; u < N; ++u) {
+      if (!(top[u] <= Kd::kMost)) {
+        raw[u] = Kd::clean(raw[u], L);
+        top[u] = Kd::top(raw[u]);
+      }
+      most = fmaxf(most, top[u]);
+    }
+    if (__any_sync(0xffffffffu, most > r.m)) {
+      r.m = warp_max(most);
+      const float to = Kd::reference(r.m);
+      r.sum = r.sum > 0.f ? r.sum * Kd::ratio(r.ref, to) : 0.f;
+      r.ref = to;
+    }
+#pragma unroll
+    for (int u = 0; u < N; ++u) {
+      if (!__any_sync(0xffffffffu, top[u] >= r.floor && top[u] > -INFINITY)) continue;
+      if (list.n > kList - 32 * L) {  // no room for the most that may come
+        __syncwarp();
+        float val;
+        int idx;
+        take_best(&list, 1, width, &val, &idx);
+        __syncwarp();
+        if (lane < width) {
+          list.val[lane] = val;
+          list.idx[lane] = idx;
+        }
+        if (lane == 0) list.n = width;
+        r.floor = fmaxf(r.floor, __shfl_sync(0xffffffffu, val, width - 1));
+        if (lane == 0) atomicMax(s_floor, order_of(r.floor));
+        __syncwarp();
+      }
+      if (top[u] >= r.floor && top[u] > -INFINITY) {
+        float x[L];
+        Kd::widen(raw[u], x);
+#pragma unroll
+        for (int i = 0; i < L; ++i)
+          if (x[i] >= r.floor && x[i] > -INFINITY) {
+            const int at = atomicAdd(&list.n, 1);
+            list.val[at] = x[i];
+            list.idx[at] = (w + u * 32) * L + i;
+          }
+      }
+      __syncwarp();
+    }
+  }
+  uint64_t s2[2] = {0, 0};
+#pragma unroll
+  for (int u = 0; u < N; ++u) {
+    float x[L];
+    Kd::widen(raw[u], x);
+#pragma unroll
+    for (int i = 0; i < L; i += 2) {
+      const uint64_t e2 = Kd::exponents(x[i], x[i + 1], r.ref);
+      s2[(i >> 1) & 1] = add2(s2[(i >> 1) & 1], pack2(fast_exp2(lo2(e2)), fast_exp2(hi2(e2))));
+    }
+  }
+  const uint64_t all2 = add2(s2[0], s2[1]);
+  r.sum += lo2(all2) + hi2(all2);
+}
+
 // Block (s, row): stretch s of row `row`, a piece per warp.
 template <typename T>
-__global__ void __launch_bounds__(kSelThreads, 4) beam_stretch_kernel(const BeamParams p) {
-  constexpr int L = 16 / sizeof(T);  // logits of a word
-  __shared__ float s_val[kSelWarps][32], s_max[kSelWarps], s_sum[kSelWarps];
-  __shared__ int s_idx[kSelWarps][32];
-  __shared__ uint32_t s_floor;  // order_of() of what `width` logits of the row reach
+__global__ void __launch_bounds__(kSelThreads, 3) beam_stretch_kernel(const BeamParams p) {
+  using Kd = Kind<T>;
+  constexpr int L = Kd::kLogits;
+  __shared__ float s_ref[kSelWarps], s_sum[kSelWarps];
+  __shared__ Candidates s_list[kSelWarps];
+  __shared__ uint32_t s_best[kSelWarps * kMaxWidth];  // the lanes' best first logits, by warp
+  __shared__ uint32_t s_floor;  // order_of() of what `width` logits of the CTA reach
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const long long row = blockIdx.y;
-  if (threadIdx.x == 0) s_floor = 0;
-  __syncthreads();
+  if (lane == 0) s_list[warp].n = 0;
   pdl_launch_dependents();
   pdl_wait();
   if (p.done != nullptr && p.done[row]) return;  // the join does not look at its stretches
@@ -240,119 +428,120 @@ __global__ void __launch_bounds__(kSelThreads, 4) beam_stretch_kernel(const Beam
   const int words = (p.vocab + L - 1) / L;
   const int w_begin = min(static_cast<int>(blockIdx.x) * p.words, words);
   const int w_end = min(w_begin + p.words, words);
-
-  Best best;
-  float m = -FLT_MAX, sum = 0.f;  // of the warp, and the lane's share
+  Candidates& list = s_list[warp];
+  Running r;
   constexpr int kAhead = 4;
   constexpr int kTurn = 32 * kAhead;  // words that a warp loads together
   const int turns = (w_end - w_begin + kSelWarps * kTurn - 1) / (kSelWarps * kTurn);
-  for (int turn = 0; turn < turns; ++turn) {  // every warp takes every turn
+  uint4 next[kAhead];
+  auto load = [&](int turn) {  // a turn inside the stretch, the row and the tensor needs no checks
     const int w0 = w_begin + (turn * kSelWarps + warp) * kTurn;
-    // A turn inside the stretch, the row and the tensor needs no checks.
-    const bool inside = w0 + kTurn <= w_end && (w0 + kTurn) * L <= p.vocab;
-    uint4 raw[kAhead];
-    if (inside) {
+    if (w0 + kTurn <= w_end && (w0 + kTurn) * L <= p.vocab) {
       const uint4* src = reinterpret_cast<const uint4*>(logits) + first + w0 + lane;
 #pragma unroll
-      for (int u = 0; u < kAhead; ++u) raw[u] = __ldg(src + u * 32);
+      for (int u = 0; u < kAhead; ++u) next[u] = __ldg(src + u * 32);
     } else {
 #pragma unroll
       for (int u = 0; u < kAhead; ++u)
-        raw[u] = tensor_word(logits, first + min(w0 + u * 32 + lane, w_end - 1), p.total);
+        next[u] = tensor_word(logits, first + min(w0 + u * 32 + lane, w_end - 1), p.total);
     }
+  };
+  if (turns > 0) load(0);
+  for (int turn = 0; turn < turns; ++turn) {  // every warp takes every turn
+    const int w0 = w_begin + (turn * kSelWarps + warp) * kTurn, w = w0 + lane;
+    uint4 raw[kAhead];
+#pragma unroll
+    for (int u = 0; u < kAhead; ++u) raw[u] = next[u];
     if (lead != 0) {
 #pragma unroll
       for (int u = 0; u < kAhead; ++u)
-        raw[u] = shifted(raw[u], tensor_word(logits, first + min(w0 + u * 32 + lane, w_end - 1) + 1, p.total),
+        raw[u] = shifted(raw[u], tensor_word(logits, first + min(w + u * 32, w_end - 1) + 1, p.total),
                          lead * static_cast<int>(sizeof(T)) / 2);
     }
-    auto logits_of = [&](int u, float(&x)[L]) {
-      widen(raw[u], x, logits);
-      if (!inside) {
-        const int n = w0 + u * 32 + lane < w_end ? p.vocab - (w0 + u * 32 + lane) * L : 0;
+    if (turn + 1 < turns) load(turn + 1);
+    if (w0 + kTurn > w_end || (w0 + kTurn) * L > p.vocab) {
 #pragma unroll
-        for (int i = 0; i < L; ++i)
-          if (i >= n) x[i] = -INFINITY;
-      }
-      float top = max3(x[0], x[1], max3(x[2], x[3], x[L - 1]));
-      if (L == 8) top = max3(top, x[4 % L], max3(x[5 % L], x[6 % L], top));
-      return top;
-    };
+      for (int u = 0; u < kAhead; ++u)
+        raw[u] = Kd::clean(raw[u], w + u * 32 < w_end ? p.vocab - (w + u * 32) * L : 0);
+    }
     if (turn == 0) {
       float top = -INFINITY;
 #pragma unroll
       for (int u = 0; u < kAhead; ++u) {
-        float x[L];
-        top = fmaxf(top, logits_of(u, x));
+        float t = Kd::top(raw[u]);
+        if (!(t <= Kd::kMost)) t = Kd::top(Kd::clean(raw[u], L));
+        top = fmaxf(top, t);
       }
-      m = fmaxf(m, of_order(__reduce_max_sync(0xffffffffu, order_of(top))));
-      s_val[warp][lane] = best_of_lanes(top, p.width);
+      r.m = fmaxf(r.m, warp_max(top));
+      if (r.m > kNothing) r.ref = Kd::reference(r.m);
+      const float best = best_of_lanes(top, p.width);
+      const int all = kSelWarps * p.width;
+      if (lane < p.width) s_best[warp * p.width + lane] = order_of(best);
       __syncthreads();
-      if (warp == 0) {  // the warps' lists into one: its last is the first floor
-        float val;
-        int idx;
-        merge_lists(kSelWarps, p.width, [&](int l, int i) { return s_val[l][i]; },
-                    [&](int l, int) { return l; }, &val, &idx);
-        val = __shfl_sync(0xffffffffu, val, p.width - 1);
-        if (lane == 0) s_floor = order_of(val);
+      for (int i = threadIdx.x; i < all; i += kSelThreads) {  // the width-th of all is the floor
+        const uint32_t v = s_best[i];
+        int before = 0;
+        for (int k = 0; k < all; ++k) before += s_best[k] > v || (s_best[k] == v && k < i);
+        if (before == p.width - 1) s_floor = v;
       }
       __syncthreads();
     }
-    float floor = of_order(max(order_of(best.floor), *const_cast<volatile uint32_t*>(&s_floor)));
-#pragma unroll
-    for (int u = 0; u < kAhead; ++u) {
-      float x[L];
-      const float top = logits_of(u, x);
-      if (__any_sync(0xffffffffu, top >= floor || top > m)) {
-        const float m_new = fmaxf(m, of_order(__reduce_max_sync(0xffffffffu, order_of(top))));
-        sum *= fast_exp2((m - m_new) * kLog2e);
-        m = m_new;
-        const int t0 = (w0 + u * 32 + lane) * L;  // token of the word's first logit
-#pragma unroll
-        for (int i = 0; i < L; ++i) best.offer(x[i] >= floor ? x[i] : -INFINITY, t0 + i, p.width);
-        if (best.floor > floor) {
-          floor = best.floor;
-          if (lane == 0) atomicMax(&s_floor, order_of(floor));
-        }
-      }
-      const uint64_t minus2 = pack2(-m, -m), log2e2 = pack2(kLog2e, kLog2e);
-      uint64_t s2 = 0;
-#pragma unroll
-      for (int i = 0; i < L; i += 2) {
-        const uint64_t d2 = mul2(add2(pack2(x[i], x[i + 1]), minus2), log2e2);
-        s2 = add2(s2, pack2(fast_exp2(lo2(d2)), fast_exp2(hi2(d2))));
-      }
-      sum += lo2(s2) + hi2(s2);
+    if (turn > 0 && (turn & (turn - 1)) == 0) {  // read twice as much as at the last floor
+      __syncthreads();
+      float val;
+      int idx, before;
+      if (candidates(s_list) <= kSelThreads && rank_of_mine(s_list, &val, &idx, &before) &&
+          before == p.width - 1)
+        atomicMax(&s_floor, order_of(val));
+      __syncthreads();
     }
+    r.floor = fmaxf(r.floor, of_order(*const_cast<volatile uint32_t*>(&s_floor)));
+    r.gate = fminf(r.floor, r.m);
+    take_turn<T>(raw, w, p.width, list, &s_floor, r);
   }
   // The lanes' sums, then the warps'.
 #pragma unroll
-  for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-  s_val[warp][lane] = best.val;
-  s_idx[warp][lane] = best.idx;
+  for (int o = 16; o > 0; o >>= 1) r.sum += __shfl_xor_sync(0xffffffffu, r.sum, o);
   if (lane == 0) {
-    s_max[warp] = m;
-    s_sum[warp] = sum;
+    s_ref[warp] = r.m > kNothing ? r.ref : kNothing;
+    s_sum[warp] = r.sum;
   }
   __syncthreads();
-  if (warp != 0) return;
-  float m_all = -FLT_MAX, sum_all = 0.f;
-#pragma unroll
-  for (int w = 0; w < kSelWarps; ++w) m_all = fmaxf(m_all, s_max[w]);
-#pragma unroll
-  for (int w = 0; w < kSelWarps; ++w) sum_all += s_sum[w] * fast_exp2((s_max[w] - m_all) * kLog2e);
-  float val;
-  int idx;
-  merge_lists(kSelWarps, p.width, [&](int l, int i) { return s_val[l][i]; },
-              [&](int l, int i) { return s_idx[l][i]; }, &val, &idx);
-  const long long at = row * p.splits + blockIdx.x;
-  if (lane == 0) {
-    p.part_max[at] = m_all;
-    p.part_sum[at] = sum_all;
+  // The candidates, each ranked among all by its own thread; more than a few come
+  // down to `width` of each warp first.
+  if (candidates(s_list) > kSelThreads) {  // the same in every thread
+    float val;
+    int idx;
+    take_best(&list, 1, p.width, &val, &idx);
+    __syncthreads();
+    if (lane < p.width) {
+      list.val[lane] = val;
+      list.idx[lane] = idx;
+    }
+    if (lane == 0) list.n = min(list.n, p.width);
+    __syncthreads();
   }
-  if (lane < p.width) {
-    p.part_val[at * p.width + lane] = val;
-    p.part_idx[at * p.width + lane] = idx;
+  const long long at = row * p.splits + blockIdx.x;
+  float val;
+  int idx, before;
+  if (rank_of_mine(s_list, &val, &idx, &before) && before < p.width) {
+    p.part_val[at * p.width + before] = val;
+    p.part_idx[at * p.width + before] = idx;
+  }
+  if (warp != 0) return;
+  const int n_all = candidates(s_list);
+  if (lane >= n_all && lane < p.width) {
+    p.part_val[at * p.width + lane] = -INFINITY;
+    p.part_idx[at * p.width + lane] = INT_MAX;
+  }
+  float ref_all = kNothing, sum_all = 0.f;
+#pragma unroll
+  for (int w = 0; w < kSelWarps; ++w) ref_all = fmaxf(ref_all, s_ref[w]);
+#pragma unroll
+  for (int w = 0; w < kSelWarps; ++w) sum_all += s_sum[w] * Kd::ratio(s_ref[w], ref_all);
+  if (lane == 0) {
+    p.part_ref[at] = ref_all;
+    p.part_sum[at] = sum_all;
   }
 }
 
@@ -389,14 +578,14 @@ __global__ void __launch_bounds__(kSelThreads) beam_join_kernel(const BeamParams
         val = s_val[warp];
         idx = s_idx[warp];
       }
-      float m = -FLT_MAX;
-      for (int s = lane; s < p.splits; s += 32) m = fmaxf(m, p.part_max[row * p.splits + s]);
+      float m = kNothing;  // the stretches' largest reference
+      for (int s = lane; s < p.splits; s += 32) m = fmaxf(m, p.part_ref[row * p.splits + s]);
 #pragma unroll
       for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
       double sum = 0.0;
       for (int s = lane; s < p.splits; s += 32) {
-        const float d = p.part_max[row * p.splits + s] - m;
-        sum += static_cast<double>(p.part_sum[row * p.splits + s]) * exp(static_cast<double>(d));
+        const double d = static_cast<double>(p.part_ref[row * p.splits + s]) - m;
+        sum += static_cast<double>(p.part_sum[row * p.splits + s]) * (p.f32 ? exp(d) : exp2(d));
       }
 #pragma unroll
       for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
@@ -405,7 +594,7 @@ __global__ void __launch_bounds__(kSelThreads) beam_join_kernel(const BeamParams
       merge_lists(p.splits, p.width, [&](int l, int i) { return val[l * p.width + i]; },
                   [&](int l, int i) { return idx[l * p.width + i]; }, &best, &token);
       if (best > -INFINITY)
-        worth = ((static_cast<double>(best) - static_cast<double>(m)) - log(sum)) + score;
+        worth = ((best - (p.f32 ? 1.0 : kLn2) * m) - log(sum)) + score;
     }
     if (!(worth > -INFINITY)) worth = -INFINITY;  // NaN scores choose nothing
     s_worth[w][lane] = worth;
@@ -486,11 +675,11 @@ int launch_reorder(ReorderParams p, long long row_bytes, cudaStream_t stream) {
   return launch(cfg, beam_reorder_kernel<V>, p);
 }
 
-// Stretches of a row: enough CTAs to fill the SMs a few times over, none shorter
-// than half a turn of its warps, none over 2^17 logits (a lane then adds at most 64
-// words' sums in FP32).
+// Stretches of a row: as many as keep all CTAs resident at once (3 an SM), since each
+// CTA pays for its floor and its ranking; none shorter than half a turn of its
+// warps, none over 2^17 logits (a lane then adds at most 64 words' sums in FP32).
 int beam_splits(long long rows, int vocab) {
-  const long long want = (8ll * sm_count() + rows - 1) / rows;
+  const long long want = 3ll * sm_count() / rows;
   const long long most = (vocab + kSelThreads * 16 - 1) / (kSelThreads * 16);
   const long long least = (vocab + (1 << 17) - 1) / (1 << 17);
   const long long s = std::max(std::min(want, most), least);
@@ -546,13 +735,14 @@ extern "C" int npu_b200_beam_select(const void* d_logits, int logits_f32, const 
   p.vocab = vocab;
   p.width = width;
   p.eos = eos;
+  p.f32 = logits_f32 != 0;
   p.total = rows * vocab;
   p.splits = beam_splits(rows, vocab);
   const int per_word = logits_f32 ? 4 : 8;
   const int words = (vocab + per_word - 1) / per_word;
   p.words = (words + p.splits - 1) / p.splits;
-  p.part_max = static_cast<float*>(d_workspace);
-  p.part_sum = p.part_max + rows * p.splits;
+  p.part_ref = static_cast<float*>(d_workspace);
+  p.part_sum = p.part_ref + rows * p.splits;
   p.part_val = p.part_sum + rows * p.splits;
   p.part_idx = reinterpret_cast<int32_t*>(p.part_val + rows * p.splits * width);
   LaunchCfg cfg;
