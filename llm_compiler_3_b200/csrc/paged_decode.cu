@@ -34,19 +34,19 @@
 namespace npu_b200 {
 namespace {
 
-constexpr int kTile = 32;   // keys per warp stage
-constexpr int kWarps = 4;
-constexpr int kMinTiles = 4;  // of a CTA's stretch: one per warp
 constexpr float kRescaleLog2 = 8.f;
 
 template <int D, int NB>
 struct PdShape {
+  static constexpr int kTile = D == 128 ? 32 : 64;       // keys per warp stage: 16 KB of K and V
+  static constexpr int kWarps = 4;
+  static constexpr int kThreads = kWarps * 32;
   static constexpr int kHeads = 8 * NB;                  // MMA columns: query heads of a unit
   static constexpr int kRegions = D / 64;                // 128-byte swizzle regions per row
   static constexpr int kRegionBytes = kTile * 128;
   static constexpr int kTileBytes = kTile * D * 2;       // K (or V) of one tile
   static constexpr int kStageBytes = 2 * kTileBytes;
-  static constexpr int kStages = D == 128 ? 3 : 6;
+  static constexpr int kStages = 3;
   static constexpr int kRing = kWarps * kStages * kStageBytes;
   static constexpr int kJoinFloats = kWarps * kHeads * (D + 3) + 2 * kHeads;
   static constexpr int kBars = kRing + ((kJoinFloats * 4 + 15) & ~15);
@@ -67,10 +67,11 @@ struct PdParams {
   float scale_log2;
 };
 
-// One sequence's keys.
+// One sequence's keys, in tiles of T.
+template <int T>
 struct Keys {
   int len, lo, s;
-  TileRange<kTile> tiles;
+  TileRange<T> tiles;
   __device__ __forceinline__ void set(const PdParams& p, int b) {
     len = min(max(p.lens[b], 0), p.entries * p.page_size);
     lo = p.window > 0 ? max(0, len - p.window) : 0;
@@ -90,9 +91,10 @@ struct Keys {
 
 // A place in the line of tiles: tile i of (sequence b, KV head h, block c of its
 // query heads).
+template <int T>
 struct Place {
   int b, h, c, i;
-  Keys keys;
+  Keys<T> keys;
   __device__ __forceinline__ void forward(const PdParams& p, int step) {
     i += step;
     while (i >= keys.tiles.n) {
@@ -131,11 +133,12 @@ __device__ __forceinline__ void unrolled(F&& f) {
 }
 
 template <int D, int NB>
-__global__ void __launch_bounds__(kWarps * 32, 1)
+__global__ void __launch_bounds__(PdShape<D, NB>::kThreads, 1)
     paged_decode_kernel(const __grid_constant__ CUtensorMap kmap,
                         const __grid_constant__ CUtensorMap vmap, const PdParams p) {
   using S = PdShape<D, NB>;
-  constexpr int KSTEPS = D / 16, DBLK = D / 16;
+  constexpr int KSTEPS = D / 16, DBLK = D / 16, kWarps = S::kWarps;
+  constexpr int kTile = S::kTile, MT = kTile / 16;  // 16-key blocks of a tile
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) &
                                              ~uintptr_t(1023));
@@ -170,7 +173,7 @@ __global__ void __launch_bounds__(kWarps * 32, 1)
   const int b_first = min(static_cast<int>(threadIdx.x) * each, p.batch);
   const int b_end = min(b_first + each, p.batch);
   long long mine = 0;
-  Place at;
+  Place<kTile> at;
   for (int b = b_first; b < b_end; ++b) {
     at.keys.set(p, b);
     mine += static_cast<long long>(at.keys.tiles.n) * units;
@@ -190,7 +193,7 @@ __global__ void __launch_bounds__(kWarps * 32, 1)
     total += s_sum[w];
   }
   long long per = (total + gridDim.x - 1) / gridDim.x;
-  per = max(per, static_cast<long long>(kMinTiles));
+  per = max(per, static_cast<long long>(kWarps));  // no warp without a tile
   const long long t0 = blockIdx.x * per, t1 = min(total, t0 + per);
   if (threadIdx.x == 0) p.joins[blockIdx.x] = make_int4(0, 0, 0, 0);
   if (t0 >= t1) return;
@@ -225,7 +228,7 @@ __global__ void __launch_bounds__(kWarps * 32, 1)
   const int combos = boxes * S::kRegions * 2;
   const int my_box = lane / (S::kRegions * 2), my_region = (lane >> 1) % S::kRegions;
   const bool my_v = lane & 1;
-  Place ahead = at;
+  Place<kTile> ahead = at;
   ahead.forward(p, warp);
   // This lane's box of the tile at `ahead`: its page (-2: no visible key in it), and
   // its row from the page's first.
@@ -312,19 +315,20 @@ __global__ void __launch_bounds__(kWarps * 32, 1)
       const uint32_t kbase = smem_u32(kst), vbase = kbase + S::kTileBytes;
       if (!whole) {
         // A hidden row may hold anything; its weight is 0, but 0 * NaN is NaN.
-        if (!at.keys.sees(key0 + lane)) {
+        for (int row = lane; row < kTile; row += 32)
+          if (!at.keys.sees(key0 + row)) {
 #pragma unroll
-          for (int r = 0; r < S::kRegions; ++r)
-            for (int x = 0; x < 128; x += 16)
-              *reinterpret_cast<uint4*>(kst + S::kTileBytes + r * S::kRegionBytes + lane * 128 + x) =
-                  make_uint4(0, 0, 0, 0);
-        }
+            for (int r = 0; r < S::kRegions; ++r)
+              for (int x = 0; x < 128; x += 16)
+                *reinterpret_cast<uint4*>(kst + S::kTileBytes + r * S::kRegionBytes + row * 128 + x) =
+                    make_uint4(0, 0, 0, 0);
+          }
         __syncwarp();
       }
 
-      // scores S^T[key, head] of two 16-key blocks
-      float sv[2][NB][4] = {};
-      unrolled<2>([&](auto mt) {
+      // scores S^T[key, head] of the 16-key blocks
+      float sv[MT][NB][4] = {};
+      unrolled<MT>([&](auto mt) {
         unrolled<KSTEPS>([&](auto s) {
           uint32_t a[4];
           ldmatrix_x4_at<(s / 4) * S::kRegionBytes + mt * 2048>(a, kbase + k_at[s % 4]);
@@ -338,7 +342,7 @@ __global__ void __launch_bounds__(kWarps * 32, 1)
       // then, and only then, the lanes of a column compare notes and O is rescaled.
       bool grows = false;
 #pragma unroll
-      for (int mt = 0; mt < 2; ++mt)
+      for (int mt = 0; mt < MT; ++mt)
 #pragma unroll
         for (int nb = 0; nb < NB; ++nb)
 #pragma unroll
@@ -354,7 +358,9 @@ __global__ void __launch_bounds__(kWarps * 32, 1)
           float alpha[2];
 #pragma unroll
           for (int j = 0; j < 2; ++j) {
-            float top = fmaxf(fmaxf(sv[0][nb][j], sv[0][nb][2 + j]), fmaxf(sv[1][nb][j], sv[1][nb][2 + j]));
+            float top = -INFINITY;
+#pragma unroll
+            for (int mt = 0; mt < MT; ++mt) top = max3(top, sv[mt][nb][j], sv[mt][nb][2 + j]);
             top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 4));
             top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 8));
             top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 16));
@@ -374,14 +380,14 @@ __global__ void __launch_bounds__(kWarps * 32, 1)
           }
         }
       }
-      uint32_t pb[2][NB][2];
+      uint32_t pb[MT][NB][2];
 #pragma unroll
       for (int nb = 0; nb < NB; ++nb) {
         float m_use[2];  // no key seen yet: all scores are -inf
 #pragma unroll
         for (int j = 0; j < 2; ++j) m_use[j] = m_run[nb][j] == -INFINITY ? 0.f : m_run[nb][j];
 #pragma unroll
-        for (int mt = 0; mt < 2; ++mt) {
+        for (int mt = 0; mt < MT; ++mt) {
           float w[4];
 #pragma unroll
           for (int r = 0; r < 4; ++r) {
@@ -393,7 +399,7 @@ __global__ void __launch_bounds__(kWarps * 32, 1)
         }
       }
       // O^T[dim, head] += V^T P^T
-      unrolled<2>([&](auto mt) {
+      unrolled<MT>([&](auto mt) {
         unrolled<DBLK>([&](auto d) {
           uint32_t a[4];
           ldmatrix_x4_trans_at<(d / 4) * S::kRegionBytes + mt * 2048>(a, vbase + v_at[d % 4]);
@@ -404,7 +410,7 @@ __global__ void __launch_bounds__(kWarps * 32, 1)
       });
       __syncwarp();
       if (issued < my_tiles) {
-        fence_proxy_async_smem();  // this stage's reads and zero-fill precede the next TMA write
+        if (!whole) fence_proxy_async_smem();  // the zero-fill precedes the next TMA write
         issue(issued++, st);
       }
       if (++st == S::kStages) {
@@ -523,15 +529,16 @@ __global__ void __launch_bounds__(D) paged_decode_join_kernel(const PdParams p) 
 }
 
 template <int D, int NB>
-int launch_pd(const CUtensorMap& km, const CUtensorMap& vm, const PdParams& p, int ctas,
+int launch_pd(const CUtensorMap& km, const CUtensorMap& vm, const PdParams& p, long long most_tiles,
               cudaStream_t stream) {
   using S = PdShape<D, NB>;
+  const int ctas = static_cast<int>(std::min<long long>(sm_count(), (most_tiles + S::kWarps - 1) / S::kWarps));
   auto kern = paged_decode_kernel<D, NB>;
   NPU_TRY_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                     static_cast<int>(S::kSmem)));
   LaunchCfg cfg;
   cfg.grid = dim3(ctas);
-  cfg.block = dim3(kWarps * 32);
+  cfg.block = dim3(S::kThreads);
   cfg.smem = S::kSmem;
   cfg.stream = stream;
   cfg.pdl = true;
@@ -593,7 +600,8 @@ extern "C" int npu_b200_paged_decode(const void* d_q, const void* d_k_pages, con
               "paged_decode: workspace of %zu bytes needed, %zu given", need, workspace_bytes);
 
   const uint64_t rows = static_cast<uint64_t>(num_pages) * kv_heads * page_size;
-  const int box = page_box(page_size, kTile);
+  const int tile = head_dim == 128 ? PdShape<128, 1>::kTile : PdShape<64, 1>::kTile;
+  const int box = page_box(page_size, tile);
   CUtensorMap km, vm;
   rc = make_tensor_map_2d(&km, d_k_pages, rows, head_dim, box, 64);
   if (rc) return rc;
@@ -623,15 +631,14 @@ extern "C" int npu_b200_paged_decode(const void* d_q, const void* d_k_pages, con
   p.scale_log2 = scale * 1.4426950408889634f;
   // No more CTAs than the longest table could keep busy.
   const int sms = sm_count();
-  long long most = (static_cast<long long>(table_entries) * page_size + kTile - 1) / kTile;
+  long long most = (static_cast<long long>(table_entries) * page_size + tile - 1) / tile;
   if (window > 0)
-    most = std::min(most, static_cast<long long>(window) / kTile + sinks / kTile + 4);
+    most = std::min(most, static_cast<long long>(window) / tile + sinks / tile + 4);
   most *= static_cast<long long>(batch) * kv_heads * p.chunks;
-  const int ctas = static_cast<int>(std::min<long long>(sms, (most + kMinTiles - 1) / kMinTiles));
   p.joins = static_cast<int4*>(d_workspace);
   p.part = reinterpret_cast<float*>(p.joins + sms);
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   if (head_dim == 128)
-    return heads == 8 ? launch_pd<128, 1>(km, vm, p, ctas, s) : launch_pd<128, 2>(km, vm, p, ctas, s);
-  return heads == 8 ? launch_pd<64, 1>(km, vm, p, ctas, s) : launch_pd<64, 2>(km, vm, p, ctas, s);
+    return heads == 8 ? launch_pd<128, 1>(km, vm, p, most, s) : launch_pd<128, 2>(km, vm, p, most, s);
+  return heads == 8 ? launch_pd<64, 1>(km, vm, p, most, s) : launch_pd<64, 2>(km, vm, p, most, s);
 }

@@ -237,8 +237,8 @@ __global__ void __launch_bounds__(kThreads, 1)
           if (lane == 0) mbar_arrive_expect_tx(bar, S::kTileBytes);
           __syncwarp();
           if (mine)
-            tma_load_3d(sRing + s * S::kTileBytes + my_region * S::kRegion + my_row * 128,
-                        kv ? &vmap : &kmap, bar, my_region * 64, row, 0);
+            tma_load_2d(smem + S::kRing + s * S::kTileBytes + my_region * S::kRegion + my_row * 128,
+                        kv ? &vmap : &kmap, bar, my_region * 64, row);
           issued = x + 1;
         }
       }
@@ -541,9 +541,9 @@ extern "C" int npu_b200_paged_prefill(const void* d_q, const void* d_k_pages, co
   rc = make_tensor_map_3d(&qm, d_q, head_dim, queries, static_cast<uint64_t>(batch) * q_heads,
                           static_cast<uint64_t>(queries) * head_dim * 2, p.bm, 64);
   if (rc) return rc;
-  rc = make_tensor_map_3d(&km, d_k_pages, head_dim, rows, 1, rows * head_dim * 2, p.box, 64);
+  rc = make_tensor_map_2d(&km, d_k_pages, rows, head_dim, p.box, 64);
   if (rc) return rc;
-  rc = make_tensor_map_3d(&vm, d_v_pages, head_dim, rows, 1, rows * head_dim * 2, p.box, 64);
+  rc = make_tensor_map_2d(&vm, d_v_pages, rows, head_dim, p.box, 64);
   if (rc) return rc;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   return head_dim == 128 ? launch_pp<128>(qm, km, vm, p, batch, s)

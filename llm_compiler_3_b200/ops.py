@@ -6,8 +6,8 @@ here runs a libnpu_b200 kernel and nothing else.  Inputs must be CUDA, FP16
 """
 from __future__ import annotations
 
-import contextlib
 import ctypes
+from functools import lru_cache
 
 import torch
 
@@ -124,26 +124,27 @@ def prefill_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Ten
 # that device's current stream; scratch comes from torch's allocator at each
 # call, so calls on several streams and captured graphs share none.
 # ---------------------------------------------------------------------------
-_HERE = contextlib.nullcontext()
-
-
-def _on(index: int):
-    """Context in which the device of that index is the current one."""
-    return _HERE if index == torch.cuda.current_device() else torch.cuda.device(index)
-
-
 def _device_index(t: torch.Tensor, name: str) -> int:
     if not isinstance(t, torch.Tensor) or not t.is_cuda:
         raise ValueError(f"{name} must be a CUDA tensor")
     return t.get_device()
 
 
+def _elsewhere(index: int) -> bool:
+    """Whether another device than that one is current (the operator then calls itself with
+    it current)."""
+    return torch._C._cuda_getDevice() != index
+
+
 def _require_on(index: int, t: torch.Tensor, name: str, dtype: torch.dtype = torch.float16,
                 ndim: int | None = None) -> None:
-    """_require, on the device of that index."""
+    """_require, on the device of that index (in one expression: these calls are short, and
+    their checks count)."""
+    if (isinstance(t, torch.Tensor) and t.dtype is dtype and t.get_device() == index
+            and t.is_contiguous() and (ndim is None or t.dim() == ndim)):
+        return
     _require(t, name, dtype, ndim)
-    if t.get_device() != index:
-        raise ValueError(f"{name} is on {t.device}, not on cuda:{index}")
+    raise ValueError(f"{name} is on {t.device}, not on cuda:{index}")
 
 
 def _require_pages(index: int, k_pages: torch.Tensor, v_pages: torch.Tensor,
@@ -173,6 +174,11 @@ def _output_like(like: torch.Tensor, out: torch.Tensor | None, index: int) -> to
     return out
 
 
+@lru_cache(maxsize=None)
+def _paged_decode_bytes(index: int, q_heads: int, kv_heads: int, head_dim: int) -> int:
+    return _native.lib().npu_b200_paged_decode_workspace_size(q_heads, kv_heads, head_dim)
+
+
 def _raw_stream(index: int) -> int:
     """The current stream of a device as a number (torch.cuda.current_stream() builds an
     object around it, which takes longer than a launch)."""
@@ -194,16 +200,18 @@ def paged_decode(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor,
     _require_pages(index, k_pages, v_pages, page_table, batch, head_dim)
     _require_counts(index, seq_lens, "seq_lens", batch)
     num_pages, kv_heads, page_size, _ = k_pages.shape
-    with _on(index):
-        out = _output_like(q, out, index)
-        lib = _native.lib()
-        need = lib.npu_b200_paged_decode_workspace_size(q_heads, kv_heads, head_dim)
-        ws = torch.empty(need, dtype=torch.uint8, device=q.device)
-        _native.check(lib.npu_b200_paged_decode(
-            q.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(), page_table.data_ptr(),
-            seq_lens.data_ptr(), out.data_ptr(), batch, q_heads, kv_heads, head_dim, num_pages,
-            page_size, page_table.shape[1], window, sinks,
-            head_dim ** -0.5 if scale is None else scale, ws.data_ptr(), need, _raw_stream(index)))
+    if _elsewhere(index):
+        with torch.cuda.device(index):
+            return paged_decode(q, k_pages, v_pages, page_table, seq_lens,
+                               window, sinks, scale, out)
+    out = _output_like(q, out, index)
+    need = _paged_decode_bytes(index, q_heads, kv_heads, head_dim)
+    ws = torch.empty(need, dtype=torch.uint8, device=q.device)
+    _native.check(_native.lib().npu_b200_paged_decode(
+        q.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(), page_table.data_ptr(),
+        seq_lens.data_ptr(), out.data_ptr(), batch, q_heads, kv_heads, head_dim, num_pages,
+        page_size, page_table.shape[1], window, sinks,
+        head_dim ** -0.5 if scale is None else scale, ws.data_ptr(), need, _raw_stream(index)))
     return out
 
 
@@ -224,13 +232,16 @@ def paged_prefill(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor,
     if q_lens is not None:
         _require_counts(index, q_lens, "q_lens", batch)
     num_pages, kv_heads, page_size, _ = k_pages.shape
-    with _on(index):
-        out = _output_like(q, out, index)
-        _native.check(_native.lib().npu_b200_paged_prefill(
-            q.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(), page_table.data_ptr(),
-            seq_lens.data_ptr(), 0 if q_lens is None else q_lens.data_ptr(), out.data_ptr(), batch,
-            q_heads, kv_heads, head_dim, queries, num_pages, page_size, page_table.shape[1],
-            window, sinks, head_dim ** -0.5 if scale is None else scale, _raw_stream(index)))
+    if _elsewhere(index):
+        with torch.cuda.device(index):
+            return paged_prefill(q, k_pages, v_pages, page_table, seq_lens,
+                                q_lens, window, sinks, scale, out)
+    out = _output_like(q, out, index)
+    _native.check(_native.lib().npu_b200_paged_prefill(
+        q.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(), page_table.data_ptr(),
+        seq_lens.data_ptr(), 0 if q_lens is None else q_lens.data_ptr(), out.data_ptr(), batch,
+        q_heads, kv_heads, head_dim, queries, num_pages, page_size, page_table.shape[1],
+        window, sinks, head_dim ** -0.5 if scale is None else scale, _raw_stream(index)))
     return out
 
 
@@ -252,12 +263,14 @@ def paged_append(k: torch.Tensor, v: torch.Tensor, k_pages: torch.Tensor, v_page
     _require_counts(index, starts, "starts", batch)
     if lens is not None:
         _require_counts(index, lens, "lens", batch)
-    with _on(index):
-        _native.check(_native.lib().npu_b200_paged_append(
-            k.data_ptr(), v.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(),
-            page_table.data_ptr(), starts.data_ptr(), 0 if lens is None else lens.data_ptr(),
-            batch, kv_heads, rows, head_dim, num_pages, page_size, page_table.shape[1],
-            _raw_stream(index)))
+    if _elsewhere(index):
+        with torch.cuda.device(index):
+            return paged_append(k, v, k_pages, v_pages, page_table, starts, lens)
+    _native.check(_native.lib().npu_b200_paged_append(
+        k.data_ptr(), v.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(),
+        page_table.data_ptr(), starts.data_ptr(), 0 if lens is None else lens.data_ptr(),
+        batch, kv_heads, rows, head_dim, num_pages, page_size, page_table.shape[1],
+        _raw_stream(index)))
 
 
 def page_update(page_table: torch.Tensor, seq_lens: torch.Tensor, parents: torch.Tensor,
@@ -278,16 +291,18 @@ def page_update(page_table: torch.Tensor, seq_lens: torch.Tensor, parents: torch
     new_rows, n = parents.shape[0], page_refs.shape[0]
     _require_counts(index, seq_lens, "seq_lens", rows)
     _require_counts(index, capacity, "capacity", new_rows)
-    with _on(index):
-        table = torch.empty_like(page_table) if new_rows == rows else page_table.new_empty(
-            (new_rows, entries))
-        lens, refs = torch.empty_like(parents), torch.empty_like(page_refs)
-        copies, info = page_refs.new_empty((2, new_rows)), page_refs.new_empty(3)
-        _native.check(_native.lib().npu_b200_page_update(
-            page_table.data_ptr(), seq_lens.data_ptr(), parents.data_ptr(), capacity.data_ptr(),
-            page_refs.data_ptr(), table.data_ptr(), lens.data_ptr(), refs.data_ptr(),
-            copies.data_ptr(), info.data_ptr(), rows, new_rows, entries, page_size, n,
-            _raw_stream(index)))
+    if _elsewhere(index):
+        with torch.cuda.device(index):
+            return page_update(page_table, seq_lens, parents, capacity, page_refs, page_size)
+    table = torch.empty_like(page_table) if new_rows == rows else page_table.new_empty(
+        (new_rows, entries))
+    lens, refs = torch.empty_like(parents), torch.empty_like(page_refs)
+    copies, info = page_refs.new_empty((2, new_rows)), page_refs.new_empty(3)
+    _native.check(_native.lib().npu_b200_page_update(
+        page_table.data_ptr(), seq_lens.data_ptr(), parents.data_ptr(), capacity.data_ptr(),
+        page_refs.data_ptr(), table.data_ptr(), lens.data_ptr(), refs.data_ptr(),
+        copies.data_ptr(), info.data_ptr(), rows, new_rows, entries, page_size, n,
+        _raw_stream(index)))
     return table, lens, refs, copies, info
 
 
@@ -303,14 +318,16 @@ def page_compact(page_table: torch.Tensor, page_refs: torch.Tensor
     _require_on(index, page_refs, "page_refs", torch.int32, 1)
     rows, entries = page_table.shape
     n = page_refs.shape[0]
-    with _on(index):
-        table, refs = torch.empty_like(page_table), torch.empty_like(page_refs)
-        where = torch.empty_like(page_refs)
-        moves, info = page_refs.new_empty((2, max(1, n // 2))), page_refs.new_empty(2)
-        _native.check(_native.lib().npu_b200_page_compact(
-            page_table.data_ptr(), page_refs.data_ptr(), table.data_ptr(), refs.data_ptr(),
-            moves.data_ptr(), where.data_ptr(), info.data_ptr(), rows, entries, n,
-            _raw_stream(index)))
+    if _elsewhere(index):
+        with torch.cuda.device(index):
+            return page_compact(page_table, page_refs)
+    table, refs = torch.empty_like(page_table), torch.empty_like(page_refs)
+    where = torch.empty_like(page_refs)
+    moves, info = page_refs.new_empty((2, max(1, n // 2))), page_refs.new_empty(2)
+    _native.check(_native.lib().npu_b200_page_compact(
+        page_table.data_ptr(), page_refs.data_ptr(), table.data_ptr(), refs.data_ptr(),
+        moves.data_ptr(), where.data_ptr(), info.data_ptr(), rows, entries, n,
+        _raw_stream(index)))
     return table, refs, moves, where, info
 
 
@@ -329,11 +346,13 @@ def page_copy(pool: torch.Tensor, pages: torch.Tensor, count: torch.Tensor | Non
         if count.shape[0] < 1:
             raise ValueError("count must hold a number")
     slabs, n = pool.shape[:2]
-    with _on(index):
-        _native.check(_native.lib().npu_b200_page_copy(
-            pool.data_ptr(), pages.data_ptr(), 0 if count is None else count.data_ptr(),
-            pages.shape[1], slabs, n, pool.numel() // (slabs * n) * pool.element_size(),
-            _raw_stream(index)))
+    if _elsewhere(index):
+        with torch.cuda.device(index):
+            return page_copy(pool, pages, count)
+    _native.check(_native.lib().npu_b200_page_copy(
+        pool.data_ptr(), pages.data_ptr(), 0 if count is None else count.data_ptr(),
+        pages.shape[1], slabs, n, pool.numel() // (slabs * n) * pool.element_size(),
+        _raw_stream(index)))
 
 
 def beam_select(logits: torch.Tensor, scores: torch.Tensor, width: int,
@@ -360,19 +379,21 @@ def beam_select(logits: torch.Tensor, scores: torch.Tensor, width: int,
             raise ValueError("done must have the shape of scores")
     if width < 1:
         raise ValueError(f"width must be positive, got {width}")
-    with _on(index):
-        lib = _native.lib()
-        out_scores = scores.new_empty((batch, width))
-        tokens = torch.empty_like(out_scores, dtype=torch.int32)
-        parents = torch.empty_like(tokens)
-        out_done = torch.empty_like(out_scores, dtype=torch.bool)
-        need = lib.npu_b200_beam_select_workspace_size(batch, beams, vocab, width)
-        ws = torch.empty(need, dtype=torch.uint8, device=logits.device)
-        _native.check(lib.npu_b200_beam_select(
-            logits.data_ptr(), logits.dtype is torch.float32, scores.data_ptr(),
-            0 if done is None else done.data_ptr(), out_scores.data_ptr(), tokens.data_ptr(),
-            parents.data_ptr(), out_done.data_ptr(), batch, beams, vocab, width, eos,
-            ws.data_ptr(), need, _raw_stream(index)))
+    if _elsewhere(index):
+        with torch.cuda.device(index):
+            return beam_select(logits, scores, width, done, eos)
+    lib = _native.lib()
+    out_scores = scores.new_empty((batch, width))
+    tokens = torch.empty_like(out_scores, dtype=torch.int32)
+    parents = torch.empty_like(tokens)
+    out_done = torch.empty_like(out_scores, dtype=torch.bool)
+    need = lib.npu_b200_beam_select_workspace_size(batch, beams, vocab, width)
+    ws = torch.empty(need, dtype=torch.uint8, device=logits.device)
+    _native.check(lib.npu_b200_beam_select(
+        logits.data_ptr(), logits.dtype is torch.float32, scores.data_ptr(),
+        0 if done is None else done.data_ptr(), out_scores.data_ptr(), tokens.data_ptr(),
+        parents.data_ptr(), out_done.data_ptr(), batch, beams, vocab, width, eos,
+        ws.data_ptr(), need, _raw_stream(index)))
     return out_scores, tokens, parents, out_done
 
 
@@ -385,17 +406,19 @@ def beam_reorder(state: torch.Tensor, parents: torch.Tensor, out: torch.Tensor |
         raise ValueError(f"state must be a contiguous [rows, ...], got {tuple(state.shape)}")
     _require_on(index, parents, "parents", torch.int32)
     rows, new_rows = state.shape[0], parents.numel()
-    with _on(index):
-        if out is None:
-            out = torch.empty_like(state) if new_rows == rows else state.new_empty(
-                (new_rows, *state.shape[1:]))
-        else:
-            _require_on(index, out, "out", state.dtype)
-            if out.shape != (new_rows, *state.shape[1:]):
-                raise ValueError(f"out must be {(new_rows, *state.shape[1:])}, got {tuple(out.shape)}")
-        _native.check(_native.lib().npu_b200_beam_reorder(
-            state.data_ptr(), parents.data_ptr(), out.data_ptr(), rows, new_rows,
-            state.numel() // rows * state.element_size(), _raw_stream(index)))
+    if _elsewhere(index):
+        with torch.cuda.device(index):
+            return beam_reorder(state, parents, out)
+    if out is None:
+        out = torch.empty_like(state) if new_rows == rows else state.new_empty(
+            (new_rows, *state.shape[1:]))
+    else:
+        _require_on(index, out, "out", state.dtype)
+        if out.shape != (new_rows, *state.shape[1:]):
+            raise ValueError(f"out must be {(new_rows, *state.shape[1:])}, got {tuple(out.shape)}")
+    _native.check(_native.lib().npu_b200_beam_reorder(
+        state.data_ptr(), parents.data_ptr(), out.data_ptr(), rows, new_rows,
+        state.numel() // rows * state.element_size(), _raw_stream(index)))
     return out
 
 

@@ -342,3 +342,29 @@ def test_append_drops_rows_without_a_page(cuda):
         _native.device_status()
     want = oracle.append_paged(new, k, table, starts)
     assert torch.equal(kg.cpu().view(torch.int16), want.view(torch.int16))
+
+
+@pytest.mark.gpu
+def test_calls_from_threads_and_streams(cuda):
+    """Two host threads, each with a stream of its own, at once."""
+    import threading
+    from llm_compiler_3_b200 import ops
+    lens = [900, 300]
+    k, v, table = (t.cuda() for t in paged_cache(lens, 2, 64, 32, seed=14))
+    n, qs = ints(lens).cuda(), [seeded((2, 8, 64), 70 + i).cuda() for i in range(2)]
+    want = [ops.paged_decode(q, k, v, table, n) for q in qs]
+    torch.cuda.synchronize()
+    bad = []
+
+    def work(i):
+        with torch.cuda.stream(torch.cuda.Stream()):
+            got = [ops.paged_decode(qs[i], k, v, table, n) for _ in range(200)]
+            torch.cuda.current_stream().synchronize()
+            bad.extend(1 for g in got if not torch.equal(g, want[i]))
+
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(2)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not bad
