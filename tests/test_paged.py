@@ -368,3 +368,32 @@ def test_calls_from_threads_and_streams(cuda):
     for t in threads:
         t.join()
     assert not bad
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dim,heads,kv_heads,lens,window", [
+    (128, 2, 1, [60000, 5, 0, 9000], 0), (64, 3, 1, [50000, 20000], 0), (64, 9, 1, [30000, 1], 0),
+    (128, 16, 1, [20000, 300, 7000], 0), (64, 2, 2, [1000, 0, 31, 400], 0), (128, 1, 1, [3], 0),
+    (64, 2, 1, [40000, 39000, 12], 9000)])
+def test_decode_of_wide_tables(cuda, dim, heads, kv_heads, lens, window):
+    """Tables with room for many more keys than there are: part of the work is dealt out
+    on the way, whatever there turns out to be.  The same bits each time."""
+    k, v, table = paged_cache(lens, kv_heads, dim, 16, seed=len(lens))
+    wide = torch.full((len(lens), 80000), -1, dtype=torch.int32)
+    wide[:, :table.shape[1]] = table
+    q = seeded((len(lens), heads, dim), 12)
+    kw = dict(window=window, sinks=3) if window else {}
+    if window:  # a window narrows what a table can hold: widen it in sequences instead
+        wide, q = wide.repeat(60, 1), q.repeat(60, 1, 1)
+        lens = lens * 60
+    first = _decode(q, k, v, wide, lens, **kw)
+    n = 3 if window else len(lens)
+    want, bound = oracle.attention_paged(q[:n, :, None], k, v, wide[:n], lens[:n],
+                                         q_lens=[min(1, x) for x in lens[:n]], **kw)
+    check(first[:n], want[:, :, 0], bound[:, :, 0])
+    if window:
+        # Every copy of a sequence is split at other places: near, not equal.
+        for c in range(1, 60):
+            check(first[3 * c:3 * c + 3], want[:, :, 0], bound[:, :, 0])
+    for _ in range(5):
+        assert torch.equal(_decode(q, k, v, wide, lens, **kw), first)
