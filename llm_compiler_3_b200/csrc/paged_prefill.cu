@@ -92,6 +92,11 @@ __device__ __forceinline__ void tmem_st32(uint32_t taddr, const uint32_t* r) {
       : "memory");
 }
 
+// A word whose first n bits are set.
+__device__ __forceinline__ uint32_t first_bits(int n) {
+  return n <= 0 ? 0u : n >= 32 ? ~0u : (1u << n) - 1u;
+}
+
 // What the two query tiles of a CTA cover.
 struct Span {
   int seq_len, q_len, first_pos;  // first_pos: position of query 0 of the chunk
@@ -370,11 +375,16 @@ __global__ void __launch_bounds__(kThreads, 1)
       for (int c = 0; c < KT; c += 32) tmem_ld32(t_s + c, sr + c);
       tmem_ld_wait();
       const int key0 = span.tiles.key0(j);
+      // Hidden keys, 32 to a word of bits (comparing key by key took 640 instructions).
       if (!__all_sync(0xffffffffu, key0 + KT - 1 <= last && (key0 >= lo || key0 + KT <= p.sinks))) {
 #pragma unroll
-        for (int e = 0; e < KT; ++e) {
-          const int key = key0 + e;
-          if (key > last || (key < lo && key >= p.sinks)) sr[e] = 0xff800000u;  // -inf
+        for (int c = 0; c < KT; c += 32) {
+          const uint32_t seen = first_bits(last + 1 - key0 - c) &
+                                (~first_bits(lo - key0 - c) | first_bits(p.sinks - key0 - c));
+          if (__all_sync(0xffffffffu, seen == ~0u)) continue;
+#pragma unroll
+          for (int e = 0; e < 32; ++e)
+            if (!(seen >> e & 1)) sr[c + e] = 0xff800000u;  // -inf
         }
       }
       float top[4];
