@@ -129,6 +129,23 @@ class Epilogue(ctypes.Structure):
     ]
 
 _lib = None
+_bound = None
+
+
+def bindings():
+    """The native binding of the paged-cache and beam operators (csrc/bindings.cpp); raises if
+    it is unavailable, like lib()."""
+    global _bound
+    if _bound is None:
+        lib()  # a missing library is named as such
+        try:
+            from . import _bindings
+        except ImportError as exc:
+            raise NativeUnavailable(
+                f"cannot load llm_compiler_3_b200/_bindings.so ({exc}): run "
+                "`python -m llm_compiler_3_b200.build`") from exc
+        _bound = _bindings
+    return _bound
 
 
 def lib() -> ctypes.CDLL:
@@ -169,5 +186,5 @@ def device_status() -> int:
     return bits.value
 
 
-__all__ = ["lib", "check", "device_status", "exported_symbols", "NativeUnavailable", "NpuError",
+__all__ = ["lib", "bindings", "check", "device_status", "exported_symbols", "NativeUnavailable", "NpuError",
            "LIBRARY", "HEADER", "c_void_p", "c_int", "c_int32", "c_float", "c_size_t", "c_uint64"]

@@ -24,6 +24,7 @@ INCLUDE = ROOT / "include"
 BUILD = ROOT / "_build"
 LIBDIR = PACKAGE / "lib"
 LIBRARY = LIBDIR / "libnpu_b200.so"
+BINDINGS = PACKAGE / "_bindings.so"
 
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
 NVCC_FLAGS = ARCH + [
@@ -57,8 +58,36 @@ def _compile(src: Path, force: bool, hdr_mtime: float, extra: list[str]) -> Path
     return obj
 
 
+def _build_bindings(force: bool, hdr_mtime: float) -> None:
+    """The Python binding of the paged-cache and beam operators (csrc/bindings.cpp): C++ against
+    torch's headers, calling the library next to it."""
+    import sysconfig
+
+    import torch
+    from torch.utils.cpp_extension import include_paths, library_paths
+    src = CSRC / "bindings.cpp"
+    if (not force and BINDINGS.exists()
+            and BINDINGS.stat().st_mtime >= max(src.stat().st_mtime, hdr_mtime)):
+        return
+    cuda = Path(nvcc()).resolve().parent.parent
+    tmp = BINDINGS.with_suffix(".so.tmp")
+    cmd = ["g++", "-O2", "-std=c++17", "-shared", "-fPIC", "-fvisibility=hidden",
+           f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
+           "-I", str(INCLUDE), "-isystem", str(cuda / "include"),
+           *[x for p in include_paths() for x in ("-isystem", p)],
+           "-isystem", sysconfig.get_path("include"), str(src), "-o", str(tmp),
+           *[f"-L{p}" for p in library_paths()], "-lc10", "-ltorch_cpu", "-ltorch", "-lc10_cuda",
+           "-ltorch_cuda", "-ltorch_python", f"-L{LIBDIR}", "-lnpu_b200",
+           "-Wl,-rpath,$ORIGIN/lib", *[f"-Wl,-rpath,{p}" for p in library_paths()]]
+    done = subprocess.run(cmd, capture_output=True, text=True)
+    if done.returncode:
+        raise RuntimeError(f"g++ failed on {src.name}:\n{done.stdout}\n{done.stderr}")
+    os.replace(tmp, BINDINGS)
+
+
 def build(force: bool = False, jobs: int | None = None, verbose_ptxas: bool = False) -> Path:
-    """Compile every csrc/*.cu for sm_100a and link libnpu_b200.so; return its path."""
+    """Compile every csrc/*.cu for sm_100a, link libnpu_b200.so, build the Python binding that
+    calls it; return the library's path."""
     BUILD.mkdir(exist_ok=True)
     LIBDIR.mkdir(exist_ok=True)
     sources = sorted(CSRC.glob("*.cu"))
@@ -75,6 +104,7 @@ def build(force: bool = False, jobs: int | None = None, verbose_ptxas: bool = Fa
         if done.returncode:
             raise RuntimeError(f"link of libnpu_b200.so failed:\n{done.stdout}\n{done.stderr}")
         os.replace(tmp, LIBRARY)
+    _build_bindings(force, hdr)
     return LIBRARY
 
 

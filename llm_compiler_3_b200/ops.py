@@ -7,7 +7,6 @@ here runs a libnpu_b200 kernel and nothing else.  Inputs must be CUDA, FP16
 from __future__ import annotations
 
 import ctypes
-from functools import lru_cache
 
 import torch
 
@@ -118,73 +117,13 @@ def prefill_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Ten
 
 
 # ---------------------------------------------------------------------------
-# Paged key-value cache (the layout and the rules are in include/npu_b200.h).
-#
-# These operators run on the device of their tensors, whichever is current, on
-# that device's current stream; scratch comes from torch's allocator at each
-# call, so calls on several streams and captured graphs share none.
+# Paged key-value cache and beam search (the layouts and rules are in
+# include/npu_b200.h).  These calls are short, so their checks, outputs and scratch
+# are made in the native binding (csrc/bindings.cpp): they run on the device of their
+# tensors, whichever is current, on that device's current stream, and scratch comes
+# from torch's allocator at each call, so calls on several streams and captured graphs
+# share none.
 # ---------------------------------------------------------------------------
-def _device_index(t: torch.Tensor, name: str) -> int:
-    if not isinstance(t, torch.Tensor) or not t.is_cuda:
-        raise ValueError(f"{name} must be a CUDA tensor")
-    return t.get_device()
-
-
-def _elsewhere(index: int) -> bool:
-    """Whether another device than that one is current (the operator then calls itself with
-    it current)."""
-    return torch._C._cuda_getDevice() != index
-
-
-def _require_on(index: int, t: torch.Tensor, name: str, dtype: torch.dtype = torch.float16,
-                ndim: int | None = None) -> None:
-    """_require, on the device of that index (in one expression: these calls are short, and
-    their checks count)."""
-    if (isinstance(t, torch.Tensor) and t.dtype is dtype and t.get_device() == index
-            and t.is_contiguous() and (ndim is None or t.dim() == ndim)):
-        return
-    _require(t, name, dtype, ndim)
-    raise ValueError(f"{name} is on {t.device}, not on cuda:{index}")
-
-
-def _require_pages(index: int, k_pages: torch.Tensor, v_pages: torch.Tensor,
-                   page_table: torch.Tensor, batch: int, head_dim: int) -> None:
-    _require_on(index, k_pages, "k_pages", ndim=4)
-    _require_on(index, v_pages, "v_pages", ndim=4)
-    _require_on(index, page_table, "page_table", torch.int32, 2)
-    if v_pages.shape != k_pages.shape or k_pages.shape[3] != head_dim:
-        raise ValueError(f"k_pages {tuple(k_pages.shape)}, v_pages {tuple(v_pages.shape)} and "
-                         f"head_dim {head_dim} disagree")
-    if page_table.shape[0] != batch:
-        raise ValueError("page_table must have one row per sequence")
-
-
-def _require_counts(index: int, t: torch.Tensor, name: str, batch: int) -> None:
-    _require_on(index, t, name, torch.int32, 1)
-    if t.shape[0] != batch:
-        raise ValueError(f"{name} must have one entry per sequence")
-
-
-def _output_like(like: torch.Tensor, out: torch.Tensor | None, index: int) -> torch.Tensor:
-    if out is None:
-        return torch.empty_like(like)
-    _require_on(index, out, "out", like.dtype)
-    if out.shape != like.shape:
-        raise ValueError(f"out must be {tuple(like.shape)}, got {tuple(out.shape)}")
-    return out
-
-
-@lru_cache(maxsize=None)
-def _paged_decode_bytes(index: int, q_heads: int, kv_heads: int, head_dim: int) -> int:
-    return _native.lib().npu_b200_paged_decode_workspace_size(q_heads, kv_heads, head_dim)
-
-
-def _raw_stream(index: int) -> int:
-    """The current stream of a device as a number (torch.cuda.current_stream() builds an
-    object around it, which takes longer than a launch)."""
-    return torch._C._cuda_getCurrentRawStream(index)
-
-
 def paged_decode(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor,
                  page_table: torch.Tensor, seq_lens: torch.Tensor, window: int = 0,
                  sinks: int = 0, scale: float | None = None, out: torch.Tensor | None = None
@@ -194,25 +133,8 @@ def paged_decode(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor,
 
     Returns out [B, Hq, D] FP16 = softmax(scale q K^T) V over keys [0, seq_lens[b]), with
     window > 0 over the last `window` of them and the first `sinks`; zero without keys."""
-    index = _device_index(q, "q")
-    _require(q, "q", ndim=3)
-    batch, q_heads, head_dim = q.shape
-    _require_pages(index, k_pages, v_pages, page_table, batch, head_dim)
-    _require_counts(index, seq_lens, "seq_lens", batch)
-    num_pages, kv_heads, page_size, _ = k_pages.shape
-    if _elsewhere(index):
-        with torch.cuda.device(index):
-            return paged_decode(q, k_pages, v_pages, page_table, seq_lens,
-                               window, sinks, scale, out)
-    out = _output_like(q, out, index)
-    need = _paged_decode_bytes(index, q_heads, kv_heads, head_dim)
-    ws = torch.empty(need, dtype=torch.uint8, device=q.device)
-    _native.check(_native.lib().npu_b200_paged_decode(
-        q.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(), page_table.data_ptr(),
-        seq_lens.data_ptr(), out.data_ptr(), batch, q_heads, kv_heads, head_dim, num_pages,
-        page_size, page_table.shape[1], window, sinks,
-        head_dim ** -0.5 if scale is None else scale, ws.data_ptr(), need, _raw_stream(index)))
-    return out
+    return _native.bindings().paged_decode(q, k_pages, v_pages, page_table, seq_lens, window,
+                                           sinks, scale, out)
 
 
 def paged_prefill(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor,
@@ -224,25 +146,8 @@ def paged_prefill(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor,
     seq_lens[b] - q_lens[b] + i.
 
     Returns out [B, Hq, M, D] FP16; rows past q_lens[b] or without a visible key are zero."""
-    index = _device_index(q, "q")
-    _require(q, "q", ndim=4)
-    batch, q_heads, queries, head_dim = q.shape
-    _require_pages(index, k_pages, v_pages, page_table, batch, head_dim)
-    _require_counts(index, seq_lens, "seq_lens", batch)
-    if q_lens is not None:
-        _require_counts(index, q_lens, "q_lens", batch)
-    num_pages, kv_heads, page_size, _ = k_pages.shape
-    if _elsewhere(index):
-        with torch.cuda.device(index):
-            return paged_prefill(q, k_pages, v_pages, page_table, seq_lens,
-                                q_lens, window, sinks, scale, out)
-    out = _output_like(q, out, index)
-    _native.check(_native.lib().npu_b200_paged_prefill(
-        q.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(), page_table.data_ptr(),
-        seq_lens.data_ptr(), 0 if q_lens is None else q_lens.data_ptr(), out.data_ptr(), batch,
-        q_heads, kv_heads, head_dim, queries, num_pages, page_size, page_table.shape[1],
-        window, sinks, head_dim ** -0.5 if scale is None else scale, _raw_stream(index)))
-    return out
+    return _native.bindings().paged_prefill(q, k_pages, v_pages, page_table, seq_lens, q_lens,
+                                            window, sinks, scale, out)
 
 
 def paged_append(k: torch.Tensor, v: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor,
@@ -250,27 +155,7 @@ def paged_append(k: torch.Tensor, v: torch.Tensor, k_pages: torch.Tensor, v_page
                  lens: torch.Tensor | None = None) -> None:
     """New keys and values into the pages, in place: k, v [B, Hkv, M, D]; row i < lens[b]
     (default: every row) of sequence b goes to position starts[b] + i."""
-    index = _device_index(k, "k")
-    _require(k, "k", ndim=4)
-    _require_on(index, v, "v", ndim=4)
-    batch, kv_heads, rows, head_dim = k.shape
-    if v.shape != k.shape:
-        raise ValueError("k and v must have one shape")
-    _require_pages(index, k_pages, v_pages, page_table, batch, head_dim)
-    num_pages, heads, page_size, _ = k_pages.shape
-    if heads != kv_heads:
-        raise ValueError(f"k has {kv_heads} heads but the pages {heads}")
-    _require_counts(index, starts, "starts", batch)
-    if lens is not None:
-        _require_counts(index, lens, "lens", batch)
-    if _elsewhere(index):
-        with torch.cuda.device(index):
-            return paged_append(k, v, k_pages, v_pages, page_table, starts, lens)
-    _native.check(_native.lib().npu_b200_paged_append(
-        k.data_ptr(), v.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(),
-        page_table.data_ptr(), starts.data_ptr(), 0 if lens is None else lens.data_ptr(),
-        batch, kv_heads, rows, head_dim, num_pages, page_size, page_table.shape[1],
-        _raw_stream(index)))
+    _native.bindings().paged_append(k, v, k_pages, v_pages, page_table, starts, lens)
 
 
 def page_update(page_table: torch.Tensor, seq_lens: torch.Tensor, parents: torch.Tensor,
@@ -283,27 +168,8 @@ def page_update(page_table: torch.Tensor, seq_lens: torch.Tensor, parents: torch
     Returns (table [R', E], lens [R'], refs [N], copies [2, R'], info [3]): pages to copy
     (from, to; packed) for `page_copy`, and info = free pages left, pages short, copies.
     The inputs stay as they are, so a step that ran short can be repeated."""
-    index = _device_index(page_table, "page_table")
-    _require(page_table, "page_table", torch.int32, 2)
-    _require_on(index, page_refs, "page_refs", torch.int32, 1)
-    _require_on(index, parents, "parents", torch.int32, 1)
-    rows, entries = page_table.shape
-    new_rows, n = parents.shape[0], page_refs.shape[0]
-    _require_counts(index, seq_lens, "seq_lens", rows)
-    _require_counts(index, capacity, "capacity", new_rows)
-    if _elsewhere(index):
-        with torch.cuda.device(index):
-            return page_update(page_table, seq_lens, parents, capacity, page_refs, page_size)
-    table = torch.empty_like(page_table) if new_rows == rows else page_table.new_empty(
-        (new_rows, entries))
-    lens, refs = torch.empty_like(parents), torch.empty_like(page_refs)
-    copies, info = page_refs.new_empty((2, new_rows)), page_refs.new_empty(3)
-    _native.check(_native.lib().npu_b200_page_update(
-        page_table.data_ptr(), seq_lens.data_ptr(), parents.data_ptr(), capacity.data_ptr(),
-        page_refs.data_ptr(), table.data_ptr(), lens.data_ptr(), refs.data_ptr(),
-        copies.data_ptr(), info.data_ptr(), rows, new_rows, entries, page_size, n,
-        _raw_stream(index)))
-    return table, lens, refs, copies, info
+    return _native.bindings().page_update(page_table, seq_lens, parents, capacity, page_refs,
+                                          page_size)
 
 
 def page_compact(page_table: torch.Tensor, page_refs: torch.Tensor
@@ -313,46 +179,14 @@ def page_compact(page_table: torch.Tensor, page_refs: torch.Tensor
     Returns (table, refs, moves [2, max(1, N // 2)], index [N], info [2]): pages to copy (from,
     to; packed), where each page is now (-1: free), and info = pages in use, moves.  Move the
     data with `page_copy(pool, moves, info[1:])` before the next use of the new table."""
-    index = _device_index(page_table, "page_table")
-    _require(page_table, "page_table", torch.int32, 2)
-    _require_on(index, page_refs, "page_refs", torch.int32, 1)
-    rows, entries = page_table.shape
-    n = page_refs.shape[0]
-    if _elsewhere(index):
-        with torch.cuda.device(index):
-            return page_compact(page_table, page_refs)
-    table, refs = torch.empty_like(page_table), torch.empty_like(page_refs)
-    where = torch.empty_like(page_refs)
-    moves, info = page_refs.new_empty((2, max(1, n // 2))), page_refs.new_empty(2)
-    _native.check(_native.lib().npu_b200_page_compact(
-        page_table.data_ptr(), page_refs.data_ptr(), table.data_ptr(), refs.data_ptr(),
-        moves.data_ptr(), where.data_ptr(), info.data_ptr(), rows, entries, n,
-        _raw_stream(index)))
-    return table, refs, moves, where, info
+    return _native.bindings().page_compact(page_table, page_refs)
 
 
 def page_copy(pool: torch.Tensor, pages: torch.Tensor, count: torch.Tensor | None = None) -> None:
     """Copies pages in place, in every slab of a pool [slabs, N, ...] of any type (K and V of
     every layer): pages [2, n] int32 (from, to), the first count[0] of them (default: all; -1
     pairs are skipped).  No page that is written may be named twice."""
-    index = _device_index(pool, "pool")
-    if not pool.is_contiguous() or pool.dim() < 3 or pool.numel() == 0:
-        raise ValueError(f"pool must be a contiguous [slabs, pages, ...], got {tuple(pool.shape)}")
-    _require_on(index, pages, "pages", torch.int32, 2)
-    if pages.shape[0] != 2:
-        raise ValueError("pages must be [2, n]: from and to")
-    if count is not None:
-        _require_on(index, count, "count", torch.int32, 1)
-        if count.shape[0] < 1:
-            raise ValueError("count must hold a number")
-    slabs, n = pool.shape[:2]
-    if _elsewhere(index):
-        with torch.cuda.device(index):
-            return page_copy(pool, pages, count)
-    _native.check(_native.lib().npu_b200_page_copy(
-        pool.data_ptr(), pages.data_ptr(), 0 if count is None else count.data_ptr(),
-        pages.shape[1], slabs, n, pool.numel() // (slabs * n) * pool.element_size(),
-        _raw_stream(index)))
+    _native.bindings().page_copy(pool, pages, count)
 
 
 def beam_select(logits: torch.Tensor, scores: torch.Tensor, width: int,
@@ -365,61 +199,14 @@ def beam_select(logits: torch.Tensor, scores: torch.Tensor, width: int,
     Returns (scores [B, width] FP32, tokens, parents [B, width] int32, done [B, width] bool),
     best first, the lowest beam x V + token among equals; parents are rows b x W + beam.  Where
     nothing is left: -inf, -1, -1, False."""
-    index = _device_index(logits, "logits")
-    if logits.dtype not in (torch.float16, torch.float32):
-        raise ValueError(f"logits must be float16 or float32, got {logits.dtype}")
-    _require(logits, "logits", logits.dtype, 3)
-    _require_on(index, scores, "scores", torch.float32, 2)
-    batch, beams, vocab = logits.shape
-    if scores.shape != (batch, beams):
-        raise ValueError(f"scores must be {(batch, beams)}, got {tuple(scores.shape)}")
-    if done is not None:
-        _require_on(index, done, "done", torch.bool, 2)
-        if done.shape != scores.shape:
-            raise ValueError("done must have the shape of scores")
-    if width < 1:
-        raise ValueError(f"width must be positive, got {width}")
-    if _elsewhere(index):
-        with torch.cuda.device(index):
-            return beam_select(logits, scores, width, done, eos)
-    lib = _native.lib()
-    out_scores = scores.new_empty((batch, width))
-    tokens = torch.empty_like(out_scores, dtype=torch.int32)
-    parents = torch.empty_like(tokens)
-    out_done = torch.empty_like(out_scores, dtype=torch.bool)
-    need = lib.npu_b200_beam_select_workspace_size(batch, beams, vocab, width)
-    ws = torch.empty(need, dtype=torch.uint8, device=logits.device)
-    _native.check(lib.npu_b200_beam_select(
-        logits.data_ptr(), logits.dtype is torch.float32, scores.data_ptr(),
-        0 if done is None else done.data_ptr(), out_scores.data_ptr(), tokens.data_ptr(),
-        parents.data_ptr(), out_done.data_ptr(), batch, beams, vocab, width, eos,
-        ws.data_ptr(), need, _raw_stream(index)))
-    return out_scores, tokens, parents, out_done
+    return _native.bindings().beam_select(logits, scores, width, done, eos)
 
 
 def beam_reorder(state: torch.Tensor, parents: torch.Tensor, out: torch.Tensor | None = None
                  ) -> torch.Tensor:
     """Rows of a per-beam state [R, ...] of any type in their new order: out[r] =
     state[parents[r]] for parents of any shape with R' numbers; -1 gives a zero row."""
-    index = _device_index(state, "state")
-    if not state.is_contiguous() or state.dim() < 1 or state.numel() == 0:
-        raise ValueError(f"state must be a contiguous [rows, ...], got {tuple(state.shape)}")
-    _require_on(index, parents, "parents", torch.int32)
-    rows, new_rows = state.shape[0], parents.numel()
-    if _elsewhere(index):
-        with torch.cuda.device(index):
-            return beam_reorder(state, parents, out)
-    if out is None:
-        out = torch.empty_like(state) if new_rows == rows else state.new_empty(
-            (new_rows, *state.shape[1:]))
-    else:
-        _require_on(index, out, "out", state.dtype)
-        if out.shape != (new_rows, *state.shape[1:]):
-            raise ValueError(f"out must be {(new_rows, *state.shape[1:])}, got {tuple(out.shape)}")
-    _native.check(_native.lib().npu_b200_beam_reorder(
-        state.data_ptr(), parents.data_ptr(), out.data_ptr(), rows, new_rows,
-        state.numel() // rows * state.element_size(), _raw_stream(index)))
-    return out
+    return _native.bindings().beam_reorder(state, parents, out)
 
 
 def linear(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | None = None,
