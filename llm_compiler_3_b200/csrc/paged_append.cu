@@ -1,12 +1,14 @@
 // New keys and values into the pages of a paged cache (paged.cuh): row i of
 // sequence b goes to position starts[b] + i.  A copy, bound by HBM (or, for one
-// row per sequence, by the launch): each thread moves 16 bytes of K and of V.
+// row per sequence, by the launch): each thread moves 16 bytes of K and of V of
+// four rows, all eight loads in flight before the first store.
 #include "paged.cuh"
 
 namespace npu_b200 {
 namespace {
 
 constexpr int kAppendThreads = 256;
+constexpr int kAtOnce = 4;  // rows of a thread
 
 struct AppendParams {
   const uint4* k;
@@ -16,36 +18,51 @@ struct AppendParams {
   const int32_t* table;
   const int32_t* starts;
   const int32_t* lens;  // or null: every row
-  int batch, kv_heads, rows, vecs;  // vecs: 16-byte words of a row
+  int kv_heads, rows;
   int entries, page_size, num_pages;
 };
 
-// Grid (words of one sequence's new rows, sequence).
+// Grid (lines, sequence): a line is one row of one head, VECS 16-byte words.
+template <int VECS>
 __global__ void __launch_bounds__(kAppendThreads) paged_append_kernel(const AppendParams p) {
+  constexpr int kLines = kAppendThreads / VECS;  // at a time
   pdl_launch_dependents();
   pdl_wait();
-  const int b = blockIdx.y;
+  const int b = blockIdx.y, x = threadIdx.x % VECS;
   const int n = p.lens != nullptr ? min(max(p.lens[b], 0), p.rows) : p.rows;
   const long long start = p.starts[b];
-  const long long words = static_cast<long long>(p.kv_heads) * p.rows * p.vecs;
-  for (long long w = blockIdx.x * static_cast<long long>(kAppendThreads) + threadIdx.x; w < words;
-       w += static_cast<long long>(gridDim.x) * kAppendThreads) {
-    const int row = static_cast<int>(w / p.vecs), x = static_cast<int>(w - static_cast<long long>(row) * p.vecs);
-    const int h = row / p.rows, i = row - h * p.rows;
-    if (i >= n) continue;
-    const long long at = start + i;
-    const long long entry = at / p.page_size;
-    int page = -1;
-    if (at >= 0 && entry < p.entries) page = p.table[static_cast<size_t>(b) * p.entries + entry];
-    if (page < 0 || page >= p.num_pages) {
-      report_error(kDevErrBounds);
-      continue;
+  const int lines = p.kv_heads * p.rows;
+  const uint4* k = p.k + static_cast<size_t>(b) * lines * VECS;
+  const uint4* v = p.v + static_cast<size_t>(b) * lines * VECS;
+  const int32_t* table = p.table + static_cast<size_t>(b) * p.entries;
+  for (int line0 = blockIdx.x * kLines * kAtOnce + threadIdx.x / VECS; line0 < lines;
+       line0 += gridDim.x * kLines * kAtOnce) {
+    uint4 kv[kAtOnce], vv[kAtOnce];
+    size_t to[kAtOnce];
+    bool ok[kAtOnce];
+#pragma unroll
+    for (int u = 0; u < kAtOnce; ++u) {
+      const int line = line0 + u * kLines;
+      const int h = line / p.rows, i = line - h * p.rows;
+      ok[u] = line < lines && i < n;
+      if (!ok[u]) continue;
+      const size_t from = static_cast<size_t>(line) * VECS + x;
+      kv[u] = __ldcs(k + from);
+      vv[u] = __ldcs(v + from);
+      const long long at = start + i;
+      const long long entry = at >= 0 ? at / p.page_size : -1;
+      const int page = entry >= 0 && entry < p.entries ? table[entry] : -1;
+      ok[u] = page >= 0 && page < p.num_pages;
+      if (!ok[u]) report_error(kDevErrBounds);
+      to[u] = ((static_cast<size_t>(page) * p.kv_heads + h) * p.page_size +
+               static_cast<int>(at - entry * p.page_size)) * VECS + x;
     }
-    const size_t src = (static_cast<size_t>(b) * p.kv_heads * p.rows + row) * p.vecs + x;
-    const size_t dst = ((static_cast<size_t>(page) * p.kv_heads + h) * p.page_size +
-                        static_cast<int>(at - entry * p.page_size)) * p.vecs + x;
-    p.k_pages[dst] = p.k[src];
-    p.v_pages[dst] = p.v[src];
+#pragma unroll
+    for (int u = 0; u < kAtOnce; ++u)
+      if (ok[u]) {
+        p.k_pages[to[u]] = kv[u];
+        p.v_pages[to[u]] = vv[u];
+      }
   }
 }
 
@@ -64,7 +81,7 @@ extern "C" int npu_b200_paged_append(const void* d_k, const void* d_v, void* d_k
   int rc = check_pages("paged_append", kv_heads, head_dim, num_pages, page_size, table_entries);
   if (rc) return rc;
   NPU_REQUIRE(batch >= 1 && batch <= 65535, "paged_append: batch %d not in [1, 65535]", batch);
-  NPU_REQUIRE(rows >= 1 && static_cast<long long>(rows) * kv_heads < (1ll << 31),
+  NPU_REQUIRE(rows >= 1 && static_cast<long long>(rows) * kv_heads < (1ll << 30),
               "paged_append: %d rows out of range", rows);
   NPU_REQUIRE(aligned16(d_k) && aligned16(d_v) && aligned16(d_k_pages) && aligned16(d_v_pages),
               "paged_append: k, v and pages must be 16-byte aligned");
@@ -76,19 +93,18 @@ extern "C" int npu_b200_paged_append(const void* d_k, const void* d_v, void* d_k
   p.table = d_page_table;
   p.starts = d_starts;
   p.lens = d_lens;
-  p.batch = batch;
   p.kv_heads = kv_heads;
   p.rows = rows;
-  p.vecs = head_dim / 8;
   p.entries = table_entries;
   p.page_size = page_size;
   p.num_pages = num_pages;
-  const long long words = static_cast<long long>(kv_heads) * rows * p.vecs;
-  const long long blocks = (words + kAppendThreads - 1) / kAppendThreads;
+  const int vecs = head_dim / 8;
+  const long long per_block = kAppendThreads / vecs * kAtOnce;
+  const long long blocks = (static_cast<long long>(kv_heads) * rows + per_block - 1) / per_block;
   LaunchCfg cfg;
   cfg.grid = dim3(static_cast<unsigned>(blocks < 65536 ? blocks : 65536), batch);
   cfg.block = dim3(kAppendThreads);
   cfg.stream = static_cast<cudaStream_t>(stream);
   cfg.pdl = true;
-  return launch(cfg, paged_append_kernel, p);
+  return head_dim == 128 ? launch(cfg, paged_append_kernel<16>, p) : launch(cfg, paged_append_kernel<8>, p);
 }
