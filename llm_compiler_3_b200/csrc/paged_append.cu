@@ -20,6 +20,7 @@ struct AppendParams {
   const int32_t* lens;  // or null: every row
   int kv_heads, rows;
   int entries, page_size, num_pages;
+  Divisor by_rows, by_page;
 };
 
 // Grid (lines, sequence): a line is one row of one head, VECS 16-byte words.
@@ -43,19 +44,19 @@ __global__ void __launch_bounds__(kAppendThreads) paged_append_kernel(const Appe
 #pragma unroll
     for (int u = 0; u < kAtOnce; ++u) {
       const int line = line0 + u * kLines;
-      const int h = line / p.rows, i = line - h * p.rows;
+      const int h = p.rows > 1 ? p.by_rows.quotient(line) : line, i = line - h * p.rows;
       ok[u] = line < lines && i < n;
       if (!ok[u]) continue;
       const size_t from = static_cast<size_t>(line) * VECS + x;
       kv[u] = __ldcs(k + from);
       vv[u] = __ldcs(v + from);
       const long long at = start + i;
-      const long long entry = at >= 0 ? at / p.page_size : -1;
-      const int page = entry >= 0 && entry < p.entries ? table[entry] : -1;
+      const bool inside = at >= 0 && at < static_cast<long long>(p.entries) * p.page_size;  // below 2^31
+      const int pos = inside ? static_cast<int>(at) : 0, entry = p.by_page.quotient(pos);
+      const int page = inside ? table[entry] : -1;
       ok[u] = page >= 0 && page < p.num_pages;
       if (!ok[u]) report_error(kDevErrBounds);
-      to[u] = ((static_cast<size_t>(page) * p.kv_heads + h) * p.page_size +
-               static_cast<int>(at - entry * p.page_size)) * VECS + x;
+      to[u] = ((static_cast<size_t>(page) * p.kv_heads + h) * p.page_size + pos - entry * p.page_size) * VECS + x;
     }
 #pragma unroll
     for (int u = 0; u < kAtOnce; ++u)
@@ -98,6 +99,8 @@ extern "C" int npu_b200_paged_append(const void* d_k, const void* d_v, void* d_k
   p.entries = table_entries;
   p.page_size = page_size;
   p.num_pages = num_pages;
+  p.by_rows = Divisor::of(rows > 1 ? rows : 2);
+  p.by_page = Divisor::of(page_size);
   const int vecs = head_dim / 8;
   const long long per_block = kAppendThreads / vecs * kAtOnce;
   const long long blocks = (static_cast<long long>(kv_heads) * rows + per_block - 1) / per_block;
