@@ -65,6 +65,13 @@ __device__ __forceinline__ void cluster_share(int mine, int* s_all) {
   }
 }
 
+__device__ __forceinline__ void cluster_arrive() {
+  asm volatile("barrier.cluster.arrive.release;" ::: "memory");
+}
+__device__ __forceinline__ void cluster_wait() {
+  asm volatile("barrier.cluster.wait.acquire;" ::: "memory");
+}
+
 __device__ __forceinline__ int ld_fresh(const int32_t* p) { return __ldcg(p); }
 
 // The pages of warp w of the cluster: a contiguous stretch, so that ranks follow
@@ -84,6 +91,7 @@ struct UpdateParams {
   const int32_t *table, *lens, *parents, *capacity, *refs;
   int32_t *new_table, *new_lens, *new_refs, *copies, *info;
   int rows, new_rows, entries, page_size, num_pages;
+  Divisor by_page;
 };
 
 // One new row, in shared memory: what it keeps of its parent.
@@ -106,7 +114,7 @@ __global__ void __launch_bounds__(kThreads) page_update_kernel(const UpdateParam
   int32_t* first = smem_i;                             // [rows] lowest new row of each old one
   Row* row = reinterpret_cast<Row*>(first + p.rows);   // [new_rows]
   __shared__ long long s_scan[kWarpsPerCta];
-  __shared__ int s_sum[kWarpsPerCta], s_free[kCtas], s_copies;
+  __shared__ int s_sum[kWarpsPerCta], s_free[kCtas];
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int rank = static_cast<int>(cluster_ctarank());
   const int all_threads = kCtas * kThreads, me = rank * kThreads + tid;
@@ -114,9 +122,10 @@ __global__ void __launch_bounds__(kThreads) page_update_kernel(const UpdateParam
   pdl_launch_dependents();
   pdl_wait();
 
+#pragma unroll 4
   for (int i = me; i < p.num_pages; i += all_threads) p.new_refs[i] = p.refs[i];
+  cluster_arrive();  // the counts are waited for once the rows are laid out
   for (int r = tid; r < p.rows; r += kThreads) first[r] = INT_MAX;
-  if (tid == 0) s_copies = 0;
   __syncthreads();
   const int each = (p.new_rows + kThreads - 1) / kThreads;
   const int b0 = min(tid * each, p.new_rows), b1 = min(b0 + each, p.new_rows);
@@ -133,7 +142,7 @@ __global__ void __launch_bounds__(kThreads) page_update_kernel(const UpdateParam
     } else {
       r.parent = -1;
     }
-    const int full = r.len / p.page_size, part = r.len - full * p.page_size;
+    const int full = p.by_page.quotient(r.len), part = r.len - full * p.page_size;
     if (part > 0) {
       r.last = p.table[static_cast<size_t>(r.parent) * p.entries + full];
       if (r.last >= 0 && r.last < p.num_pages)
@@ -141,7 +150,7 @@ __global__ void __launch_bounds__(kThreads) page_update_kernel(const UpdateParam
       else
         r.last = -1;
     }
-    r.need = (max(cap, r.len) + p.page_size - 1) / p.page_size - full - (part > 0);
+    r.need = p.by_page.quotient(max(cap, r.len) + p.page_size - 1) - full - (part > 0);
     row[b] = r;
   }
   __syncthreads();
@@ -161,13 +170,14 @@ __global__ void __launch_bounds__(kThreads) page_update_kernel(const UpdateParam
     at_row += n;
   }
   const int wanted = static_cast<int>(total & 0xffffffffll);
-  cluster_sync_all();
+  __syncthreads();
+  cluster_wait();
 
   // One warp per piece of a row, so that few long rows spread over the cluster too.
   const long long pieces = (p.entries + kRowPiece - 1) / kRowPiece;
   const long long warps = kCtas * kWarpsPerCta, my_warp = rank * kWarpsPerCta + warp;
   for (long long w = my_warp; w < p.rows * pieces; w += warps) {
-    const int r = static_cast<int>(w / pieces);
+    const int r = static_cast<int>(pieces == 1 ? w : w / pieces);
     const int e0 = static_cast<int>(w - r * pieces) * kRowPiece;
 #pragma unroll 4
     for (int e = e0 + lane; e < min(e0 + kRowPiece, p.entries); e += 32) {
@@ -176,10 +186,10 @@ __global__ void __launch_bounds__(kThreads) page_update_kernel(const UpdateParam
     }
   }
   for (long long w = my_warp; w < p.new_rows * pieces; w += warps) {
-    const int b = static_cast<int>(w / pieces);
+    const int b = static_cast<int>(pieces == 1 ? w : w / pieces);
     const int e0 = static_cast<int>(w - b * pieces) * kRowPiece;
     const Row r = row[b];
-    const int full = r.len / p.page_size;
+    const int full = p.by_page.quotient(r.len);
     const bool keeps = r.last >= 0 && !(r.copy & 1);
 #pragma unroll 4
     for (int e = e0 + lane; e < min(e0 + kRowPiece, p.entries); e += 32) {
@@ -233,7 +243,7 @@ __global__ void __launch_bounds__(kThreads) page_update_kernel(const UpdateParam
       }
       const Row r = row[lo];
       const bool copies = r.copy & 1;
-      const int j = k - r.need, full = r.len / p.page_size;
+      const int j = k - r.need, full = p.by_page.quotient(r.len);
       const int e = full + j + (r.len > full * p.page_size && !copies);
       p.new_table[static_cast<size_t>(lo) * p.entries + e] = page;
       p.new_refs[page] = 1;
@@ -244,16 +254,15 @@ __global__ void __launch_bounds__(kThreads) page_update_kernel(const UpdateParam
     }
   }
   if (rank == 0) {  // the rows whose copy got its page are the first ones that copy
-    for (int b = tid; b < p.new_rows; b += kThreads)
-      if ((row[b].copy & 1) && row[b].need < n_free) atomicMax(&s_copies, (row[b].copy >> 1) + 1);
-    __syncthreads();
-    for (int i = s_copies + tid; i < p.new_rows; i += kThreads)
-      p.copies[i] = p.copies[p.new_rows + i] = -1;
+    int copies = 0;
+    for (int b = tid; b - tid < p.new_rows; b += kThreads)
+      copies += __syncthreads_count(b < p.new_rows && (row[b].copy & 1) && row[b].need < n_free);
+    for (int i = copies + tid; i < p.new_rows; i += kThreads) p.copies[i] = p.copies[p.new_rows + i] = -1;
     if (tid == 0) {
       const int got = min(wanted, n_free);
       p.info[0] = n_free - got;
       p.info[1] = wanted - got;
-      p.info[2] = s_copies;
+      p.info[2] = copies;
     }
   }
 }
@@ -269,7 +278,7 @@ struct CompactParams {
 // live page at or above n.
 __global__ void __launch_bounds__(kThreads) page_compact_kernel(const CompactParams p) {
   __shared__ int s_sum[kWarpsPerCta], s_warp[kWarpsPerCta], s_live[kCtas], s_low[kCtas];
-  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const int tid = threadIdx.x, lane = tid & 31;
   const int rank = static_cast<int>(cluster_ctarank());
   const int all_threads = kCtas * kThreads, me = rank * kThreads + tid;
   pdl_launch_dependents();
@@ -427,7 +436,7 @@ extern "C" int npu_b200_page_update(const int32_t* d_page_table, const int32_t* 
               "page_update: the new table, lengths and counts must not overlap the old ones");
   UpdateParams p = {d_page_table, d_seq_lens, d_parents, d_capacity, d_page_refs,
                     d_new_table, d_new_lens, d_new_refs, d_copies, d_info,
-                    rows, new_rows, table_entries, page_size, num_pages};
+                    rows, new_rows, table_entries, page_size, num_pages, Divisor::of(page_size)};
   const size_t smem = static_cast<size_t>(rows) * 4 + static_cast<size_t>(new_rows) * sizeof(Row);
   NPU_TRY_CUDA(cudaFuncSetAttribute(page_update_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                     kMaxRows * static_cast<int>(4 + sizeof(Row))));
