@@ -247,7 +247,8 @@ NPU_B200_API int npu_b200_paged_append(const void* d_k, const void* d_v, void* d
  *   row of its parent if nothing else holds it (count 1); every other child gets
  *   a fresh page and an entry in d_copies, for npu_b200_page_copy.  Pages past the
  *   tokens are fresh.  The old rows' holds end: their pages that no new row
- *   shares, and that nobody outside the table holds, are free at once.
+ *   shares, and that nobody outside the table holds, are free at once, but for
+ *   those that d_copies reads: they are free after this step.
  *   Fresh pages are the lowest free ones (count <= 0), in the order of rows and
  *   entries.  Entries that are no page stay -1 and cost none.
  *

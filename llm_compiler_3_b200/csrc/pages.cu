@@ -21,6 +21,9 @@ constexpr int kWarpsPerCta = kThreads / 32;
 constexpr int kMaxRows = 8192;
 constexpr int kRowPiece = 256;  // table entries of one warp's turn
 constexpr int kAtOnce = 4;      // groups of 32 pages whose counts a warp loads together
+// What a copying row adds to the count of a page that others hold too, so that it is not
+// free in this step, whoever gives it up: 8192 of them and a count stay below 2^31.
+constexpr int kHold = 1 << 17;
 
 // Exclusive prefix of `v` over the CTA's threads and the CTA's total.
 __device__ __forceinline__ long long block_scan(long long v, long long* s_warp, long long* total) {
@@ -109,6 +112,7 @@ struct Row {
 //      are written, the others cleared
 //   3. free pages are counted per warp
 //   4. the k-th free page goes to the k-th need
+// and, if a page that others hold too is copied, a fifth that lets go of it.
 __global__ void __launch_bounds__(kThreads) page_update_kernel(const UpdateParams p) {
   extern __shared__ int32_t smem_i[];
   int32_t* first = smem_i;                             // [rows] lowest new row of each old one
@@ -129,6 +133,7 @@ __global__ void __launch_bounds__(kThreads) page_update_kernel(const UpdateParam
   __syncthreads();
   const int each = (p.new_rows + kThreads - 1) / kThreads;
   const int b0 = min(tid * each, p.new_rows), b1 = min(b0 + each, p.new_rows);
+  int held = 0;  // a page to copy is held elsewhere
   for (int b = b0; b < b1; ++b) {
     Row r;
     r.parent = p.parents[b];
@@ -146,14 +151,14 @@ __global__ void __launch_bounds__(kThreads) page_update_kernel(const UpdateParam
     if (part > 0) {
       r.last = p.table[static_cast<size_t>(r.parent) * p.entries + full];
       if (r.last >= 0 && r.last < p.num_pages)
-        r.copy = p.refs[r.last] != 1;  // held elsewhere too
+        held |= r.copy = p.refs[r.last] != 1;
       else
         r.last = -1;
     }
     r.need = p.by_page.quotient(max(cap, r.len) + p.page_size - 1) - full - (part > 0);
     row[b] = r;
   }
-  __syncthreads();
+  const bool holds = __syncthreads_or(held);  // the same in every CTA
   long long mine = 0;  // needs, and copying rows in the upper half
   for (int b = b0; b < b1; ++b) {
     Row& r = row[b];
@@ -201,7 +206,10 @@ __global__ void __launch_bounds__(kThreads) page_update_kernel(const UpdateParam
       }
       p.new_table[static_cast<size_t>(b) * p.entries + e] = page;
     }
-    if (lane == 0 && e0 == 0) p.new_lens[b] = r.len;
+    if (lane == 0 && e0 == 0) {
+      p.new_lens[b] = r.len;
+      if (holds && (r.copy & 1) && p.refs[r.last] != 1) atomicAdd(&p.new_refs[r.last], kHold);
+    }
   }
   cluster_sync_all();
 
@@ -264,6 +272,16 @@ __global__ void __launch_bounds__(kThreads) page_update_kernel(const UpdateParam
       p.info[1] = wanted - got;
       p.info[2] = copies;
     }
+  }
+  if (!holds) return;
+  cluster_sync_all();
+  for (int b = me; b < p.new_rows; b += all_threads) {
+    const Row r = row[b];
+    if (!(r.copy & 1) || p.refs[r.last] == 1) continue;
+    const int left = atomicSub(&p.new_refs[r.last], kHold) - kHold;
+    if (left > 0) continue;  // held still, or by rows that have yet to let go
+    if (left < 0) p.new_refs[r.last] = 0;
+    atomicAdd(&p.info[0], 1);
   }
 }
 

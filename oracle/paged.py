@@ -124,7 +124,8 @@ def page_update(table, lens, parents, capacity, refs, page_size):
         new.append(row)
         new_lens.append(length)
     left = [max(x, 0) for x in left]
-    free = [p for p in range(n) if left[p] == 0]
+    sources = {s for _, _, s in wants if s is not None}
+    free = [p for p in range(n) if left[p] == 0 and p not in sources]
     copies, short = [], 0
     for b, e, source in wants:
         if not free:
@@ -136,7 +137,8 @@ def page_update(table, lens, parents, capacity, refs, page_size):
             copies.append((source, new[b][e]))
     pad = len(new) - len(copies)
     moves = [[s for s, _ in copies] + [-1] * pad, [d for _, d in copies] + [-1] * pad]
-    return new, new_lens, left, moves, [len(free), short, len(copies)]
+    return new, new_lens, left, moves, [len(free) + sum(left[p] == 0 for p in sources), short,
+                                        len(copies)]
 
 
 def page_compact(table, refs):

@@ -54,6 +54,15 @@ def test_oracle_compact_by_hand():
     assert index == [-1, 1, -1, 0, -1, 2]
 
 
+def test_oracle_pages_to_copy_from_are_not_handed_out():
+    """Rows 0 and 1 share page 0 and rows 2 and 3 page 1, rolled back to 5 of 8 tokens: every
+    child copies, nobody holds pages 0 and 1 any more, and they are free after the step only."""
+    table, lens, refs, copies, info = oracle.page_update(
+        [[0], [0], [1], [1]], [5, 5, 5, 5], [2, 3, 0, 1], [6, 6, 6, 6], [2, 2, 0, 0, 0, 0, 0], 8)
+    assert table == [[2], [3], [4], [5]] and copies == [[1, 1, 0, 0], [2, 3, 4, 5]]
+    assert refs == [0, 0, 1, 1, 1, 1, 0] and info == [3, 0, 4]
+
+
 @pytest.mark.parametrize("change,message", [
     (dict(rows=0), "0 rows"), (dict(rows=8193), "8193 rows"), (dict(new_rows=0), "to 0"),
     (dict(new_rows=8193), "to 8193"), (dict(entries=0), "0 table entries"), (dict(page=12), "page_size 12"),
@@ -127,6 +136,26 @@ def test_update_of_beams(cuda, seed, page):
     parents = [r.choice([-1, r.randrange(rows), r.randrange(rows)]) for _ in range(r.randint(1, 2 * rows))]
     capacity = [r.randint(0, entries * page + 20) if q < 0 else lens[q] + r.choice([0, 1, 1, page]) for q in parents]
     check_update(table, lens, parents, capacity, refs, page)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("seed", range(8))
+def test_update_of_rows_rolled_back(cuda, seed):
+    """Rows cut back into pages that others share, with and without holds outside the table: each
+    child copies, and no page is copied from and to in one step."""
+    r = random.Random(seed)
+    page, groups, width = r.choice([8, 16]), r.randint(2, 5), r.randint(2, 4)
+    table, _, refs, pages = [], [], [], groups * (1 + width) + 6
+    for g in range(groups):
+        table += [[2 * g, 2 * g + 1, -1]] * width
+        refs += [width, width + r.choice([0, 0, 1])]
+    refs += [0] * (pages + width * groups)
+    rows = groups * width
+    lens = [r.choice([page + 1, page + r.randrange(1, page), 3, page]) for _ in range(rows)]
+    parents = [r.randrange(rows) for _ in range(rows)]
+    got = check_update(table, lens, parents, [lens[q] + 1 for q in parents], refs, page)
+    n = got[4][2]
+    assert not set(got[3][0][:n]) & set(got[3][1][:n]) and got[4][1] == 0
 
 
 @pytest.mark.gpu
