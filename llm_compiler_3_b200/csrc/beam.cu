@@ -15,7 +15,8 @@
 // read, the width-th best candidate.  That leaves some width x log2(length / 4096)
 // candidates of a stretch, so the selection costs one comparison per 8 logits (sorted
 // lists that each warp kept for itself cost twice the rest).  A warp whose list runs
-// full, on rising logits, keeps its `width` best and raises the floor.  A second, dependent launch joins the stretches.
+// full, on rising logits, keeps its `width` best and raises the floor.  A second,
+// dependent launch joins the stretches.
 //
 // Which of two candidates is larger decides whole beams, so what follows the
 // stretches (the sum over them, its logarithm, the candidates' worth) is in FP64;
@@ -42,7 +43,7 @@ constexpr int kList = 320;      // candidates of a warp; one word of each lane a
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLog2eLow = static_cast<float>(1.4426950408889634 - static_cast<double>(kLog2e));
 constexpr double kLn2 = 0.69314718055994530942;
-constexpr float kNothing = -FLT_MAX;  // the maximum and the reference before any logit above -inf
+constexpr float kNothing = -FLT_MAX;  // the reference of a stretch without a logit above -inf
 
 struct BeamParams {
   const void* logits;
@@ -322,7 +323,7 @@ __device__ __forceinline__ int candidates(const Candidates* lists) {
 // lane's share of the sum; no logit below `floor` is a candidate, none below `gate`
 // a candidate or a new maximum.
 struct Running {
-  float m = kNothing, ref = 0.f, sum = 0.f;
+  float m = -INFINITY, ref = 0.f, sum = 0.f;
   float floor = -INFINITY, gate = -INFINITY;
 };
 
@@ -473,7 +474,7 @@ __global__ void __launch_bounds__(kSelThreads, 3) beam_stretch_kernel(const Beam
         top = fmaxf(top, t);
       }
       r.m = fmaxf(r.m, warp_max(top));
-      if (r.m > kNothing) r.ref = Kd::reference(r.m);
+      if (r.m > -INFINITY) r.ref = Kd::reference(r.m);
       const float best = best_of_lanes(top, p.width);
       const int all = kSelWarps * p.width;
       if (lane < p.width) s_best[warp * p.width + lane] = order_of(best);
@@ -496,14 +497,14 @@ __global__ void __launch_bounds__(kSelThreads, 3) beam_stretch_kernel(const Beam
       __syncthreads();
     }
     r.floor = fmaxf(r.floor, of_order(*const_cast<volatile uint32_t*>(&s_floor)));
-    r.gate = fminf(r.floor, r.m);
+    r.gate = fminf(r.floor, fmaxf(r.m, -FLT_MAX));
     take_turn<T>(raw, w, p.width, list, &s_floor, r);
   }
   // The lanes' sums, then the warps'.
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) r.sum += __shfl_xor_sync(0xffffffffu, r.sum, o);
   if (lane == 0) {
-    s_ref[warp] = r.m > kNothing ? r.ref : kNothing;
+    s_ref[warp] = r.m > -INFINITY ? r.ref : kNothing;
     s_sum[warp] = r.sum;
   }
   __syncthreads();

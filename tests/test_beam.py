@@ -161,6 +161,24 @@ def test_masked_and_special_logits(cuda, dtype):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.float16, torch.float32])
+def test_rows_masked_with_the_lowest_number(cuda, dtype):
+    """A mask of the type's lowest value leaves its tokens equal candidates: over a whole row, over
+    all but a few tokens, over the rest of a row of -inf, over one stretch of a longer row."""
+    low = torch.finfo(dtype).min
+    logits = seeded((5, 2, 20000), 8, std=2.0).to(dtype)
+    logits[0] = low
+    logits[1, 0] = low
+    logits[1, 1, 300:] = low
+    logits[2] = -INF
+    logits[2, :, 5:9] = low
+    logits[3, :, 3000:9000] = low
+    logits[4, 0, :19999] = low
+    check(logits, -torch.rand(5, 2, generator=torch.Generator().manual_seed(3)), 7)
+    check(logits[:, :, :50].contiguous(), torch.zeros(5, 2), 7)
+
+
+@pytest.mark.gpu
 def test_largest_logits(cuda):
     """Differences up to the type's range, and -1e9 as the scores of a first step's copies."""
     logits = seeded((2, 4, 3001), 9).float() * 1e37
