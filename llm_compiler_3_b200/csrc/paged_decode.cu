@@ -312,7 +312,7 @@ __global__ void __launch_bounds__(PdShape<D, NB>::kThreads, 1)
     }
 
     for (; !bad && k * kWarps + warp < done + here; ++k) {
-      if (!mbar_wait(&my_bars[st], phase, kDevErrTmaTimeout)) {
+      if (!__all_sync(0xffffffffu, mbar_wait(&my_bars[st], phase, kDevErrTmaTimeout))) {
         bad = true;
         break;
       }
