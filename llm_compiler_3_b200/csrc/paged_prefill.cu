@@ -59,6 +59,7 @@ struct PpShape {
 constexpr int kS = 0, kO = 2 * KT;  // TMEM columns; O_t at kO + t D
 
 struct PpParams {
+  const __half *q, *k_pages, *v_pages;  // for single rows: tiles come through the tensor maps
   const int32_t* table;
   const int32_t* seq_lens;
   const int32_t* q_lens;  // or null: every query
@@ -109,11 +110,73 @@ struct Span {
   }
 };
 
+// Row `at` of q and out once more, by one warp and over the keys that it sees alone:
+// [0, s) and [lo, last].  Tiles give a key that a row does not see the weight 0, but
+// 0 x inf is NaN: where a later token's value is infinite or NaN, rows of its tile
+// before it come out as NaN, and only then are they done again.
+template <int D>
+__device__ __noinline__ void row_alone(const PpParams& p, int b, int hk, long long at, int last, int lo) {
+  const int lane = threadIdx.x & 31, s = min(p.sinks, lo);
+  const int keys = last < 0 ? 0 : s + last + 1 - lo;
+  const uint4* q = reinterpret_cast<const uint4*>(p.q + at * D);
+  const float scale = p.negate ? -p.scale_log2 : p.scale_log2;
+  float m = -INFINITY, l = 0.f, o[D / 32] = {};
+  for (int x0 = 0; x0 < keys; x0 += 32) {
+    // Scores of 32 keys, one to a lane.
+    const int x = x0 + lane, j = x < s ? x : lo + x - s;
+    long long row = -1;  // of the pool
+    float score = -INFINITY;
+    if (x < keys) {
+      const int page = p.table[static_cast<size_t>(b) * p.entries + j / p.page_size];
+      if (page >= 0 && page < p.num_pages) row = (page * p.kv_heads + hk) * p.page_size + j % p.page_size;
+      score = 0.f;
+      if (row >= 0) {
+        const uint4* k = reinterpret_cast<const uint4*>(p.k_pages + row * D);
+        for (int c = 0; c < D / 8; ++c) {
+          const uint4 qw = q[c], kw = k[c];
+          const uint32_t qu[4] = {qw.x, qw.y, qw.z, qw.w}, ku[4] = {kw.x, kw.y, kw.z, kw.w};
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const float2 a = __half22float2(*reinterpret_cast<const __half2*>(&qu[e]));
+            const float2 d = __half22float2(*reinterpret_cast<const __half2*>(&ku[e]));
+            score += a.x * d.x + a.y * d.y;
+          }
+        }
+      }
+      score *= scale;
+    }
+    float top = fmaxf(score, m);
+#pragma unroll
+    for (int w = 16; w > 0; w >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, w));
+    const float alpha = m == -INFINITY ? 0.f : fast_exp2(m - top);
+    m = top;
+    const float weight = fast_exp2(score - (m == -INFINITY ? 0.f : m));
+    l = l * alpha + weight;
+#pragma unroll
+    for (int e = 0; e < D / 32; ++e) o[e] *= alpha;
+    // Each lane sums D / 32 of the values' dimensions.
+    for (int k = 0; k < min(32, keys - x0); ++k) {
+      const float w = __shfl_sync(0xffffffffu, weight, k);
+      const long long from = __shfl_sync(0xffffffffu, row, k);
+      if (from < 0) continue;
+      const __half* v = p.v_pages + from * D + lane * (D / 32);
+#pragma unroll
+      for (int e = 0; e < D / 32; ++e) o[e] += w * __half2float(v[e]);
+    }
+  }
+#pragma unroll
+  for (int w = 16; w > 0; w >>= 1) l += __shfl_xor_sync(0xffffffffu, l, w);
+  const float inv = l == 0.f ? 0.f : 1.f / l;
+#pragma unroll
+  for (int e = 0; e < D / 32; ++e) p.out[at * D + lane * (D / 32) + e] = __float2half_rn(o[e] * inv);
+}
+
 template <int D>
 __global__ void __launch_bounds__(kThreads, 1)
     paged_prefill_kernel(const __grid_constant__ CUtensorMap qmap,
                          const __grid_constant__ CUtensorMap kmap,
-                         const __grid_constant__ CUtensorMap vmap, const PpParams p) {
+                         const __grid_constant__ CUtensorMap vmap,
+                         const __grid_constant__ PpParams p) {
   using S = PpShape<D>;
   constexpr int kStages = S::kStages;
   extern __shared__ uint8_t smem_raw[];
@@ -142,7 +205,6 @@ __global__ void __launch_bounds__(kThreads, 1)
   const bool has1 = u0 + 1 < n_units;
   auto unit_m0 = [&](int u) { return (p.q_blocks - 1 - u / subgroups) * p.bm; };
 
-  pdl_launch_dependents();
   pdl_wait();
   Span span;
   span.seq_len = min(max(p.seq_lens[b], 0), p.entries * p.page_size);
@@ -183,10 +245,13 @@ __global__ void __launch_bounds__(kThreads, 1)
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
+  // Not before: a dependent kernel's CTA that took this SM's TMEM first would wait for
+  // this one to end, and this one for the TMEM.
+  pdl_launch_dependents();
   const uint32_t tmem = __shfl_sync(0xffffffffu, *tmem_slot, 0);
 
   // Phase of raw[x % stages] for the V tile at place x: how many border tiles used
-    // the stage before.
+  // the stage before.
   auto raw_phase = [&](int x) {
     uint32_t n = 0;
     for (int y = x - kStages; y > 0; y -= kStages)
@@ -449,8 +514,9 @@ __global__ void __launch_bounds__(kThreads, 1)
       tc_fence_after();
       const bool any = n_tiles > 0 && l_run != 0.f;
       const float inv = any ? 1.f / l_run : 0.f;
-      uint4* row = reinterpret_cast<uint4*>(
-          p.out + ((static_cast<size_t>(b) * p.q_heads + hk * group + gs * p.hp + g) * p.queries + m0 + i) * D);
+      const long long at = (static_cast<long long>(b) * p.q_heads + hk * group + gs * p.hp + g) * p.queries + m0 + i;
+      uint4* row = reinterpret_cast<uint4*>(p.out + at * D);
+      bool odd = false;  // not a number
 #pragma unroll 1
       for (int c = 0; c < D; c += 16) {
         uint32_t o[16];
@@ -461,12 +527,21 @@ __global__ void __launch_bounds__(kThreads, 1)
         if (row_ok) {
           float f[16];
 #pragma unroll
-          for (int e = 0; e < 16; ++e) f[e] = any ? __uint_as_float(o[e]) * inv : 0.f;
+          for (int e = 0; e < 16; ++e) {
+            f[e] = any ? __uint_as_float(o[e]) * inv : 0.f;
+            odd |= f[e] != f[e];
+          }
           row[c / 8] = make_uint4(pack_half2(f[0], f[1]), pack_half2(f[2], f[3]), pack_half2(f[4], f[5]),
                                   pack_half2(f[6], f[7]));
           row[c / 8 + 1] = make_uint4(pack_half2(f[8], f[9]), pack_half2(f[10], f[11]),
                                       pack_half2(f[12], f[13]), pack_half2(f[14], f[15]));
         }
+      }
+      __syncwarp();
+      for (unsigned todo = __ballot_sync(0xffffffffu, odd); todo != 0; todo &= todo - 1) {
+        const int from = __ffs(todo) - 1;
+        row_alone<D>(p, b, hk, __shfl_sync(0xffffffffu, at, from), __shfl_sync(0xffffffffu, last, from),
+                     __shfl_sync(0xffffffffu, lo, from));
       }
     }
   }
@@ -523,6 +598,9 @@ extern "C" int npu_b200_paged_prefill(const void* d_q, const void* d_k_pages, co
   NPU_REQUIRE(aligned16(d_q) && aligned16(d_k_pages) && aligned16(d_v_pages) && aligned16(d_out),
               "paged_prefill: q, pages and out must be 16-byte aligned");
   PpParams p;
+  p.q = static_cast<const __half*>(d_q);
+  p.k_pages = static_cast<const __half*>(d_k_pages);
+  p.v_pages = static_cast<const __half*>(d_v_pages);
   p.table = d_page_table;
   p.seq_lens = d_seq_lens;
   p.q_lens = d_q_lens;

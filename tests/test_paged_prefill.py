@@ -202,3 +202,22 @@ def test_checks_of_the_wrapper(cuda):
                    dict(out=torch.empty_like(q)[:1]), dict(q_lens=n.cpu())):
         with pytest.raises(ValueError):
             ops.paged_prefill(**dict(good, **change))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("heads,dim,window,sinks", [(2, 64, 0, 0), (4, 128, 0, 0), (4, 64, 20, 3), (2, 128, 9, 0)])
+def test_values_that_are_no_numbers_stay_with_the_queries_that_see_them(cuda, heads, dim, window, sinks):
+    """Infinite and NaN values of some tokens reach exactly the queries and dimensions that see
+    them: not the queries before, though they share a tile, nor those whose window has passed."""
+    lens, q_lens = [150, 300], [150, 140]
+    k, v, table = paged_cache(lens, 2, dim, 16, seed=dim + window)
+    for b, j, d, x in ((0, 40, 3, NAN), (0, 120, 7, INF), (1, 170, 1, -INF), (1, 290, 0, NAN)):
+        v[int(table[b, j // 16]), :, j % 16, d] = x
+    q = seeded((2, heads, 150, dim), 6)
+    got = _prefill(q, k, v, table, lens, q_lens, window=window, sinks=sinks)
+    want = oracle.attention_paged(q, k, v, table, lens, q_lens, window=window, sinks=sinks)[0]
+    odd = ~want.isfinite()
+    assert odd.any() and torch.equal(got.double().nan_to_num(1e9, 2e9, 3e9)[odd], want.nan_to_num(1e9, 2e9, 3e9)[odd])
+    # The other elements do not depend on them: as with zeros in their places.
+    want, bound = oracle.attention_paged(q, k, v.nan_to_num(0, 0, 0), table, lens, q_lens, window=window, sinks=sinks)
+    check(torch.where(odd, want.half(), got), want, torch.where(odd, want.abs(), bound))
