@@ -11,7 +11,7 @@
 // allocator at each call, so calls on several streams and captured graphs share
 // none.
 #include <ATen/cuda/CUDAContext.h>
-#include <ATen/ops/empty.h>
+#include <ATen/cuda/EmptyTensor.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <torch/csrc/utils/pybind.h>
 
@@ -70,8 +70,10 @@ void status(int rc) {
   throw py::error_already_set();
 }
 
+// A new tensor on t's device, past torch's dispatcher (a call with five of them 9.1 ->
+// 7.8 us).
 Tensor like(const Tensor& t, at::IntArrayRef size, at::ScalarType type) {
-  return at::empty(size, t.options().dtype(type));
+  return at::detail::empty_cuda(size, type, t.device(), std::nullopt);
 }
 
 Tensor output(const Tensor& t, const Maybe& out, int index) {
