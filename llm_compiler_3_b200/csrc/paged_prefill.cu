@@ -22,6 +22,8 @@
 //                   ...), one box per piece of a page, each lane one
 //   warp 9          MMA issue: O_t += P_t V, then the next S_t = Q_t K^T
 //   warp 10         clears the hidden rows of V tiles on a border
+// When there are few query tiles, a cluster of up to 8 CTAs shares the keys of each pair;
+// their O, maxima and sums meet in shared memory, each CTA joining a share of the dimensions.
 // TMEM: S0, S1 (128 columns each), O0, O1 (D each); P_t, FP16, lies over the first
 // half of S_t.  The tensor pipe works in order, so S_t(j + 1), issued after
 // P_t(j) V, cannot overwrite weights that are still read, and its completion says
@@ -43,6 +45,7 @@ constexpr int KT = 128;           // keys per tile
 constexpr int kThreads = 352;
 constexpr uint32_t kTmemCols = 512;
 constexpr float kRescaleLog2 = 8.f;
+constexpr int kMaxSplits = 8;     // CTAs that share a tile pair's keys
 
 template <int D>
 struct PpShape {
@@ -65,7 +68,7 @@ struct PpParams {
   const int32_t* q_lens;  // or null: every query
   __half* out;
   int q_heads, kv_heads, queries, entries, page_size, box, num_pages, total_rows;
-  int bm, hp, q_blocks, window, sinks, negate;
+  int bm, hp, q_blocks, window, sinks, negate, splits;
   float scale_log2;  // > 0
 };
 
@@ -110,12 +113,13 @@ struct Span {
   }
 };
 
-// Row `at` of q and out once more, by one warp and over the keys that it sees alone:
-// [0, s) and [lo, last].  Tiles give a key that a row does not see the weight 0, but
+// Dimensions [d0, d1) of row `at` of out once more, by one warp and over the keys that it
+// sees alone: [0, s) and [lo, last].  Tiles give a key that a row does not see the weight 0, but
 // 0 x inf is NaN: where a later token's value is infinite or NaN, rows of its tile
 // before it come out as NaN, and only then are they done again.
 template <int D>
-__device__ __noinline__ void row_alone(const PpParams& p, int b, int hk, long long at, int last, int lo) {
+__device__ __noinline__ void row_alone(const PpParams& p, int b, int hk, long long at, int last, int lo,
+                                       int d0, int d1) {
   const int lane = threadIdx.x & 31, s = min(p.sinks, lo);
   const int keys = last < 0 ? 0 : s + last + 1 - lo;
   const uint4* q = reinterpret_cast<const uint4*>(p.q + at * D);
@@ -168,7 +172,10 @@ __device__ __noinline__ void row_alone(const PpParams& p, int b, int hk, long lo
   for (int w = 16; w > 0; w >>= 1) l += __shfl_xor_sync(0xffffffffu, l, w);
   const float inv = l == 0.f ? 0.f : 1.f / l;
 #pragma unroll
-  for (int e = 0; e < D / 32; ++e) p.out[at * D + lane * (D / 32) + e] = __float2half_rn(o[e] * inv);
+  for (int e = 0; e < D / 32; ++e) {
+    const int d = lane * (D / 32) + e;
+    if (d >= d0 && d < d1) p.out[at * D + d] = __float2half_rn(o[e] * inv);
+  }
 }
 
 template <int D>
@@ -193,12 +200,17 @@ __global__ void __launch_bounds__(kThreads, 1)
   uint64_t* drain = o_done + 2;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(drain + 1);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+  // Over the ring at the end: O of a CTA that has a share of the keys, [tile][D / 4][row], and
+  // its rows' maxima and sums.
+  uint4* parts = reinterpret_cast<uint4*>(smem + S::kRing);
+  float2* part_ml = reinterpret_cast<float2*>(parts + 2 * (D / 4) * 128);
+  static_assert(2 * D * 512 + 2048 <= kStages * S::kTileBytes, "parts over the ring");
 
   const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
   const int group = p.q_heads / p.kv_heads, subgroups = group / p.hp;
   const int n_units = p.q_blocks * subgroups;
-  const int hk = static_cast<int>(blockIdx.x) % p.kv_heads;
-  const int b = static_cast<int>(blockIdx.x) / p.kv_heads;
+  const int rank = static_cast<int>(blockIdx.x) % p.splits;  // in the cluster
+  const int bh = static_cast<int>(blockIdx.x) / p.splits, hk = bh % p.kv_heads, b = bh / p.kv_heads;
   // Units (query block, head subgroup), last query blocks first; this CTA has
   // units u0 (tile 0) and u0 + 1 (tile 1, if there is one).
   const int u0 = 2 * static_cast<int>(blockIdx.y);
@@ -220,7 +232,10 @@ __global__ void __launch_bounds__(kThreads, 1)
     span.tiles.set(span.lo, span.len, p.sinks);
     if (span.len == 0) span.tiles.n = 0;
   }
-  const int n_tiles = span.tiles.n;
+  // This CTA's tiles of keys: all, or its even share of them.
+  const int tile0 = static_cast<int>(static_cast<long long>(span.tiles.n) * rank / p.splits);
+  const int n_tiles = static_cast<int>(static_cast<long long>(span.tiles.n) * (rank + 1) / p.splits) - tile0;
+  auto key_of = [&](int j) { return span.tiles.key0(tile0 + j); };
 
   if (threadIdx.x == 0) {
     mbar_init(q_full, 1);
@@ -255,8 +270,28 @@ __global__ void __launch_bounds__(kThreads, 1)
   auto raw_phase = [&](int x) {
     uint32_t n = 0;
     for (int y = x - kStages; y > 0; y -= kStages)
-      if ((y & 1) && !span.sees_all(span.tiles.key0(y / 2), KT)) ++n;
+      if ((y & 1) && !span.sees_all(key_of(y / 2), KT)) ++n;
     return n & 1;
+  };
+
+  // A softmax thread's row.
+  const int tt = (warp >> 2) & 1, r = threadIdx.x & 127;
+  const bool unit_ok = tt == 0 || has1;
+  const int m0 = unit_ok ? unit_m0(u0 + tt) : 0, g = r / p.bm, i = r % p.bm;
+  const bool row_ok = unit_ok && g < p.hp && m0 + i < p.queries;
+  const long long at =  // of q and out
+      (static_cast<long long>(b) * p.q_heads + hk * group + (u0 + tt) % subgroups * p.hp + g) * p.queries + m0 + i;
+  // Keys of this row: j <= last and (j >= lo or j < sinks).
+  const int last = row_ok && m0 + i < span.q_len ? span.first_pos + m0 + i : -1;
+  const int lo = p.window > 0 ? max(0, last - p.window + 1) : 0;
+  // Rows that came out as NaN, by the whole warp; dimensions [d0, d1).
+  auto redo = [&](bool odd, int d0, int d1) {
+    __syncwarp();
+    for (unsigned todo = __ballot_sync(0xffffffffu, odd); todo != 0; todo &= todo - 1) {
+      const int from = __ffs(todo) - 1;
+      row_alone<D>(p, b, hk, __shfl_sync(0xffffffffu, at, from), __shfl_sync(0xffffffffu, last, from),
+                   __shfl_sync(0xffffffffu, lo, from), d0, d1);
+    }
   };
 
   if (warp == 8) {
@@ -283,7 +318,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       const int my_region = lane % S::kRegions, my_row = lane / S::kRegions * p.box;
       const bool mine = lane < combos;
       auto look_up = [&](int j) {  // the page of this lane's box of tile j; -2: nothing visible
-        const int at = span.tiles.key0(j) + my_row;
+        const int at = key_of(j) + my_row;
         if (!mine || !span.sees_any(at, p.box)) return -2;
         return p.table[static_cast<size_t>(b) * p.entries + at / p.page_size];
       };
@@ -291,7 +326,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       bool ok = true;
       int issued = 0;
       for (int j = 0; ok && j < n_tiles; ++j) {
-        const int at = span.tiles.key0(j) + my_row;
+        const int at = key_of(j) + my_row;
         int row = p.total_rows;  // past the pool: the box is filled with zeros
         if (page >= 0 && page < p.num_pages)
           row = (page * p.kv_heads + hk) * p.page_size + at % p.page_size;
@@ -303,7 +338,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           if (x >= kStages)
             ok = __all_sync(0xffffffffu, wait_or_abort(&empty[s], ((x / kStages) - 1) & 1, abort_flag));
           if (!ok) break;
-          uint64_t* bar = kv && !span.sees_all(span.tiles.key0(j), KT) ? &raw[s] : &full[s];
+          uint64_t* bar = kv && !span.sees_all(key_of(j), KT) ? &raw[s] : &full[s];
           if (lane == 0) mbar_arrive_expect_tx(bar, S::kTileBytes);
           __syncwarp();
           if (mine)
@@ -317,7 +352,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       mbar_wait(q_full, 0, kDevErrTmaTimeout);
       for (int x = max(0, issued - kStages); x < issued; ++x) {
         const int s = x % kStages;
-        const bool border = (x & 1) && !span.sees_all(span.tiles.key0(x / 2), KT);
+        const bool border = (x & 1) && !span.sees_all(key_of(x / 2), KT);
         mbar_wait(border ? &raw[s] : &full[s], border ? raw_phase(x) : (x / kStages) & 1, kDevErrTmaTimeout);
       }
     }
@@ -400,7 +435,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     // Rows that no query here sees may hold anything; their weights are 0, but
     // 0 * NaN is NaN.
     for (int j = 0; j < n_tiles; ++j) {
-      const int key0 = span.tiles.key0(j), x = 2 * j + 1, s = x % kStages;
+      const int key0 = key_of(j), x = 2 * j + 1, s = x % kStages;
       if (span.sees_all(key0, KT)) continue;
       if (!__all_sync(0xffffffffu, wait_or_abort(&raw[s], raw_phase(x), abort_flag))) break;
       for (int r = lane; r < KT; r += 32)
@@ -415,15 +450,6 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
   } else {
     // ---------------- softmax warpgroups ----------------
-    const int tt = warp >> 2, r = threadIdx.x & 127;
-    const bool unit_ok = tt == 0 || has1;
-    const int u = u0 + tt;
-    const int m0 = unit_ok ? unit_m0(u) : 0, gs = u % subgroups;
-    const int g = r / p.bm, i = r % p.bm;
-    const bool row_ok = unit_ok && g < p.hp && m0 + i < p.queries;
-    // Keys of this row: j <= last and (j >= lo or j < sinks).
-    const int last = row_ok && m0 + i < span.q_len ? span.first_pos + m0 + i : -1;
-    const int lo = p.window > 0 ? max(0, last - p.window + 1) : 0;
     const uint32_t t_lane = tmem + (static_cast<uint32_t>((warp & 3) * 32) << 16);
     const uint32_t t_s = t_lane + kS + tt * KT, t_o = t_lane + kO + tt * D;
     auto wait = [&](uint64_t* bar, uint32_t phase) {
@@ -439,7 +465,7 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll
       for (int c = 0; c < KT; c += 32) tmem_ld32(t_s + c, sr + c);
       tmem_ld_wait();
-      const int key0 = span.tiles.key0(j);
+      const int key0 = key_of(j);
       // Hidden keys, 32 to a word of bits (comparing key by key took 640 instructions).
       if (!__all_sync(0xffffffffu, key0 + KT - 1 <= last && (key0 >= lo || key0 + KT <= p.sinks))) {
 #pragma unroll
@@ -508,13 +534,28 @@ __global__ void __launch_bounds__(kThreads, 1)
       l_run += lo2(all2) + hi2(all2);
     }
     if (ok && n_tiles > 0) ok = wait(&o_done[tt], 0);
+    // Parts go over the ring, which the other tile's last product reads too.
+    if (ok && n_tiles > 0 && p.splits > 1) ok = wait(&o_done[tt ^ 1], 0);
     if (!ok) {
       if (lane == 0) *abort_flag = 1;
+    } else if (p.splits > 1) {
+      tc_fence_after();
+      if (n_tiles > 0) {
+#pragma unroll 1
+        for (int c = 0; c < D; c += 16) {
+          uint32_t o[16];
+          tmem_ld16(t_o + c, o);
+          tmem_ld_wait();
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            parts[(tt * (D / 4) + c / 4 + e) * 128 + r] = make_uint4(o[4 * e], o[4 * e + 1], o[4 * e + 2], o[4 * e + 3]);
+        }
+      }
+      part_ml[tt * 128 + r] = make_float2(m_run, l_run);
     } else {
       tc_fence_after();
       const bool any = n_tiles > 0 && l_run != 0.f;
       const float inv = any ? 1.f / l_run : 0.f;
-      const long long at = (static_cast<long long>(b) * p.q_heads + hk * group + gs * p.hp + g) * p.queries + m0 + i;
       uint4* row = reinterpret_cast<uint4*>(p.out + at * D);
       bool odd = false;  // not a number
 #pragma unroll 1
@@ -537,15 +578,57 @@ __global__ void __launch_bounds__(kThreads, 1)
                                       pack_half2(f[12], f[13]), pack_half2(f[14], f[15]));
         }
       }
-      __syncwarp();
-      for (unsigned todo = __ballot_sync(0xffffffffu, odd); todo != 0; todo &= todo - 1) {
-        const int from = __ffs(todo) - 1;
-        row_alone<D>(p, b, hk, __shfl_sync(0xffffffffu, at, from), __shfl_sync(0xffffffffu, last, from),
-                     __shfl_sync(0xffffffffu, lo, from));
-      }
+      redo(odd, 0, D);
     }
   }
 
+  if (p.splits > 1) {
+    // ---------------- the cluster's parts of every row join ----------------
+    // CTA `rank` takes its share of the dimensions; parts in the order of the CTAs.
+    cluster_sync_all();
+    if (warp < 8) {
+      float w[kMaxSplits], l[kMaxSplits], top = -INFINITY, sum = 0.f;
+#pragma unroll
+      for (int c = 0; c < kMaxSplits; ++c) {
+        w[c] = -INFINITY;
+        if (c >= p.splits) continue;
+        const uint32_t ml = cluster_map(smem_u32(part_ml + tt * 128 + r), c);
+        w[c] = ld_cluster_f32(ml);
+        l[c] = ld_cluster_f32(ml + 4);
+        top = fmaxf(top, w[c]);
+      }
+#pragma unroll
+      for (int c = 0; c < kMaxSplits; ++c) {
+        w[c] = w[c] == -INFINITY ? 0.f : fast_exp2(w[c] - top);
+        if (w[c] != 0.f) sum += w[c] * l[c];
+      }
+      const float inv = sum != 0.f ? 1.f / sum : 0.f;
+      const int each = D / 4 / p.splits;  // groups of four dimensions
+      bool odd = false;
+#pragma unroll 1
+      for (int q = rank * each; q < (rank + 1) * each; q += 2) {
+        float f[8] = {};
+#pragma unroll
+        for (int c = 0; c < kMaxSplits; ++c) {
+          if (c >= p.splits || w[c] == 0.f) continue;
+          const uint32_t from = cluster_map(smem_u32(parts + (tt * (D / 4) + q) * 128 + r), c);
+          const float4 x = ld_cluster_v4(from), y = ld_cluster_v4(from + 128 * 16);
+          f[0] += w[c] * x.x, f[1] += w[c] * x.y, f[2] += w[c] * x.z, f[3] += w[c] * x.w;
+          f[4] += w[c] * y.x, f[5] += w[c] * y.y, f[6] += w[c] * y.z, f[7] += w[c] * y.w;
+        }
+        if (!row_ok) continue;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          f[e] *= inv;
+          odd |= f[e] != f[e];
+        }
+        *reinterpret_cast<uint4*>(p.out + at * D + q * 4) = make_uint4(
+            pack_half2(f[0], f[1]), pack_half2(f[2], f[3]), pack_half2(f[4], f[5]), pack_half2(f[6], f[7]));
+      }
+      redo(odd, rank * each * 4, (rank + 1) * each * 4);
+    }
+    cluster_sync_all();  // nobody reads this CTA's parts any more
+  }
   tc_fence_before();
   __syncthreads();
   if (warp == 9) {
@@ -555,14 +638,26 @@ __global__ void __launch_bounds__(kThreads, 1)
 }
 
 template <int D>
-int launch_pp(const CUtensorMap& qm, const CUtensorMap& km, const CUtensorMap& vm, const PpParams& p,
+int launch_pp(const CUtensorMap& qm, const CUtensorMap& km, const CUtensorMap& vm, PpParams& p,
               int batch, cudaStream_t stream) {
   using S = PpShape<D>;
   auto kern = paged_prefill_kernel<D>;
   NPU_TRY_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, S::kSmem));
   const int n_units = p.q_blocks * (p.q_heads / p.kv_heads / p.hp);
+  // Few query tiles leave SMs idle: then a cluster of CTAs shares each pair's keys, as many
+  // as there are SMs for, and not more than the longest table has tiles.  A chunk of 40
+  // tokens, 32 heads on 8: behind 16384 keys 289 -> 48 us, 4 of them behind 540 21.1 -> 18.2;
+  // where the table has room for several tiles and the sequence is one, the cluster costs
+  // 2 us (11.8 -> 14.0).
+  const long long pairs = static_cast<long long>(batch) * p.kv_heads * ((n_units + 1) / 2);
+  const long long keys = static_cast<long long>(p.entries) * p.page_size;
+  long long most = (keys + KT - 1) / KT;
+  if (p.window > 0) most = std::min(most, (static_cast<long long>(p.window) + 2 * p.bm) / KT + p.sinks / KT + 2);
+  p.splits = 1;
+  while (p.splits < kMaxSplits && pairs * p.splits * 2 <= sm_count() && p.splits * 2 <= most) p.splits *= 2;
   LaunchCfg cfg;
-  cfg.grid = dim3(batch * p.kv_heads, (n_units + 1) / 2);
+  cfg.cluster = p.splits;
+  cfg.grid = dim3(batch * p.kv_heads * p.splits, (n_units + 1) / 2);
   cfg.block = dim3(kThreads);
   cfg.smem = S::kSmem;
   cfg.stream = stream;

@@ -221,3 +221,18 @@ def test_values_that_are_no_numbers_stay_with_the_queries_that_see_them(cuda, he
     # The other elements do not depend on them: as with zeros in their places.
     want, bound = oracle.attention_paged(q, k, v.nan_to_num(0, 0, 0), table, lens, q_lens, window=window, sinks=sinks)
     check(torch.where(odd, want.half(), got), want, torch.where(odd, want.abs(), bound))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("heads,kv_heads,dim,queries", [(4, 1, 64, 7), (4, 1, 128, 7), (2, 2, 128, 130), (8, 4, 64, 40),
+                                                        (16, 16, 128, 3), (8, 8, 128, 300)])
+@pytest.mark.parametrize("window,sinks", [(0, 0), (300, 9)])
+def test_keys_shared_by_a_cluster(cuda, heads, kv_heads, dim, queries, window, sinks):
+    """Few query tiles behind long prefixes: CTAs that share the keys of a tile, some of them
+    without any; all of a row's keys in one CTA's share; empty sequences; the same bits twice."""
+    lens, q_lens = [1400, queries, 129, 0], [queries, queries, 1, 0]
+    k, v, table = paged_cache(lens, kv_heads, dim, 16, seed=dim + queries)
+    q = seeded((4, heads, queries, dim), 8)
+    got = check_prefill(q, k, v, table, lens, q_lens, window=window, sinks=sinks)
+    assert torch.equal(got, _prefill(q, k, v, table, lens, q_lens, window=window, sinks=sinks))
+    check_prefill(q[:1], k, v, table[:1], lens[:1], q_lens[:1], window=window, sinks=sinks)
