@@ -72,20 +72,6 @@ __device__ __forceinline__ float of_order(uint32_t k) {
   return __uint_as_float(k & 0x80000000u ? k ^ 0x80000000u : ~k);
 }
 
-// The `width` largest of the lanes' values in falling order (equal ones each):
-// lane k < width returns the k-th.
-__device__ __forceinline__ float best_of_lanes(float v, int width) {
-  const int lane = threadIdx.x & 31;
-  uint32_t k = order_of(v), mine = order_of(-INFINITY);
-  for (int i = 0; i < width; ++i) {
-    const uint32_t top = __reduce_max_sync(0xffffffffu, k);
-    const unsigned who = __ballot_sync(0xffffffffu, k == top);
-    if (lane == __ffs(who) - 1) k = 0;
-    if (lane == i) mine = top;
-  }
-  return of_order(mine);
-}
-
 // One warp's candidates.
 struct Candidates {
   float val[kList];
@@ -93,10 +79,9 @@ struct Candidates {
   int n;
 };
 
-// The `width` best of the lists' candidates, larger first, lower token among equals:
+// The `width` best of a list's candidates, larger first, lower token among equals:
 // lane k returns the k-th.  Each turn takes the best that comes after the last one.
-__device__ __forceinline__ void take_best(const Candidates* lists, int count, int width, float* out_v,
-                                          int* out_i) {
+__device__ __forceinline__ void take_best(const Candidates& list, int width, float* out_v, int* out_i) {
   const int lane = threadIdx.x & 31;
   uint32_t last = 0xffffffffu;
   int last_i = -1;
@@ -105,16 +90,15 @@ __device__ __forceinline__ void take_best(const Candidates* lists, int count, in
   for (int k = 0; k < width; ++k) {
     uint32_t best = 0;
     int best_i = INT_MAX;
-    for (int l = 0; l < count; ++l)
-      for (int e = lane; e < lists[l].n; e += 32) {
-        const uint32_t v = order_of(lists[l].val[e]);
-        const int i = lists[l].idx[e];
-        const bool after = v < last || (v == last && i > last_i);
-        if (after && (v > best || (v == best && i < best_i))) {
-          best = v;
-          best_i = i;
-        }
+    for (int e = lane; e < list.n; e += 32) {
+      const uint32_t v = order_of(list.val[e]);
+      const int i = list.idx[e];
+      const bool after = v < last || (v == last && i > last_i);
+      if (after && (v > best || (v == best && i < best_i))) {
+        best = v;
+        best_i = i;
       }
+    }
     last = __reduce_max_sync(0xffffffffu, best);
     if (last == 0) break;  // no more
     last_i = __reduce_min_sync(0xffffffffu, best == last ? best_i : INT_MAX);
@@ -293,24 +277,57 @@ __device__ __forceinline__ float warp_max(float v) {
   return of_order(__reduce_max_sync(0xffffffffu, order_of(v)));
 }
 
-// This thread's candidate among all of the CTA's lists (false: it has none), and how
-// many come before it.
-__device__ __forceinline__ bool rank_of_mine(const Candidates* lists, float* val, int* idx, int* before) {
-  int own = 0, e = threadIdx.x;  // number e of list `own`
-  while (own < kSelWarps && e >= lists[own].n) e -= lists[own++].n;
-  if (own == kSelWarps) return false;
-  *val = lists[own].val[e];
-  *idx = lists[own].idx[e];
-  const uint32_t v = order_of(*val);
+// The `width` best of up to 256 candidates in one warp's registers (order_of() keys, 0:
+// none), larger first, lower token among equals: take(k, key, token) in every lane.
+// (Ranking each candidate among all, by a thread of its own, is quadratic in their
+// number: 64 x 8 rows of 128256 took 72 us instead of 57.)
+constexpr int kPerLane = kSelThreads / 32;
+template <typename Take>
+__device__ __forceinline__ void best_of(uint32_t (&key)[kPerLane], const int (&token)[kPerLane], int width,
+                                        Take take) {
+  for (int k = 0; k < width; ++k) {
+    uint32_t most = 0;
+#pragma unroll
+    for (int u = 0; u < kPerLane; ++u) most = max(most, key[u]);
+    most = __reduce_max_sync(0xffffffffu, most);
+    if (most == 0) break;
+    int low = INT_MAX;
+#pragma unroll
+    for (int u = 0; u < kPerLane; ++u)
+      if (key[u] == most) low = min(low, token[u]);
+    low = __reduce_min_sync(0xffffffffu, low);
+    take(k, most, low);
+#pragma unroll
+    for (int u = 0; u < kPerLane; ++u)
+      if (key[u] == most && token[u] == low) key[u] = 0;
+  }
+}
+
+// All lists' candidates, at most 256, to one warp's registers.
+__device__ __forceinline__ void gather(const Candidates* lists, uint32_t (&key)[kPerLane], int (&token)[kPerLane]) {
+  int from[kSelWarps];  // of the lists, one behind the other
   int n = 0;
-  for (int w = 0; w < kSelWarps; ++w)
-#pragma unroll 4
-    for (int k = 0; k < lists[w].n; ++k) {
-      const uint32_t o = order_of(lists[w].val[k]);
-      n += o > v || (o == v && lists[w].idx[k] < *idx);
-    }
-  *before = n;
-  return true;
+#pragma unroll
+  for (int w = 0; w < kSelWarps; ++w) {
+    from[w] = n;
+    n += lists[w].n;
+  }
+#pragma unroll
+  for (int u = 0; u < kPerLane; ++u) {
+    const int e = (threadIdx.x & 31) + 32 * u;
+    key[u] = 0;
+    token[u] = INT_MAX;
+    if (e >= n) continue;
+    int w = 0, first = 0;
+#pragma unroll
+    for (int v = 1; v < kSelWarps; ++v)
+      if (e >= from[v]) {
+        w = v;
+        first = from[v];
+      }
+    key[u] = order_of(lists[w].val[e - first]);
+    token[u] = lists[w].idx[e - first];
+  }
 }
 __device__ __forceinline__ int candidates(const Candidates* lists) {
   int n = 0;
@@ -365,7 +382,7 @@ __device__ __forceinline__ void take_turn(uint4 (&raw)[N], int w, int width, Can
         __syncwarp();
         float val;
         int idx;
-        take_best(&list, 1, width, &val, &idx);
+        take_best(list, width, &val, &idx);
         __syncwarp();
         if (lane < width) {
           list.val[lane] = val;
@@ -412,7 +429,7 @@ __global__ void __launch_bounds__(kSelThreads, 3) beam_stretch_kernel(const Beam
   constexpr int L = Kd::kLogits;
   __shared__ float s_ref[kSelWarps], s_sum[kSelWarps];
   __shared__ Candidates s_list[kSelWarps];
-  __shared__ uint32_t s_best[kSelWarps * kMaxWidth];  // the lanes' best first logits, by warp
+  __shared__ uint32_t s_top[kSelThreads];  // the lanes' best first logits
   __shared__ uint32_t s_floor;  // order_of() of what `width` logits of the CTA reach
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const long long row = blockIdx.y;
@@ -475,25 +492,29 @@ __global__ void __launch_bounds__(kSelThreads, 3) beam_stretch_kernel(const Beam
       }
       r.m = fmaxf(r.m, warp_max(top));
       if (r.m > -INFINITY) r.ref = Kd::reference(r.m);
-      const float best = best_of_lanes(top, p.width);
-      const int all = kSelWarps * p.width;
-      if (lane < p.width) s_best[warp * p.width + lane] = order_of(best);
+      s_top[threadIdx.x] = order_of(top);
       __syncthreads();
-      for (int i = threadIdx.x; i < all; i += kSelThreads) {  // the width-th of all is the floor
-        const uint32_t v = s_best[i];
-        int before = 0;
-        for (int k = 0; k < all; ++k) before += s_best[k] > v || (s_best[k] == v && k < i);
-        if (before == p.width - 1) s_floor = v;
+      if (warp == 0) {  // the width-th of all is the floor
+        uint32_t key[kPerLane];
+        int at[kPerLane];
+#pragma unroll
+        for (int u = 0; u < kPerLane; ++u) key[u] = s_top[at[u] = lane + 32 * u];
+        best_of(key, at, p.width, [&](int k, uint32_t v, int) {
+          if (k == p.width - 1) s_floor = v;
+        });
       }
       __syncthreads();
     }
     if (turn > 0 && (turn & (turn - 1)) == 0) {  // read twice as much as at the last floor
       __syncthreads();
-      float val;
-      int idx, before;
-      if (candidates(s_list) <= kSelThreads && rank_of_mine(s_list, &val, &idx, &before) &&
-          before == p.width - 1)
-        atomicMax(&s_floor, order_of(val));
+      if (warp == 0 && candidates(s_list) <= kSelThreads) {
+        uint32_t key[kPerLane];
+        int token[kPerLane];
+        gather(s_list, key, token);
+        best_of(key, token, p.width, [&](int k, uint32_t v, int) {
+          if (k == p.width - 1) atomicMax(&s_floor, v);
+        });
+      }
       __syncthreads();
     }
     r.floor = fmaxf(r.floor, of_order(*const_cast<volatile uint32_t*>(&s_floor)));
@@ -508,12 +529,11 @@ __global__ void __launch_bounds__(kSelThreads, 3) beam_stretch_kernel(const Beam
     s_sum[warp] = r.sum;
   }
   __syncthreads();
-  // The candidates, each ranked among all by its own thread; more than a few come
-  // down to `width` of each warp first.
+  // Of more candidates than one warp's registers take, `width` of each warp are enough.
   if (candidates(s_list) > kSelThreads) {  // the same in every thread
     float val;
     int idx;
-    take_best(&list, 1, p.width, &val, &idx);
+    take_best(list, p.width, &val, &idx);
     __syncthreads();
     if (lane < p.width) {
       list.val[lane] = val;
@@ -522,18 +542,20 @@ __global__ void __launch_bounds__(kSelThreads, 3) beam_stretch_kernel(const Beam
     if (lane == 0) list.n = min(list.n, p.width);
     __syncthreads();
   }
-  const long long at = row * p.splits + blockIdx.x;
-  float val;
-  int idx, before;
-  if (rank_of_mine(s_list, &val, &idx, &before) && before < p.width) {
-    p.part_val[at * p.width + before] = val;
-    p.part_idx[at * p.width + before] = idx;
-  }
   if (warp != 0) return;
-  const int n_all = candidates(s_list);
-  if (lane >= n_all && lane < p.width) {
-    p.part_val[at * p.width + lane] = -INFINITY;
-    p.part_idx[at * p.width + lane] = INT_MAX;
+  const long long at = row * p.splits + blockIdx.x;
+  uint32_t key[kPerLane], value = order_of(-INFINITY);
+  int tokens[kPerLane], token = INT_MAX;
+  gather(s_list, key, tokens);
+  best_of(key, tokens, p.width, [&](int k, uint32_t v, int t) {
+    if (lane == k) {
+      value = v;
+      token = t;
+    }
+  });
+  if (lane < p.width) {
+    p.part_val[at * p.width + lane] = of_order(value);
+    p.part_idx[at * p.width + lane] = token;
   }
   float ref_all = kNothing, sum_all = 0.f;
 #pragma unroll
