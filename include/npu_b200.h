@@ -184,7 +184,7 @@ NPU_B200_API int npu_b200_prefill_attention(const void* d_q, const void* d_k, co
  * own key and value are in the pages already: npu_b200_paged_append), head h with
  * KV head h / (q_heads / kv_heads); the counterpart of npu_b200_flash_decode:
  *
- *   d_q, d_out [batch, q_heads, head_dim] FP16, 16-byte aligned; any group
+ *   d_q, d_out [batch, q_heads, head_dim] FP16, 16-byte aligned, apart; any group
  *   d_seq_lens [batch] int32 keys per sequence, clamped to [0, table_entries x
  *              page_size]; 0 keys gives a zero row
  *   d_workspace npu_b200_paged_decode_workspace_size() bytes, 16-byte aligned, on
@@ -210,9 +210,9 @@ NPU_B200_API int npu_b200_paged_decode(const void* d_q, const void* d_k_pages,
  * and values being in the pages already.  Causal, with the window and the sinks
  * of every query's own position.
  *
- *   d_q, d_out [batch, q_heads, queries, head_dim] FP16, 16-byte aligned.  Rows past
- *              d_q_lens[b], at a negative position, or without a visible key, are
- *              zero
+ *   d_q, d_out [batch, q_heads, queries, head_dim] FP16, 16-byte aligned, apart.
+ *              Rows past d_q_lens[b], at a negative position, or without a visible
+ *              key, are zero
  *   d_seq_lens [batch] int32 keys per sequence, the chunk included, clamped to
  *              [0, table_entries x page_size]; d_q_lens [batch] int32, clamped to
  *              [0, queries]
@@ -227,8 +227,8 @@ NPU_B200_API int npu_b200_paged_prefill(const void* d_q, const void* d_k_pages,
 
 /* New rows of K and V into the pages: row i < d_lens[b] (NULL: every row) of
  * sequence b to position d_starts[b] + i.  d_k, d_v [batch, kv_heads, rows,
- * head_dim] FP16, 16-byte aligned; batch <= 65535.  Two rows that the tables send
- * to one place leave either of them there. */
+ * head_dim] FP16, 16-byte aligned, apart from the pages; batch <= 65535.  Two rows
+ * that the tables send to one place leave either of them there. */
 NPU_B200_API int npu_b200_paged_append(const void* d_k, const void* d_v, void* d_k_pages,
                                        void* d_v_pages, const int32_t* d_page_table,
                                        const int32_t* d_starts, const int32_t* d_lens, int batch,
@@ -304,7 +304,8 @@ NPU_B200_API int npu_b200_page_copy(void* d_pool, const int32_t* d_pages, const 
  *   d_out_scores, d_out_tokens, d_out_parents [batch, width]: parents are rows
  *     batch x beams + beam, as npu_b200_page_update and npu_b200_beam_reorder take
  *     them.  Where no continuation is left: -inf, -1, -1
- *   d_out_done [batch, width] bytes or NULL: finished, now or before
+ *   d_out_done [batch, width] bytes or NULL: finished, now or before; scores and flags
+ *     apart from the old ones
  *   beams and width in 1..32, batch x beams <= 65535, vocab <= 2^24
  *   d_workspace npu_b200_beam_select_workspace_size() bytes, 16-byte aligned, on
  *     the current device; holds nothing between calls

@@ -746,6 +746,10 @@ extern "C" int npu_b200_beam_select(const void* d_logits, int logits_f32, const 
               "beam_select: workspace of %zu bytes (16-byte aligned) needed, %zu given", need,
               workspace_bytes);
   const long long rows = static_cast<long long>(batch) * beams;
+  const size_t chosen = static_cast<size_t>(batch) * width;
+  NPU_REQUIRE(!overlap(d_scores, rows * 4, d_out_scores, chosen * 4) &&
+                  !(d_done != nullptr && d_out_done != nullptr && overlap(d_done, rows, d_out_done, chosen)),
+              "beam_select: the new scores and flags must not overlap the old ones");
   BeamParams p;
   p.logits = d_logits;
   p.scores = d_scores;
@@ -787,7 +791,7 @@ extern "C" int npu_b200_beam_reorder(const void* d_state, const int32_t* d_paren
   NPU_REQUIRE(rows >= 1 && new_rows >= 1 && row_bytes >= 1 && row_bytes < size_t(1) << 40,
               "beam_reorder: %d rows to %d of %zu bytes", rows, new_rows, row_bytes);
   const uintptr_t a = reinterpret_cast<uintptr_t>(d_state), b = reinterpret_cast<uintptr_t>(d_out);
-  NPU_REQUIRE(a >= b + row_bytes * new_rows || b >= a + row_bytes * rows,
+  NPU_REQUIRE(!overlap(d_state, row_bytes * rows, d_out, row_bytes * new_rows),
               "beam_reorder: the output must not overlap the state");
   ReorderParams p = {d_state, d_out, d_parents, 0, rows, new_rows};
   const cudaStream_t s = static_cast<cudaStream_t>(stream);

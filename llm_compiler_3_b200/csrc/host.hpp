@@ -53,6 +53,12 @@ void graph_free(GraphState* g);
 int ctx_device(const npu_b200_ctx* c);
 GraphState*& ctx_graph(npu_b200_ctx* c);
 
+// Whether two ranges of memory have a byte in common.
+inline bool overlap(const void* a, size_t an, const void* b, size_t bn) {
+  const uintptr_t x = reinterpret_cast<uintptr_t>(a), y = reinterpret_cast<uintptr_t>(b);
+  return x < y + bn && y < x + an;
+}
+
 // Launch helper: enables programmatic dependent launch when `pdl` is set.
 struct LaunchCfg {
   dim3 grid, block;

@@ -86,6 +86,11 @@ extern "C" int npu_b200_paged_append(const void* d_k, const void* d_v, void* d_k
               "paged_append: %d rows out of range", rows);
   NPU_REQUIRE(aligned16(d_k) && aligned16(d_v) && aligned16(d_k_pages) && aligned16(d_v_pages),
               "paged_append: k, v and pages must be 16-byte aligned");
+  const size_t bytes = static_cast<size_t>(batch) * kv_heads * rows * head_dim * 2;
+  const size_t pool = static_cast<size_t>(num_pages) * kv_heads * page_size * head_dim * 2;
+  NPU_REQUIRE(!overlap(d_k, bytes, d_k_pages, pool) && !overlap(d_v, bytes, d_v_pages, pool) &&
+                  !overlap(d_k, bytes, d_v_pages, pool) && !overlap(d_v, bytes, d_k_pages, pool),
+              "paged_append: k and v must not overlap the pages");
   AppendParams p;
   p.k = static_cast<const uint4*>(d_k);
   p.v = static_cast<const uint4*>(d_v);

@@ -420,11 +420,6 @@ __global__ void __launch_bounds__(kCopyThreads) page_copy_kernel(const CopyParam
   }
 }
 
-bool overlap(const void* a, size_t an, const void* b, size_t bn) {
-  const uintptr_t x = reinterpret_cast<uintptr_t>(a), y = reinterpret_cast<uintptr_t>(b);
-  return x < y + bn && y < x + an;
-}
-
 }  // namespace
 }  // namespace npu_b200
 

@@ -145,6 +145,28 @@ def test_append_refusals(change, message):
     assert message.encode() in _native.lib().npu_b200_last_error()
 
 
+def test_outputs_over_inputs_are_refused():
+    """On the host, before any CUDA call: the kernels read what they would overwrite."""
+    from llm_compiler_3_b200 import _native
+    lib = _native.lib()
+    p = [(i + 1) << 28 for i in range(9)]
+
+    def refused(rc):
+        return rc == -1 and b"overlap" in lib.npu_b200_last_error()
+
+    q_bytes = 3 * 8 * 128 * 2
+    for shift in (0, 16, q_bytes - 16, 16 - q_bytes):
+        assert refused(lib.npu_b200_paged_decode(*p[:5], p[0] + shift, 3, 8, 2, 128, 9, 16, 4, 0, 0, 0.1, p[6],
+                                                 1 << 26, None))
+        assert refused(lib.npu_b200_paged_prefill(p[0], p[1], p[2], p[3], p[4], None, p[0] + 5 * shift, 3, 8, 2, 128,
+                                                  5, 9, 16, 4, 0, 0, 0.1, None))
+    for k, v in ((p[2], p[1]), (p[0], p[3] + 16), (p[3], p[1]), (p[0], p[2] + 9 * 2 * 16 * 128 * 2 - 16)):
+        assert refused(lib.npu_b200_paged_append(k, v, p[2], p[3], p[4], p[5], None, 3, 2, 5, 128, 9, 16, 4, None))
+    for scores, done in ((p[1], p[7]), (p[3], p[2])):
+        assert refused(lib.npu_b200_beam_select(p[0], 0, p[1], p[2], scores, p[4], p[5], done, 2, 4, 50, 4, 1, p[8],
+                                                1 << 26, None))
+
+
 def test_operators_refuse_cpu_tensors():
     from llm_compiler_3_b200 import ops
     k, v, table = paged_cache([5], 1, 64, 8)
