@@ -42,6 +42,10 @@ void prefill_blocking(int queries, int group, int* bm, int* hp);  // prefill_att
 namespace {
 
 constexpr int KT = 128;           // keys per tile
+// A tile is four units of 32 keys, one after the other in the list of the units that hold
+// visible keys: sinks and the window's ragged ends cost a unit, not a tile (a window of
+// 1024 with 8 sinks, two chunks up to 2999 at head size 64: 87 -> 77 us).
+constexpr int kUnit = 32;
 constexpr int kThreads = 352;
 constexpr uint32_t kTmemCols = 512;
 constexpr float kRescaleLog2 = 8.f;
@@ -105,7 +109,7 @@ __device__ __forceinline__ uint32_t first_bits(int n) {
 struct Span {
   int seq_len, q_len, first_pos;  // first_pos: position of query 0 of the chunk
   int lo, len, s;                 // keys that some of the CTA's queries see: [0, s) and [lo, len)
-  TileRange<KT> tiles;
+  TileRange<kUnit> units;
   __device__ __forceinline__ bool sees(int j) const { return j < len && (j >= lo || j < s); }
   __device__ __forceinline__ bool sees_any(int j, int n) const { return j < len && (j + n > lo || j < s); }
   __device__ __forceinline__ bool sees_all(int j, int n) const {
@@ -229,13 +233,23 @@ __global__ void __launch_bounds__(kThreads, 1)
     span.len = m_hi > m_lo ? max(0, span.first_pos + m_hi) : 0;
     span.lo = p.window > 0 ? max(0, first - p.window + 1) : 0;
     span.s = min(p.sinks, span.lo);
-    span.tiles.set(span.lo, span.len, p.sinks);
-    if (span.len == 0) span.tiles.n = 0;
+    span.units.set(span.lo, span.len, p.sinks);
+    if (span.len == 0) span.units.n = 0;
   }
   // This CTA's tiles of keys: all, or its even share of them.
-  const int tile0 = static_cast<int>(static_cast<long long>(span.tiles.n) * rank / p.splits);
-  const int n_tiles = static_cast<int>(static_cast<long long>(span.tiles.n) * (rank + 1) / p.splits) - tile0;
-  auto key_of = [&](int j) { return span.tiles.key0(tile0 + j); };
+  const long long n_all = (span.units.n + KT / kUnit - 1) / (KT / kUnit);
+  const int tile0 = static_cast<int>(n_all * rank / p.splits);
+  const int n_tiles = static_cast<int>(n_all * (rank + 1) / p.splits) - tile0;
+  // The key of row `row` of tile j (past the last unit: a hidden one), and whether some query
+  // sees each key of the tile.
+  auto key_of = [&](int j, int row) {
+    return span.units.key0((tile0 + j) * (KT / kUnit) + row / kUnit) + row % kUnit;
+  };
+  auto whole = [&](int j) {
+    bool all = true;
+    for (int row = 0; row < KT; row += kUnit) all = all && span.sees_all(key_of(j, row), kUnit);
+    return all;
+  };
 
   if (threadIdx.x == 0) {
     mbar_init(q_full, 1);
@@ -264,15 +278,6 @@ __global__ void __launch_bounds__(kThreads, 1)
   // this one to end, and this one for the TMEM.
   pdl_launch_dependents();
   const uint32_t tmem = __shfl_sync(0xffffffffu, *tmem_slot, 0);
-
-  // Phase of raw[x % stages] for the V tile at place x: how many border tiles used
-  // the stage before.
-  auto raw_phase = [&](int x) {
-    uint32_t n = 0;
-    for (int y = x - kStages; y > 0; y -= kStages)
-      if ((y & 1) && !span.sees_all(key_of(y / 2), KT)) ++n;
-    return n & 1;
-  };
 
   // A softmax thread's row.
   const int tt = (warp >> 2) & 1, r = threadIdx.x & 127;
@@ -318,15 +323,16 @@ __global__ void __launch_bounds__(kThreads, 1)
       const int my_region = lane % S::kRegions, my_row = lane / S::kRegions * p.box;
       const bool mine = lane < combos;
       auto look_up = [&](int j) {  // the page of this lane's box of tile j; -2: nothing visible
-        const int at = key_of(j) + my_row;
+        const int at = key_of(j, my_row);
         if (!mine || !span.sees_any(at, p.box)) return -2;
         return p.table[static_cast<size_t>(b) * p.entries + at / p.page_size];
       };
       int page = look_up(0);
       bool ok = true;
       int issued = 0;
+      uint32_t raw_uses = 0, was_raw = 0;  // bit s: raw[s] was used an odd number of times; last
       for (int j = 0; ok && j < n_tiles; ++j) {
-        const int at = key_of(j) + my_row;
+        const int at = key_of(j, my_row);
         int row = p.total_rows;  // past the pool: the box is filled with zeros
         if (page >= 0 && page < p.num_pages)
           row = (page * p.kv_heads + hk) * p.page_size + at % p.page_size;
@@ -338,7 +344,10 @@ __global__ void __launch_bounds__(kThreads, 1)
           if (x >= kStages)
             ok = __all_sync(0xffffffffu, wait_or_abort(&empty[s], ((x / kStages) - 1) & 1, abort_flag));
           if (!ok) break;
-          uint64_t* bar = kv && !span.sees_all(key_of(j), KT) ? &raw[s] : &full[s];
+          const bool border = kv && !whole(j);
+          uint64_t* bar = border ? &raw[s] : &full[s];
+          was_raw = (was_raw & ~(1u << s)) | (border ? 1u << s : 0u);
+          raw_uses ^= border ? 1u << s : 0u;
           if (lane == 0) mbar_arrive_expect_tx(bar, S::kTileBytes);
           __syncwarp();
           if (mine)
@@ -352,8 +361,8 @@ __global__ void __launch_bounds__(kThreads, 1)
       mbar_wait(q_full, 0, kDevErrTmaTimeout);
       for (int x = max(0, issued - kStages); x < issued; ++x) {
         const int s = x % kStages;
-        const bool border = (x & 1) && !span.sees_all(key_of(x / 2), KT);
-        mbar_wait(border ? &raw[s] : &full[s], border ? raw_phase(x) : (x / kStages) & 1, kDevErrTmaTimeout);
+        const bool border = was_raw >> s & 1;
+        mbar_wait(border ? &raw[s] : &full[s], border ? ~raw_uses >> s & 1 : (x / kStages) & 1, kDevErrTmaTimeout);
       }
     }
   } else if (warp == 9) {
@@ -434,12 +443,14 @@ __global__ void __launch_bounds__(kThreads, 1)
     // ---------------- hidden rows of V ----------------
     // Rows that no query here sees may hold anything; their weights are 0, but
     // 0 * NaN is NaN.
+    uint32_t raw_uses = 0;  // bit s: raw[s] was used an odd number of times
     for (int j = 0; j < n_tiles; ++j) {
-      const int key0 = key_of(j), x = 2 * j + 1, s = x % kStages;
-      if (span.sees_all(key0, KT)) continue;
-      if (!__all_sync(0xffffffffu, wait_or_abort(&raw[s], raw_phase(x), abort_flag))) break;
+      const int s = (2 * j + 1) % kStages;
+      if (whole(j)) continue;
+      if (!__all_sync(0xffffffffu, wait_or_abort(&raw[s], raw_uses >> s & 1, abort_flag))) break;
+      raw_uses ^= 1u << s;
       for (int r = lane; r < KT; r += 32)
-        if (!span.sees(key0 + r))
+        if (!span.sees(key_of(j, r)))
           for (int a = 0; a < S::kRegions; ++a)
             for (int c = 0; c < 128; c += 16)
               *reinterpret_cast<uint4*>(smem + S::kRing + s * S::kTileBytes + a * S::kRegion +
@@ -465,13 +476,13 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll
       for (int c = 0; c < KT; c += 32) tmem_ld32(t_s + c, sr + c);
       tmem_ld_wait();
-      const int key0 = key_of(j);
-      // Hidden keys, 32 to a word of bits (comparing key by key took 640 instructions).
-      if (!__all_sync(0xffffffffu, key0 + KT - 1 <= last && (key0 >= lo || key0 + KT <= p.sinks))) {
+      // Hidden keys, a unit to a word of bits (comparing key by key took 640 instructions).
+      const int first_key = key_of(j, 0), last_key = key_of(j, KT - 1);
+      if (!__all_sync(0xffffffffu, last_key <= last && (first_key >= lo || last_key < p.sinks))) {
 #pragma unroll
         for (int c = 0; c < KT; c += 32) {
-          const uint32_t seen = first_bits(last + 1 - key0 - c) &
-                                (~first_bits(lo - key0 - c) | first_bits(p.sinks - key0 - c));
+          const int key0 = key_of(j, c);
+          const uint32_t seen = first_bits(last + 1 - key0) & (~first_bits(lo - key0) | first_bits(p.sinks - key0));
           if (__all_sync(0xffffffffu, seen == ~0u)) continue;
 #pragma unroll
           for (int e = 0; e < 32; ++e)
@@ -652,7 +663,7 @@ int launch_pp(const CUtensorMap& qm, const CUtensorMap& km, const CUtensorMap& v
   const long long pairs = static_cast<long long>(batch) * p.kv_heads * ((n_units + 1) / 2);
   const long long keys = static_cast<long long>(p.entries) * p.page_size;
   long long most = (keys + KT - 1) / KT;
-  if (p.window > 0) most = std::min(most, (static_cast<long long>(p.window) + 2 * p.bm) / KT + p.sinks / KT + 2);
+  if (p.window > 0) most = std::min(most, (static_cast<long long>(p.window) + 2 * p.bm + p.sinks) / KT + 2);
   p.splits = 1;
   while (p.splits < kMaxSplits && pairs * p.splits * 2 <= sm_count() && p.splits * 2 <= most) p.splits *= 2;
   LaunchCfg cfg;
@@ -705,7 +716,7 @@ extern "C" int npu_b200_paged_prefill(const void* d_q, const void* d_k_pages, co
   p.queries = queries;
   p.entries = table_entries;
   p.page_size = page_size;
-  p.box = page_box(page_size, KT);
+  p.box = page_box(page_size, window > 0 ? kUnit : KT);  // without a window units are in line
   p.num_pages = num_pages;
   const uint64_t rows = static_cast<uint64_t>(num_pages) * kv_heads * page_size;
   p.total_rows = static_cast<int>(rows);

@@ -236,3 +236,14 @@ def test_keys_shared_by_a_cluster(cuda, heads, kv_heads, dim, queries, window, s
     got = check_prefill(q, k, v, table, lens, q_lens, window=window, sinks=sinks)
     assert torch.equal(got, _prefill(q, k, v, table, lens, q_lens, window=window, sinks=sinks))
     check_prefill(q[:1], k, v, table[:1], lens[:1], q_lens[:1], window=window, sinks=sinks)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("page", [8, 24, 40, 64, 128])
+@pytest.mark.parametrize("dim,window,sinks", [(64, 150, 33), (128, 95, 8), (64, 1, 200), (128, 257, 0), (64, 32, 32)])
+def test_windows_over_units_of_keys(cuda, page, dim, window, sinks):
+    """Sinks, gap and window in one tile, in units of 32 keys that pages of other sizes cut across;
+    sinks that run into the window; chunks that begin anywhere."""
+    lens, q_lens = [700, 333, 65, 20], [140, 33, 65, 7]
+    k, v, table = paged_cache(lens, 1, dim, page, seed=page + sinks)
+    check_prefill(seeded((4, 2, 140, dim), 9), k, v, table, lens, q_lens, window=window, sinks=sinks)
