@@ -44,7 +44,8 @@ namespace {
 constexpr int KT = 128;           // keys per tile
 // A tile is four units of 32 keys, one after the other in the list of the units that hold
 // visible keys: sinks and the window's ragged ends cost a unit, not a tile (a window of
-// 1024 with 8 sinks, two chunks up to 2999 at head size 64: 87 -> 77 us).
+// 1024 with 8 sinks, two chunks up to 2999 at head size 64, 128 queries to a tile: 87 -> 77
+// us).
 constexpr int kUnit = 32;
 constexpr int kThreads = 352;
 constexpr uint32_t kTmemCols = 512;
@@ -721,6 +722,14 @@ extern "C" int npu_b200_paged_prefill(const void* d_q, const void* d_k_pages, co
   const uint64_t rows = static_cast<uint64_t>(num_pages) * kv_heads * page_size;
   p.total_rows = static_cast<int>(rows);
   prefill_blocking(queries, q_heads / kv_heads, &p.bm, &p.hp);
+  // Behind a window, more heads of fewer queries, which see fewer keys between them: 64
+  // queries on 4 heads see 1087 of a window of 1024, 128 on 2 see 1151 (two chunks up to 2999
+  // at head size 64: 77 -> 55 us).  Without one it only costs copies of Q (40 queries of 32
+  // heads on 8 behind 16384 keys: 49 -> 52 us).
+  while (window > 0 && p.bm > 16 && q_heads / kv_heads % (2 * p.hp) == 0) {
+    p.bm /= 2;
+    p.hp *= 2;
+  }
   p.q_blocks = (queries + p.bm - 1) / p.bm;
   NPU_REQUIRE((static_cast<long long>(p.q_blocks) * (q_heads / kv_heads / p.hp) + 1) / 2 <= 65535,
               "paged_prefill: %d queries make too many query blocks", queries);
