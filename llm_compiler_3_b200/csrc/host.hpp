@@ -95,4 +95,32 @@ int launch(const LaunchCfg& c, void (*kernel)(KArgs...), Args&&... args) {
                     "cudaLaunchKernelEx");
 }
 
+// How many clusters of `size` CTAs (2, 4 or 8; `size` 1: CTAs) of KERNEL run at once on the
+// current device, asked once: clusters of 8 that fill an SM each leave 28 of 148 SMs idle.
+template <auto KERNEL>
+int clusters_at_once(int size, dim3 block, size_t smem) {
+  static int cached[64][9] = {};
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64 || size > 8) return 0;
+  if (cached[dev][size] == 0) {
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(size);
+    cfg.blockDim = block;
+    cfg.dynamicSmemBytes = smem;
+    cudaLaunchAttribute attr = {};
+    attr.id = cudaLaunchAttributeClusterDimension;
+    attr.val.clusterDim.x = size;
+    attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
+    cfg.attrs = &attr;
+    cfg.numAttrs = 1;
+    int n = 0;
+    if (cudaOccupancyMaxActiveClusters(&n, KERNEL, &cfg) != cudaSuccess) {
+      cudaGetLastError();
+      n = 0;
+    }
+    cached[dev][size] = n > 0 ? n : -1;
+  }
+  return cached[dev][size];
+}
+
 }  // namespace npu_b200

@@ -16,11 +16,14 @@
 // lies in one stretch is written out at once; the parts of one that crosses a
 // border go to the workspace and are joined by a second, dependent launch in
 // the order of the stretches (no counters to clear, and no order that changes
-// between runs).  Measured: 1.09 GB of ragged lengths up to 8192 in 186 us, 5.9
+// between runs).  Measured: 1.09 GB of ragged lengths up to 8192 in 187 us, 5.8
 // TB/s.  What is left is that equal stretches do not take equal time (126 to 193
 // us); dealing out the last three tenths in small stretches through a counter
 // evened that out and still took as long (188 to 200 us), for the time that each
 // change of stretch costs.
+//
+// Few short units go without the line: a cluster of up to 8 CTAs takes each, and
+// joins its parts in distributed shared memory, so that one launch does it all.
 //
 // Inside a stretch every warp takes each WARPS-th tile through its own TMA ring
 // (K and V of 32 keys, 128-byte swizzle, one box per page piece: 32 rows, or
@@ -39,6 +42,8 @@ namespace npu_b200 {
 namespace {
 
 constexpr float kRescaleLog2 = 8.f;
+constexpr int kMaxShares = 8;  // CTAs of a cluster
+constexpr int kFewTiles = 8;   // tiles of a warp, at most, where clusters take the units
 
 template <int D, int NB>
 struct PdShape {
@@ -70,6 +75,7 @@ struct PdParams {
   int batch, q_heads, kv_heads, group, chunks;  // chunks: blocks of 8 NB query heads per KV head
   int entries, page_size, box, num_pages, total_rows;
   int window, sinks, pitch;
+  int shares;       // CTAs of a cluster that share one unit; 0: stretches of the line
   Divisor by_page;
   float scale_log2;
 };
@@ -156,6 +162,8 @@ __global__ void __launch_bounds__(PdShape<D, NB>::kThreads, 1)
   float* cM = cw + kWarps * S::kHeads;                     // [heads]
   float* cL = cM + S::kHeads;                              // [heads]
   uint64_t* bars = reinterpret_cast<uint64_t*>(smem + S::kBars);
+  // A share's part, O [heads][D] and the heads' maxima and sums, over the ring at the end.
+  float* share = reinterpret_cast<float*>(smem);
   __shared__ long long s_sum[kWarps];
   __shared__ long long s_base;
   __shared__ int s_b;
@@ -175,57 +183,70 @@ __global__ void __launch_bounds__(PdShape<D, NB>::kThreads, 1)
   pdl_wait();
 
   // ---- this CTA's stretch [t0, t1) of the line, and where it begins ----
-  const int units = p.kv_heads * p.chunks;
-  const int each = (p.batch + kWarps * 32 - 1) / (kWarps * 32);  // sequences per thread
-  const int b_first = min(static_cast<int>(threadIdx.x) * each, p.batch);
-  const int b_end = min(b_first + each, p.batch);
-  long long mine = 0;
   Place<kTile> at;
-  for (int b = b_first; b < b_end; ++b) {
-    at.keys.set(p, b);
-    mine += static_cast<long long>(at.keys.tiles.n) * units;
-  }
-  long long upto = mine;  // inclusive scan over the threads
-#pragma unroll
-  for (int o = 1; o < 32; o <<= 1) {
-    const long long v = __shfl_up_sync(0xffffffffu, upto, o);
-    if (lane >= o) upto += v;
-  }
-  if (lane == 31) s_sum[warp] = upto;
-  __syncthreads();
-  long long total = 0;
-#pragma unroll
-  for (int w = 0; w < kWarps; ++w) {
-    if (w < warp) upto += s_sum[w];
-    total += s_sum[w];
-  }
-  long long per = (total + gridDim.x - 1) / gridDim.x;
-  per = max(per, static_cast<long long>(kWarps));  // no warp without a tile
-  const long long t0 = blockIdx.x * per, t1 = min(total, t0 + per);
-  if (threadIdx.x == 0) p.joins[blockIdx.x] = make_int4(0, 0, 0, 0);
-  if (t0 >= t1) return;
-  if (t0 >= upto - mine && t0 < upto) {  // exactly one thread
-    long long base = upto - mine;
+  long long t0, t1, per = 1;
+  const int units = p.kv_heads * p.chunks;
+  if (p.shares > 0) {  // or its share of one unit's tiles
+    const int unit = static_cast<int>(blockIdx.x) / p.shares, rank = static_cast<int>(blockIdx.x) % p.shares;
+    at.b = unit / units;
+    at.h = (unit - at.b * units) / p.chunks;
+    at.c = unit - at.b * units - at.h * p.chunks;
+    at.keys.set(p, at.b);
+    t0 = static_cast<long long>(at.keys.tiles.n) * rank / p.shares;
+    t1 = static_cast<long long>(at.keys.tiles.n) * (rank + 1) / p.shares;
+    at.i = static_cast<int>(t0);
+  } else {
+    const int each = (p.batch + kWarps * 32 - 1) / (kWarps * 32);  // sequences per thread
+    const int b_first = min(static_cast<int>(threadIdx.x) * each, p.batch);
+    const int b_end = min(b_first + each, p.batch);
+    long long mine = 0;
     for (int b = b_first; b < b_end; ++b) {
       at.keys.set(p, b);
-      const long long n = static_cast<long long>(at.keys.tiles.n) * units;
-      if (t0 < base + n) {
-        s_b = b;
-        s_base = base;
-        break;
-      }
-      base += n;
+      mine += static_cast<long long>(at.keys.tiles.n) * units;
     }
-  }
-  __syncthreads();
-  at.b = s_b;
-  at.keys.set(p, at.b);
-  {
-    const long long rem = t0 - s_base;
-    const int unit = static_cast<int>(rem / at.keys.tiles.n);
-    at.i = static_cast<int>(rem - static_cast<long long>(unit) * at.keys.tiles.n);
-    at.h = unit / p.chunks;
-    at.c = unit - at.h * p.chunks;
+    long long upto = mine;  // inclusive scan over the threads
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const long long v = __shfl_up_sync(0xffffffffu, upto, o);
+      if (lane >= o) upto += v;
+    }
+    if (lane == 31) s_sum[warp] = upto;
+    __syncthreads();
+    long long total = 0;
+#pragma unroll
+    for (int w = 0; w < kWarps; ++w) {
+      if (w < warp) upto += s_sum[w];
+      total += s_sum[w];
+    }
+    per = (total + gridDim.x - 1) / gridDim.x;
+    per = max(per, static_cast<long long>(kWarps));  // no warp without a tile
+    t0 = blockIdx.x * per;
+    t1 = min(total, t0 + per);
+    if (threadIdx.x == 0) p.joins[blockIdx.x] = make_int4(0, 0, 0, 0);
+    if (t0 >= t1) return;
+    if (t0 >= upto - mine && t0 < upto) {  // exactly one thread
+      long long base = upto - mine;
+      for (int b = b_first; b < b_end; ++b) {
+        at.keys.set(p, b);
+        const long long n = static_cast<long long>(at.keys.tiles.n) * units;
+        if (t0 < base + n) {
+          s_b = b;
+          s_base = base;
+          break;
+        }
+        base += n;
+      }
+    }
+    __syncthreads();
+    at.b = s_b;
+    at.keys.set(p, at.b);
+    {
+      const long long rem = t0 - s_base;
+      const int unit = static_cast<int>(rem / at.keys.tiles.n);
+      at.i = static_cast<int>(rem - static_cast<long long>(unit) * at.keys.tiles.n);
+      at.h = unit / p.chunks;
+      at.c = unit - at.h * p.chunks;
+    }
   }
   const int n_mine = static_cast<int>(t1 - t0);
   const int my_tiles = n_mine > warp ? (n_mine - warp + kWarps - 1) / kWarps : 0;
@@ -465,8 +486,8 @@ __global__ void __launch_bounds__(PdShape<D, NB>::kThreads, 1)
       cL[head] = L;
     }
     __syncthreads();
-    const bool alone = at.i == 0 && here == at.keys.tiles.n;
-    float* slot = p.part + (static_cast<size_t>(blockIdx.x) * 2 + (done == 0 ? 0 : 1)) * p.pitch;
+    const bool alone = p.shares < 2 && at.i == 0 && here == at.keys.tiles.n;
+    float* slot = p.shares > 0 ? share : p.part + (static_cast<size_t>(blockIdx.x) * 2 + (done == 0 ? 0 : 1)) * p.pitch;
     for (int x = threadIdx.x; x < heads * D / 4; x += kWarps * 32) {
       const int head = x * 4 / D, dim = x * 4 - head * D;
       float4 O = make_float4(0.f, 0.f, 0.f, 0.f);
@@ -493,13 +514,50 @@ __global__ void __launch_bounds__(PdShape<D, NB>::kThreads, 1)
     }
     // A unit that begins here and goes on in the next stretches: its parts are
     // this slot and the first slots of the CTAs that follow.
-    if (threadIdx.x == 0 && at.i == 0 && here < at.keys.tiles.n) {
+    if (threadIdx.x == 0 && at.i == 0 && here < at.keys.tiles.n && p.shares == 0) {
       const int others = static_cast<int>((at.keys.tiles.n - here + per - 1) / per);
       p.joins[blockIdx.x] = make_int4(1 + others, static_cast<int>(q_row), heads, done == 0 ? 0 : 1);
     }
     done += here;
+    if (p.shares > 0) break;
     at.forward(p, here);
     __syncthreads();  // the join buffer is free again
+  }
+  if (p.shares > 1) {
+    // ---- the cluster's parts of the unit join, each CTA's share of the output ----
+    const int heads = min(S::kHeads, p.group - at.c * S::kHeads);
+    if (n_mine == 0 && threadIdx.x < S::kHeads) {
+      share[S::kHeads * D + threadIdx.x] = -INFINITY;
+      share[S::kHeads * D + S::kHeads + threadIdx.x] = 0.f;
+    }
+    cluster_sync_all();
+    const int rank = static_cast<int>(blockIdx.x) % p.shares;
+    const size_t q_row = static_cast<size_t>(at.b) * p.q_heads + at.h * p.group + at.c * S::kHeads;
+    for (int x = rank * S::kThreads + threadIdx.x; x < heads * D / 4; x += p.shares * S::kThreads) {
+      const int head = x * 4 / D, dim = x * 4 - head * D;
+      float m[kMaxShares], mx = -INFINITY, L = 0.f;
+      float4 O = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+      for (int c = 0; c < kMaxShares; ++c) {
+        m[c] = c < p.shares ? ld_cluster_f32(cluster_map(smem_u32(share + S::kHeads * D + head), c)) : -INFINITY;
+        mx = fmaxf(mx, m[c]);
+      }
+#pragma unroll
+      for (int c = 0; c < kMaxShares; ++c) {
+        if (m[c] == -INFINITY) continue;
+        const float wt = fast_exp2(m[c] - mx);
+        L += wt * ld_cluster_f32(cluster_map(smem_u32(share + S::kHeads * D + S::kHeads + head), c));
+        const float4 v = ld_cluster_v4(cluster_map(smem_u32(share + head * D + dim), c));
+        O.x += v.x * wt;
+        O.y += v.y * wt;
+        O.z += v.z * wt;
+        O.w += v.w * wt;
+      }
+      const float inv = L == 0.f ? 0.f : 1.f / L;
+      *reinterpret_cast<uint2*>(p.out + (q_row + head) * D + dim) =
+          make_uint2(pack_half2(O.x * inv, O.y * inv), pack_half2(O.z * inv, O.w * inv));
+    }
+    cluster_sync_all();  // nobody reads this CTA's part any more
   }
   if (bad) {  // leave no copy in flight into this CTA's shared memory
     for (; k < issued; ++k)
@@ -536,19 +594,35 @@ __global__ void __launch_bounds__(D) paged_decode_join_kernel(const PdParams p) 
 }
 
 template <int D, int NB>
-int launch_pd(const CUtensorMap& km, const CUtensorMap& vm, const PdParams& p, long long most_tiles,
-              cudaStream_t stream) {
+int launch_pd(const CUtensorMap& km, const CUtensorMap& vm, PdParams& p, long long most, cudaStream_t stream) {
   using S = PdShape<D, NB>;
-  const int ctas = static_cast<int>(std::min<long long>(sm_count(), (most_tiles + S::kWarps - 1) / S::kWarps));
-  auto kern = paged_decode_kernel<D, NB>;
+  constexpr auto kern = paged_decode_kernel<D, NB>;
   NPU_TRY_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                     static_cast<int>(S::kSmem)));
   LaunchCfg cfg;
-  cfg.grid = dim3(ctas);
   cfg.block = dim3(S::kThreads);
   cfg.smem = S::kSmem;
   cfg.stream = stream;
   cfg.pdl = true;
+  // Few units of few tiles: a cluster to each, its CTAs sharing the keys and joining
+  // through distributed shared memory, in one launch.  32 heads on 8, 1 sequence of 1000
+  // keys 7.5 -> 6.3 us, of 4000 12.8 -> 9.3, 16 of up to 500 16.0 -> 8.3; the line is the
+  // faster one again from some 8 tiles a warp (12000 keys: 17.1, with clusters 19.3), where
+  // its even stretches and all SMs are worth a second launch.
+  const long long units = static_cast<long long>(p.batch) * p.kv_heads * p.chunks;
+  int shares = 1;
+  while (shares < kMaxShares && shares * S::kWarps < most &&
+         units <= clusters_at_once<kern>(shares * 2, cfg.block, cfg.smem))
+    shares *= 2;
+  if (units <= sm_count() && most <= static_cast<long long>(kFewTiles) * S::kWarps * shares) {
+    p.shares = shares;
+    cfg.grid = dim3(static_cast<unsigned>(units) * shares);
+    cfg.cluster = shares;
+    return launch(cfg, kern, km, vm, p);
+  }
+  p.shares = 0;
+  const int ctas = static_cast<int>(std::min<long long>(sm_count(), (most * units + S::kWarps - 1) / S::kWarps));
+  cfg.grid = dim3(ctas);
   int rc = launch(cfg, kern, km, vm, p);
   if (rc) return rc;
   LaunchCfg join;
@@ -643,9 +717,8 @@ extern "C" int npu_b200_paged_decode(const void* d_q, const void* d_k_pages, con
   long long most = (static_cast<long long>(table_entries) * page_size + tile - 1) / tile;
   if (window > 0)
     most = std::min(most, static_cast<long long>(window) / tile + sinks / tile + 4);
-  most *= static_cast<long long>(batch) * kv_heads * p.chunks;
-  NPU_REQUIRE(most < 1ll << 36, "paged_decode: a batch of %d over tables of %d entries is too large", batch,
-              table_entries);
+  NPU_REQUIRE(most * batch * kv_heads * p.chunks < 1ll << 36,
+              "paged_decode: a batch of %d over tables of %d entries is too large", batch, table_entries);
   p.joins = static_cast<int4*>(d_workspace);
   p.part = reinterpret_cast<float*>(p.joins + sm_count());
   cudaStream_t s = static_cast<cudaStream_t>(stream);

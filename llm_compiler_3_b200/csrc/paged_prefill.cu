@@ -653,11 +653,11 @@ template <int D>
 int launch_pp(const CUtensorMap& qm, const CUtensorMap& km, const CUtensorMap& vm, PpParams& p,
               int batch, cudaStream_t stream) {
   using S = PpShape<D>;
-  auto kern = paged_prefill_kernel<D>;
+  constexpr auto kern = paged_prefill_kernel<D>;
   NPU_TRY_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, S::kSmem));
   const int n_units = p.q_blocks * (p.q_heads / p.kv_heads / p.hp);
   // Few query tiles leave SMs idle: then a cluster of CTAs shares each pair's keys, as many
-  // as there are SMs for, and not more than the longest table has tiles.  A chunk of 40
+  // as run at once, and not more than the longest table has tiles.  A chunk of 40
   // tokens, 32 heads on 8: behind 16384 keys 289 -> 48 us, 4 of them behind 540 21.1 -> 18.2;
   // where the table has room for several tiles and the sequence is one, the cluster costs
   // 2 us (11.8 -> 14.0).
@@ -666,7 +666,9 @@ int launch_pp(const CUtensorMap& qm, const CUtensorMap& km, const CUtensorMap& v
   long long most = (keys + KT - 1) / KT;
   if (p.window > 0) most = std::min(most, (static_cast<long long>(p.window) + 2 * p.bm + p.sinks) / KT + 2);
   p.splits = 1;
-  while (p.splits < kMaxSplits && pairs * p.splits * 2 <= sm_count() && p.splits * 2 <= most) p.splits *= 2;
+  while (p.splits < kMaxSplits && p.splits * 2 <= most &&
+         pairs <= clusters_at_once<kern>(p.splits * 2, dim3(kThreads), S::kSmem))
+    p.splits *= 2;
   LaunchCfg cfg;
   cfg.cluster = p.splits;
   cfg.grid = dim3(batch * p.kv_heads * p.splits, (n_units + 1) / 2);

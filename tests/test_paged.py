@@ -242,6 +242,24 @@ def test_decode_batches(cuda, batch):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("batch,heads,kv_heads,dim", [(1, 4, 1, 64), (1, 20, 2, 128), (3, 12, 4, 64), (9, 5, 5, 128),
+                                                      (18, 8, 8, 64), (40, 6, 2, 128)])
+@pytest.mark.parametrize("window,sinks", [(0, 0), (90, 20)])
+def test_decode_of_few_units(cuda, batch, heads, kv_heads, dim, window, sinks):
+    """Units that clusters of 8, 4, 2 and single CTAs take, some of the CTAs without a tile, and the
+    same sequences under tables too wide for them, over the line; each the same bits twice."""
+    lens = [(i * 353 + 1) % 900 for i in range(batch)]
+    lens[-1] = max(lens[-1], 777)
+    k, v, table = paged_cache(lens, kv_heads, dim, 16, seed=batch)
+    q = seeded((batch, heads, dim), 11)
+    wide = torch.full((batch, 4096), -1, dtype=torch.int32)
+    wide[:, :table.shape[1]] = table
+    for entries in (table, wide):
+        got = check_decode(q, k, v, entries, lens, window=window, sinks=sinks)
+        assert torch.equal(got, _decode(q, k, v, entries, lens, window=window, sinks=sinks))
+
+
+@pytest.mark.gpu
 def test_decode_scores_of_any_size(cuda):
     """Scores far apart, all equal, a negative scale, and -inf keys' weights."""
     lens = [200, 200]
