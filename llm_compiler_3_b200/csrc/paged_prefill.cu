@@ -252,6 +252,16 @@ __global__ void __launch_bounds__(kThreads, 1)
     return all;
   };
 
+  // A lane of the TMA warp loads one box of each tile: rows of one page, one 64-dim region.
+  const int my_region = lane % S::kRegions, my_row = lane / S::kRegions * p.box;
+  const bool my_box = warp == 8 && lane < KT / p.box * S::kRegions;
+  auto look_up = [&](int j) {  // the page of this lane's box of tile j; -2: nothing visible
+    const int at = key_of(j, my_row);
+    if (!my_box || !span.sees_any(at, p.box)) return -2;
+    return p.table[static_cast<size_t>(b) * p.entries + at / p.page_size];
+  };
+  int page = n_tiles > 0 ? look_up(0) : -2;  // asked for before the barrier
+
   if (threadIdx.x == 0) {
     mbar_init(q_full, 1);
     for (int s = 0; s < kStages; ++s) {
@@ -319,16 +329,6 @@ __global__ void __launch_bounds__(kThreads, 1)
           }
         }
       }
-      // Each lane loads one box: rows of one page, one 64-dim region.
-      const int combos = KT / p.box * S::kRegions;
-      const int my_region = lane % S::kRegions, my_row = lane / S::kRegions * p.box;
-      const bool mine = lane < combos;
-      auto look_up = [&](int j) {  // the page of this lane's box of tile j; -2: nothing visible
-        const int at = key_of(j, my_row);
-        if (!mine || !span.sees_any(at, p.box)) return -2;
-        return p.table[static_cast<size_t>(b) * p.entries + at / p.page_size];
-      };
-      int page = look_up(0);
       bool ok = true;
       int issued = 0;
       uint32_t raw_uses = 0, was_raw = 0;  // bit s: raw[s] was used an odd number of times; last
@@ -351,7 +351,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           raw_uses ^= border ? 1u << s : 0u;
           if (lane == 0) mbar_arrive_expect_tx(bar, S::kTileBytes);
           __syncwarp();
-          if (mine)
+          if (my_box)
             tma_load_2d(smem + S::kRing + s * S::kTileBytes + my_region * S::kRegion + my_row * 128,
                         kv ? &vmap : &kmap, bar, my_region * 64, row);
           issued = x + 1;
@@ -553,15 +553,13 @@ __global__ void __launch_bounds__(kThreads, 1)
     } else if (p.splits > 1) {
       tc_fence_after();
       if (n_tiles > 0) {
-#pragma unroll 1
-        for (int c = 0; c < D; c += 16) {
-          uint32_t o[16];
-          tmem_ld16(t_o + c, o);
-          tmem_ld_wait();
+        uint32_t o[D];
 #pragma unroll
-          for (int e = 0; e < 4; ++e)
-            parts[(tt * (D / 4) + c / 4 + e) * 128 + r] = make_uint4(o[4 * e], o[4 * e + 1], o[4 * e + 2], o[4 * e + 3]);
-        }
+        for (int c = 0; c < D; c += 32) tmem_ld32(t_o + c, o + c);
+        tmem_ld_wait();
+#pragma unroll
+        for (int e = 0; e < D / 4; ++e)
+          parts[(tt * (D / 4) + e) * 128 + r] = make_uint4(o[4 * e], o[4 * e + 1], o[4 * e + 2], o[4 * e + 3]);
       }
       part_ml[tt * 128 + r] = make_float2(m_run, l_run);
     } else {
@@ -570,24 +568,23 @@ __global__ void __launch_bounds__(kThreads, 1)
       const float inv = any ? 1.f / l_run : 0.f;
       uint4* row = reinterpret_cast<uint4*>(p.out + at * D);
       bool odd = false;  // not a number
-#pragma unroll 1
-      for (int c = 0; c < D; c += 16) {
-        uint32_t o[16];
-        if (n_tiles > 0) {
-          tmem_ld16(t_o + c, o);
-          tmem_ld_wait();
-        }
-        if (row_ok) {
-          float f[16];
+      uint32_t o[D];
+      if (n_tiles > 0) {
 #pragma unroll
-          for (int e = 0; e < 16; ++e) {
-            f[e] = any ? __uint_as_float(o[e]) * inv : 0.f;
+        for (int c = 0; c < D; c += 32) tmem_ld32(t_o + c, o + c);
+        tmem_ld_wait();
+      }
+      if (row_ok) {
+#pragma unroll
+        for (int c = 0; c < D; c += 8) {
+          float f[8];
+#pragma unroll
+          for (int e = 0; e < 8; ++e) {
+            f[e] = any ? __uint_as_float(o[c + e]) * inv : 0.f;
             odd |= f[e] != f[e];
           }
           row[c / 8] = make_uint4(pack_half2(f[0], f[1]), pack_half2(f[2], f[3]), pack_half2(f[4], f[5]),
                                   pack_half2(f[6], f[7]));
-          row[c / 8 + 1] = make_uint4(pack_half2(f[8], f[9]), pack_half2(f[10], f[11]),
-                                      pack_half2(f[12], f[13]), pack_half2(f[14], f[15]));
         }
       }
       redo(odd, 0, D);
