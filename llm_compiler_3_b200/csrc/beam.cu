@@ -422,9 +422,10 @@ __device__ __forceinline__ void take_turn(uint4 (&raw)[N], int w, int width, Can
   r.sum += lo2(all2) + hi2(all2);
 }
 
-// Block (s, row): stretch s of row `row`, a piece per warp.
-template <typename T>
-__global__ void __launch_bounds__(kSelThreads, 3) beam_stretch_kernel(const BeamParams p) {
+// Block (s, row): stretch s of row `row`, a piece per warp.  CTAS to an SM: registers for
+// three, or fewer for four.
+template <typename T, int CTAS>
+__global__ void __launch_bounds__(kSelThreads, CTAS) beam_stretch_kernel(const BeamParams p) {
   using Kd = Kind<T>;
   constexpr int L = Kd::kLogits;
   __shared__ float s_ref[kSelWarps], s_sum[kSelWarps];
@@ -698,8 +699,8 @@ int launch_reorder(ReorderParams p, long long row_bytes, cudaStream_t stream) {
   return launch(cfg, beam_reorder_kernel<V>, p);
 }
 
-// Stretches of a row: as many as keep all CTAs resident at once (3 an SM), since each
-// CTA pays for its floor and its ranking; none shorter than half a turn of its
+// Stretches of a row: as many as keep all CTAs resident at once (3 an SM), since each CTA pays
+// for its floor and its last choice; none shorter than half a turn of its
 // warps, none over 2^17 logits (a lane then adds at most 64 words' sums in FP32).
 int beam_splits(long long rows, int vocab) {
   const long long want = 3ll * sm_count() / rows;
@@ -777,7 +778,14 @@ extern "C" int npu_b200_beam_select(const void* d_logits, int logits_f32, const 
   cfg.block = dim3(kSelThreads);
   cfg.stream = static_cast<cudaStream_t>(stream);
   cfg.pdl = true;
-  int rc = logits_f32 ? launch(cfg, beam_stretch_kernel<float>, p) : launch(cfg, beam_stretch_kernel<__half>, p);
+  // Where three CTAs an SM do not hold all rows at once, four do with some spilled registers
+  // (64 x 8 rows of 128256 tokens 57 -> 46 us; 100 x 4 of 32000, which three hold, 15.9 ->
+  // 18).  Not with finished beams, whose CTAs end at once: the places they leave go to the
+  // rows that wait (a fifth of them finished: 43 us, with four 49).
+  const bool four = rows * p.splits > 3ll * sm_count() && d_done == nullptr;
+  const auto stretch = logits_f32 ? (four ? beam_stretch_kernel<float, 4> : beam_stretch_kernel<float, 3>)
+                                  : (four ? beam_stretch_kernel<__half, 4> : beam_stretch_kernel<__half, 3>);
+  int rc = launch(cfg, stretch, p);
   if (rc) return rc;
   cfg.grid = dim3(batch);
   return launch(cfg, beam_join_kernel, p);

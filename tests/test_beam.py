@@ -118,6 +118,17 @@ def test_select(cuda, batch, beams, vocab, width, dtype):
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("dtype", [torch.float16, torch.float32])
+@pytest.mark.parametrize("finished", [False, True])
+def test_select_of_many_rows(cuda, dtype, finished):
+    """More rows than three CTAs an SM hold at once, with and without finished beams."""
+    logits = seeded((151, 4, 1300), 31, std=3.0).to(dtype)
+    scores = -3 * torch.rand(151, 4, generator=torch.Generator().manual_seed(7))
+    done = torch.rand(151, 4, generator=torch.Generator().manual_seed(8)) < 0.3
+    check(logits, scores, 4, *((done, 17) if finished else ()))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.float16, torch.float32])
 def test_ties_go_to_the_lowest_index(cuda, dtype):
     """All logits equal, in one and in several beams; steps of equal values."""
     logits = torch.zeros(2, 3, 9001, dtype=dtype)
