@@ -247,3 +247,39 @@ def test_windows_over_units_of_keys(cuda, page, dim, window, sinks):
     lens, q_lens = [700, 333, 65, 20], [140, 33, 65, 7]
     k, v, table = paged_cache(lens, 1, dim, page, seed=page + sinks)
     check_prefill(seeded((4, 2, 140, dim), 9), k, v, table, lens, q_lens, window=window, sinks=sinks)
+
+
+@pytest.mark.gpu
+def test_captured_and_overlapping_calls(cuda):
+    """A captured call follows the lengths and tables it finds; calls on two streams, of clusters and
+    of many CTAs, keep apart."""
+    from llm_compiler_3_b200 import _native, ops
+    lens, q_lens = [500, 61], [33, 20]
+    k, v, table = paged_cache(lens, 2, 128, 16, seed=5)
+    q = seeded((2, 8, 33, 128), 12)
+    state = [t.cuda() for t in (q, k, v, table, ints(lens), ints(q_lens))]
+    ops.paged_prefill(*state)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = ops.paged_prefill(*state)
+    for new_lens, new_q in (([500, 61], [33, 20]), ([61, 7], [1, 0]), ([300, 60], [0, 33])):
+        state[4].copy_(ints(new_lens))
+        state[5].copy_(ints(new_q))
+        graph.replay()
+        torch.cuda.synchronize()
+        check(out.cpu(), *oracle.attention_paged(q, k, v, table, new_lens, new_q))
+    other = seeded((2, 8, 700, 128), 13).cuda()
+    long = ints([500, 61]).cuda()
+    want = [ops.paged_prefill(*state), ops.paged_prefill(other, *state[1:4], long, long)]
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    for s in streams:
+        s.wait_stream(torch.cuda.current_stream())
+    got = [[], []]
+    for _ in range(8):
+        with torch.cuda.stream(streams[0]):
+            got[0].append(ops.paged_prefill(*state))
+        with torch.cuda.stream(streams[1]):
+            got[1].append(ops.paged_prefill(other, *state[1:4], long, long))
+    torch.cuda.synchronize()
+    assert _native.device_status() == 0
+    assert all(torch.equal(g, w) for gs, w in zip(got, want) for g in gs)
