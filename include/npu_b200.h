@@ -193,7 +193,8 @@ NPU_B200_API int npu_b200_prefill_attention(const void* d_q, const void* d_k, co
  * FP32 scores, softmax statistics and accumulation, softmax weights rounded to
  * FP16, the output rounded once; the work is split over the keys evenly over
  * the SMs and joined in a fixed order, so the same inputs give the same bits.
- * Launched as programmatic dependents of the stream's previous work, like
+ * Infinite and NaN queries, keys and values reach the rows that see them, whatever
+ * the split.  Launched as programmatic dependents of the stream's previous work, like
  * npu_b200_flash_decode. */
 NPU_B200_API size_t npu_b200_paged_decode_workspace_size(int q_heads, int kv_heads, int head_dim);
 NPU_B200_API int npu_b200_paged_decode(const void* d_q, const void* d_k_pages,

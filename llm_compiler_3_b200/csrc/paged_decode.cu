@@ -526,27 +526,34 @@ __global__ void __launch_bounds__(PdShape<D, NB>::kThreads, 1)
   if (p.shares > 1) {
     // ---- the cluster's parts of the unit join, each CTA's share of the output ----
     const int heads = min(S::kHeads, p.group - at.c * S::kHeads);
-    if (n_mine == 0 && threadIdx.x < S::kHeads) {
+    if (n_mine == 0 && threadIdx.x < S::kHeads) {  // no part: a sum that none has
       share[S::kHeads * D + threadIdx.x] = -INFINITY;
-      share[S::kHeads * D + S::kHeads + threadIdx.x] = 0.f;
+      share[S::kHeads * D + S::kHeads + threadIdx.x] = -1.f;
     }
     cluster_sync_all();
     const int rank = static_cast<int>(blockIdx.x) % p.shares;
     const size_t q_row = static_cast<size_t>(at.b) * p.q_heads + at.h * p.group + at.c * S::kHeads;
     for (int x = rank * S::kThreads + threadIdx.x; x < heads * D / 4; x += p.shares * S::kThreads) {
       const int head = x * 4 / D, dim = x * 4 - head * D;
-      float m[kMaxShares], mx = -INFINITY, L = 0.f;
+      float m[kMaxShares], l[kMaxShares], mx = -INFINITY, L = 0.f;
       float4 O = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
       for (int c = 0; c < kMaxShares; ++c) {
-        m[c] = c < p.shares ? ld_cluster_f32(cluster_map(smem_u32(share + S::kHeads * D + head), c)) : -INFINITY;
+        m[c] = -INFINITY;
+        l[c] = -1.f;
+        if (c >= p.shares) continue;
+        const uint32_t ml = cluster_map(smem_u32(share + S::kHeads * D + head), c);
+        m[c] = ld_cluster_f32(ml);
+        l[c] = ld_cluster_f32(ml + S::kHeads * 4);
         mx = fmaxf(mx, m[c]);
       }
 #pragma unroll
       for (int c = 0; c < kMaxShares; ++c) {
-        if (m[c] == -INFINITY) continue;
-        const float wt = fast_exp2(m[c] - mx);
-        L += wt * ld_cluster_f32(cluster_map(smem_u32(share + S::kHeads * D + S::kHeads + head), c));
+        if (l[c] < 0.f) continue;
+        // Weight 0 is no reason to leave a part out: one whose scores are all NaN has no
+        // maximum either, and its sum and O are NaN.
+        const float wt = m[c] == -INFINITY ? 0.f : fast_exp2(m[c] - mx);
+        L += wt * l[c];
         const float4 v = ld_cluster_v4(cluster_map(smem_u32(share + head * D + dim), c));
         O.x += v.x * wt;
         O.y += v.y * wt;

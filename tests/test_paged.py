@@ -437,3 +437,39 @@ def test_decode_of_wide_tables(cuda, dim, heads, kv_heads, lens, window):
             check(first[3 * c:3 * c + 3], want[:, :, 0], bound[:, :, 0])
     for _ in range(5):
         assert torch.equal(_decode(q, k, v, wide, lens, **kw), first)
+
+
+def check_with_nan(got, want, bound):
+    """NaN exactly where the definition has it; the rest within its bound."""
+    odd = want.isnan()
+    assert odd.any() and torch.equal(got.isnan(), odd)
+    check(torch.where(odd, 0, got), torch.where(odd, 0, want), torch.where(odd, 0, bound))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dim,heads,kv_heads,copies,reach", [
+    (128, 4, 1, 1, 1000),   # clusters of 8 CTAs
+    (64, 4, 1, 1, 2100),
+    (64, 20, 2, 1, 2100),
+    (128, 4, 1, 4, 1000),   # of 4
+    (128, 4, 1, 9, 1000),   # of 2
+    (128, 4, 1, 20, 1000),  # one CTA to a unit
+    (64, 4, 1, 1, 80000),   # the line of tiles
+    (128, 4, 1, 20, 80000),
+])
+def test_decode_of_queries_and_keys_that_are_no_numbers(cuda, dim, heads, kv_heads, copies, reach):
+    """NaN in a query, in the newest key alone in its tile (and in its CTA's share), in every key of a
+    tile, in one key among others: the rows that see it are NaN, whoever joins their parts."""
+    lens = [225, 225, 225, 225, 33] * copies
+    k, v, table = paged_cache(lens, kv_heads, dim, 16, seed=dim + copies)
+    wide = torch.full((len(lens), (reach + 15) // 16), -1, dtype=torch.int32)
+    wide[:, :table.shape[1]] = table
+    q = seeded((len(lens), heads, dim), 13)
+    for c in range(0, len(lens), 5):
+        q[c, 1, 5] = NAN
+        for row, keys in ((c + 1, [224]), (c + 2, range(64, 96)), (c + 3, [100])):
+            for j in keys:
+                k[int(wide[row, j // 16]), kv_heads - 1, j % 16, 7] = NAN
+    got = _decode(q, k, v, wide, lens)
+    want, bound = oracle.attention_paged(q[:, :, None], k, v, wide, lens, q_lens=[1] * len(lens))
+    check_with_nan(got, want[:, :, 0], bound[:, :, 0])
