@@ -561,7 +561,8 @@ __global__ void __launch_bounds__(kThreads, 1)
         for (int e = 0; e < D / 4; ++e)
           parts[(tt * (D / 4) + e) * 128 + r] = make_uint4(o[4 * e], o[4 * e + 1], o[4 * e + 2], o[4 * e + 3]);
       }
-      part_ml[tt * 128 + r] = make_float2(m_run, l_run);
+      // Without a tile there is no part: a sum that none has.
+      part_ml[tt * 128 + r] = make_float2(m_run, n_tiles > 0 ? l_run : -1.f);
     } else {
       tc_fence_after();
       const bool any = n_tiles > 0 && l_run != 0.f;
@@ -596,10 +597,14 @@ __global__ void __launch_bounds__(kThreads, 1)
     // CTA `rank` takes its share of the dimensions; parts in the order of the CTAs.
     cluster_sync_all();
     if (warp < 8) {
+      // Weight 0 is no reason to leave a part out: one whose scores are all NaN has no
+      // maximum, one with a NaN among scores far below the others' weighs nothing, and both
+      // have NaN as their sum.
       float w[kMaxSplits], l[kMaxSplits], top = -INFINITY, sum = 0.f;
 #pragma unroll
       for (int c = 0; c < kMaxSplits; ++c) {
         w[c] = -INFINITY;
+        l[c] = -1.f;
         if (c >= p.splits) continue;
         const uint32_t ml = cluster_map(smem_u32(part_ml + tt * 128 + r), c);
         w[c] = ld_cluster_f32(ml);
@@ -609,7 +614,7 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll
       for (int c = 0; c < kMaxSplits; ++c) {
         w[c] = w[c] == -INFINITY ? 0.f : fast_exp2(w[c] - top);
-        if (w[c] != 0.f) sum += w[c] * l[c];
+        if (!(l[c] < 0.f)) sum += w[c] * l[c];
       }
       const float inv = sum != 0.f ? 1.f / sum : 0.f;
       const int each = D / 4 / p.splits;  // groups of four dimensions
@@ -619,7 +624,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         float f[8] = {};
 #pragma unroll
         for (int c = 0; c < kMaxSplits; ++c) {
-          if (c >= p.splits || w[c] == 0.f) continue;
+          if (l[c] < 0.f) continue;
           const uint32_t from = cluster_map(smem_u32(parts + (tt * (D / 4) + q) * 128 + r), c);
           const float4 x = ld_cluster_v4(from), y = ld_cluster_v4(from + 128 * 16);
           f[0] += w[c] * x.x, f[1] += w[c] * x.y, f[2] += w[c] * x.z, f[3] += w[c] * x.w;

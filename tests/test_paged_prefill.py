@@ -7,7 +7,7 @@ import torch
 
 import oracle
 from conftest import seeded
-from test_paged import INF, NAN, check, ints, paged_cache
+from test_paged import INF, NAN, check, check_with_nan, ints, paged_cache
 
 
 def _prefill(q, k, v, table, lens, q_lens=None, **kw):
@@ -283,3 +283,34 @@ def test_captured_and_overlapping_calls(cuda):
     torch.cuda.synchronize()
     assert _native.device_status() == 0
     assert all(torch.equal(g, w) for gs, w in zip(got, want) for g in gs)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("copies", [1, 4, 9, 20])
+@pytest.mark.parametrize("dim,queries", [(64, 3), (128, 3), (128, 40), (64, 200)])
+def test_queries_and_keys_that_are_no_numbers(cuda, dim, queries, copies):
+    """NaN in a query, in the newest key alone in its tile (and in its CTA's share), in every key of a
+    tile, in one key of a tile whose other keys weigh nothing: the rows that see it are NaN, whether
+    clusters of 8, 4 or 2 CTAs join their parts or one CTA has them all."""
+    lens = [897, 897, 897, 897] * copies
+    k, v, table = paged_cache(lens, 1, dim, 16, seed=dim + queries)
+    q = seeded((len(lens), 2, queries, dim), 14)
+
+    def key(row, j):
+        return k[int(table[row, j // 16]), 0, j % 16]
+
+    for c in range(0, len(lens), 4):
+        q[c, 1, queries // 2, 5] = NAN
+        key(c + 1, 896)[7] = NAN
+        for j in range(256, 384):
+            key(c + 2, j)[0] = NAN
+            key(c + 3, j)[:] = -30
+        q[c + 3] = q[c + 3].abs() + 1  # the scores of tile 2 lie 240 and more below the others
+        key(c + 3, 300)[9] = NAN
+    got = _prefill(q, k, v, table, lens, [queries] * len(lens))
+    want, bound = oracle.attention_paged(q[:4], k, v, table[:4], lens[:4], [queries] * 4)
+    for c in range(0, len(lens), 4):
+        if c:  # the same tokens, other pages and values: only where NaN is
+            assert torch.equal(got[c:c + 4].isnan(), want.isnan())
+        else:
+            check_with_nan(got[:4], want, bound)
