@@ -60,7 +60,7 @@ __device__ __forceinline__ int warps_before(const int* s_warp) {
 }
 
 // Every CTA's `mine` into s_all[kCtas] of every CTA (needs a cluster barrier
-// before it is read).
+// before it is read, and one before the kernel's first call: all CTAs have started).
 __device__ __forceinline__ void cluster_share(int mine, int* s_all) {
   if (threadIdx.x < kCtas) {
     const uint32_t to = cluster_map(smem_u32(s_all + cluster_ctarank()), threadIdx.x);
@@ -300,11 +300,13 @@ __global__ void __launch_bounds__(kThreads) page_compact_kernel(const CompactPar
   const int rank = static_cast<int>(cluster_ctarank());
   const int all_threads = kCtas * kThreads, me = rank * kThreads + tid;
   pdl_launch_dependents();
+  cluster_arrive();  // a CTA's shared memory may be written once it has started
   pdl_wait();
   const Stretch pages(p.num_pages);
 
   int mine = 0;
   for (int i = pages.begin + lane; i < pages.end; i += 32) mine += p.refs[i] > 0;
+  cluster_wait();
   cluster_share(block_sum(__reduce_add_sync(0xffffffffu, mine), s_warp), s_live);
   cluster_sync_all();
   int at = 0, n = 0;  // live pages before this warp's, and all

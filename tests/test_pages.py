@@ -63,6 +63,18 @@ def test_oracle_pages_to_copy_from_are_not_handed_out():
     assert refs == [0, 0, 1, 1, 1, 1, 0] and info == [3, 0, 4]
 
 
+def test_clusters_have_started_before_their_shared_memory_is_written():
+    """By reading: a CTA of a cluster may start after another has counted, so each kernel passes a
+    cluster barrier before its first write to the others."""
+    from llm_compiler_3_b200 import build
+    kernels = (build.CSRC / "pages.cu").read_text().split("__global__")[1:]
+    writes = [k for k in kernels if "cluster_share(" in k]
+    assert len(writes) == 2
+    for k in writes:
+        before = k[:k.index("cluster_share(")]
+        assert "cluster_wait();" in before or "cluster_sync_all();" in before
+
+
 @pytest.mark.parametrize("change,message", [
     (dict(rows=0), "0 rows"), (dict(rows=8193), "8193 rows"), (dict(new_rows=0), "to 0"),
     (dict(new_rows=8193), "to 8193"), (dict(entries=0), "0 table entries"), (dict(page=12), "page_size 12"),
@@ -277,3 +289,26 @@ def test_update_and_copy_in_a_graph(cuda):
         for g, w in zip(got, want):
             assert g.cpu().tolist() == w
         assert torch.equal(pool.cpu(), oracle.page_copy(before, want[3], want[4][2]))
+
+
+@pytest.mark.gpu
+def test_compactions_beside_other_work(cuda):
+    """Many compactions in a row while another stream keeps the SMs busy, so that a cluster's CTAs
+    start apart: the same results each time."""
+    from llm_compiler_3_b200 import ops
+    r = random.Random(9)
+    refs = [r.choice([0, 0, 1, 2]) for _ in range(3000)]
+    table = [[r.randint(-1, 2999) for _ in range(40)] for _ in range(20)]
+    state = ints(table).cuda(), ints(refs).cuda()
+    pool = torch.zeros(2, 4000, 8192, dtype=torch.float16, device="cuda")
+    pages = torch.stack([torch.arange(2000), torch.arange(2000, 4000)]).int().cuda()
+    busy, got = torch.cuda.Stream(), []
+    torch.cuda.synchronize()
+    for _ in range(50):
+        with torch.cuda.stream(busy):
+            ops.page_copy(pool, pages)
+        got.append(ops.page_compact(*state))
+    torch.cuda.synchronize()
+    want = [ints(w) for w in oracle.page_compact(table, refs)]
+    for g in got:
+        assert all(torch.equal(x.cpu(), w) for x, w in zip(g, want))
