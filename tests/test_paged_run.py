@@ -117,3 +117,58 @@ def test_beam_search_over_a_paged_cache(cuda, window, sinks, seed):
     _, _, refs, _, info = ops.page_update(table, lens, ints([-1]).to(dev), ints([0]).to(dev), refs, PAGE)
     assert info.tolist() == [pool_pages, 0, 0] and torch.count_nonzero(refs) == 0
     assert _native.device_status() == 0
+
+
+@pytest.mark.gpu
+def test_the_documented_step_with_beams_that_end(cuda):
+    """The README's step, run as it stands, where most tokens are banned: beams without a
+    continuation take no pages, write no rows and give zeros, and their places fill again."""
+    import re
+    from conftest import ROOT
+    from llm_compiler_3_b200 import _native
+    blocks = re.findall(r"```python\n(.*?)```", (ROOT / "README.md").read_text(), re.S)
+    step, = [b for b in blocks if "ops.page_update(" in b]
+    batch, width, kv, page, pages, entries, vocab = 3, 2, 2, 8, 50, 45, 40
+    dev = torch.device("cuda", 0)
+    lens, at = [9, 9, 20, 20, 300, 300], 0
+    table, refs = torch.full((batch * width, entries), -1, dtype=torch.int32), torch.zeros(pages, dtype=torch.int32)
+    for row in range(0, batch * width, 2):  # both beams of a sequence share their full pages
+        full, held = lens[row] // page, -(-lens[row] // page)
+        for r in (row, row + 1):
+            table[r, :full] = torch.arange(at, at + full)
+        at += full
+        for r in (row, row + 1):
+            table[r, full:held] = torch.arange(at, at + held - full)
+            at += held - full
+        refs += torch.bincount(table[row:row + 2][table[row:row + 2] >= 0].long(), minlength=pages).int()
+    pool = seeded((2, pages, kv, page, 128), 1).to(dev)
+    state = dict(pool=pool, table=table.to(dev), lens=ints(lens).to(dev), refs=refs.to(dev), page_size=page, eos=3,
+                 width=width, layers=1, scores=torch.zeros(batch, width, device=dev),
+                 done=torch.zeros(batch, width, dtype=torch.bool, device=dev))
+    # Sequence 0 has one continuation left, sequence 1 none (for good); then two for sequence 0.
+    want_lens = ([10, 0, 0, 0, 301, 301], [11, 11, 0, 0, 302, 302])
+    for n, wanted in enumerate(want_lens):
+        logits = seeded((batch, width, vocab), 10 + n).float()
+        logits[0] = -float("inf")
+        logits[0, 0, 5:6 + n] = 1.0
+        if n == 0:
+            logits[1] = -float("inf")
+        state.update(logits=logits.to(dev), q=seeded((batch * width, 4, 128), 20 + n).to(dev),
+                     k=seeded((batch * width, kv, 1, 128), 30 + n).to(dev),
+                     v=seeded((batch * width, kv, 1, 128), 40 + n).to(dev))
+        before = state["logits"].cpu(), state["scores"].cpu(), width, state["done"].cpu(), 3
+        exec(step, state)
+        assert _native.device_status() == 0
+        want = oracle.beam_select(*before)
+        assert state["parents"].tolist() == want[2].tolist() and state["tokens"].tolist() == want[1].tolist()
+        assert state["lens"].tolist() == wanted and state["info"].tolist()[1] == 0
+        rows = state["table"].cpu()
+        assert [int((row >= 0).sum()) for row in rows] == [-(-x // page) for x in wanted]
+        assert torch.equal(torch.bincount(rows[rows >= 0].long(), minlength=pages).int(), state["refs"].cpu())
+        for r, x in enumerate(wanted):  # the new key stands where the row ends
+            if x:
+                held = pool[0, int(rows[r, (x - 1) // page]), :, (x - 1) % page]
+                assert torch.equal(held, state["k"][r, :, 0])
+        out, bound = oracle.attention_paged(state["q"].cpu()[:, :, None], pool[0].cpu(), pool[1].cpu(), rows, wanted,
+                                            [min(1, x) for x in wanted], window=4096, sinks=4)
+        check(state["out"].cpu(), out[:, :, 0], bound[:, :, 0])
