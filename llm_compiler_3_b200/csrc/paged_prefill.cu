@@ -29,6 +29,7 @@
 // P_t(j) V, cannot overwrite weights that are still read, and its completion says
 // that O_t is up to date.  A row's maximum moves, and its O row is rescaled, only
 // when a tile's exceeds it by 2^8: weights stay below 256, exact enough in FP16.
+#include <limits.h>
 #include <math.h>
 
 #include <algorithm>
@@ -67,7 +68,7 @@ struct PpShape {
 constexpr int kS = 0, kO = 2 * KT;  // TMEM columns; O_t at kO + t D
 
 struct PpParams {
-  const __half *q, *k_pages, *v_pages;  // for single rows: tiles come through the tensor maps
+  const __half* v_pages;  // for values that are no numbers: tiles come through the tensor maps
   const int32_t* table;
   const int32_t* seq_lens;
   const int32_t* q_lens;  // or null: every query
@@ -110,76 +111,84 @@ __device__ __forceinline__ uint32_t first_bits(int n) {
 struct Span {
   int seq_len, q_len, first_pos;  // first_pos: position of query 0 of the chunk
   int lo, len, s;                 // keys that some of the CTA's queries see: [0, s) and [lo, len)
+  int all_lo, all_len, sinks;     // that all at a position see: [0, sinks) and [all_lo, all_len)
   TileRange<kUnit> units;
   __device__ __forceinline__ bool sees(int j) const { return j < len && (j >= lo || j < s); }
   __device__ __forceinline__ bool sees_any(int j, int n) const { return j < len && (j + n > lo || j < s); }
-  __device__ __forceinline__ bool sees_all(int j, int n) const {
-    return j + n <= len && (j >= lo || j + n <= s);
+  __device__ __forceinline__ bool seen_by_all(int j, int n) const {  // each key of [j, j + n)
+    return j + n <= all_len && (j >= all_lo || j + n <= sinks);
   }
 };
 
-// Dimensions [d0, d1) of row `at` of out once more, by one warp and over the keys that it
-// sees alone: [0, s) and [lo, last].  Tiles give a key that a row does not see the weight 0, but
-// 0 x inf is NaN: where a later token's value is infinite or NaN, rows of its tile
-// before it come out as NaN, and only then are they done again.
-template <int D>
-__device__ __noinline__ void row_alone(const PpParams& p, int b, int hk, long long at, int last, int lo,
-                                       int d0, int d1) {
-  const int lane = threadIdx.x & 31, s = min(p.sinks, lo);
-  const int keys = last < 0 ? 0 : s + last + 1 - lo;
-  const uint4* q = reinterpret_cast<const uint4*>(p.q + at * D);
-  const float scale = p.negate ? -p.scale_log2 : p.scale_log2;
-  float m = -INFINITY, l = 0.f, o[D / 32] = {};
-  for (int x0 = 0; x0 < keys; x0 += 32) {
-    // Scores of 32 keys, one to a lane.
-    const int x = x0 + lane, j = x < s ? x : lo + x - s;
-    long long row = -1;  // of the pool
-    float score = -INFINITY;
-    if (x < keys) {
-      const int page = p.table[static_cast<size_t>(b) * p.entries + j / p.page_size];
-      if (page >= 0 && page < p.num_pages) row = (page * p.kv_heads + hk) * p.page_size + j % p.page_size;
-      score = 0.f;
-      if (row >= 0) {
-        const uint4* k = reinterpret_cast<const uint4*>(p.k_pages + row * D);
-        for (int c = 0; c < D / 8; ++c) {
-          const uint4 qw = q[c], kw = k[c];
-          const uint32_t qu[4] = {qw.x, qw.y, qw.z, qw.w}, ku[4] = {kw.x, kw.y, kw.z, kw.w};
+// Whether one of 8 numbers is infinite or NaN: times 0 they are NaN, all others 0.
+__device__ __forceinline__ __half2 times_zero(const uint4& w, __half2 sum) {
+  const uint32_t u[4] = {w.x, w.y, w.z, w.w};
 #pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            const float2 a = __half22float2(*reinterpret_cast<const __half2*>(&qu[e]));
-            const float2 d = __half22float2(*reinterpret_cast<const __half2*>(&ku[e]));
-            score += a.x * d.x + a.y * d.y;
-          }
+  for (int i = 0; i < 4; ++i)
+    sum = __hfma2(*reinterpret_cast<const __half2*>(&u[i]), __half2half2(__ushort_as_half(0)), sum);
+  return sum;
+}
+__device__ __forceinline__ bool is_odd(__half2 sum) {
+  return (*reinterpret_cast<const uint32_t*>(&sum) & 0x7c007c00u) != 0;
+}
+// Infinite and NaN numbers become 0.
+__device__ __forceinline__ uint4 without_odd(const uint4& w) {
+  uint32_t u[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const uint32_t low = (u[i] & 0x7c00u) == 0x7c00u ? 0xffffu : 0u;
+    const uint32_t high = (u[i] & 0x7c000000u) == 0x7c000000u ? 0xffff0000u : 0u;
+    u[i] &= ~(low | high);
+  }
+  return make_uint4(u[0], u[1], u[2], u[3]);
+}
+
+// The infinite and NaN values that tiles went without (warp 10), onto dimensions [d0, d1) of
+// the rows of out that see them: any weight of such a value is that value.  One warp walks the
+// keys [first, first + keys), its lanes over the dimensions, each with the places of the newest
+// such values; lane r's row `at` sees the keys up to its turn's (none: a negative turn) from `lo`
+// on, and the sinks.
+template <int D>
+__device__ __noinline__ void add_odd_values(const PpParams& p, int b, int hk, long long at, int turn, int lo,
+                                            int first, int keys, int d0, int d1) {
+  const int lane = threadIdx.x & 31;
+  int nan[D / 32], high[D / 32], low[D / 32];
+#pragma unroll
+  for (int e = 0; e < D / 32; ++e) nan[e] = high[e] = low[e] = -1;
+  __syncwarp();  // each lane has written its row
+  for (int k0 = 0; k0 < keys; k0 += 32) {
+    long long row = -1;  // of the pool
+    if (k0 + lane < keys) {
+      const int j = first + k0 + lane, page = p.table[static_cast<size_t>(b) * p.entries + j / p.page_size];
+      if (page >= 0 && page < p.num_pages) row = (page * p.kv_heads + hk) * p.page_size + j % p.page_size;
+    }
+#pragma unroll 4
+    for (int k = 0; k < 32; ++k) {
+      const long long from = __shfl_sync(0xffffffffu, row, k);
+      if (from >= 0) {
+        const int j = first + k0 + k < p.sinks ? INT_MAX : first + k0 + k;
+        const __half* v = p.v_pages + from * D + lane * (D / 32);
+#pragma unroll
+        for (int e = 0; e < D / 32; ++e) {
+          const float x = __half2float(v[e]);
+          if (isnan(x)) nan[e] = max(nan[e], j);
+          if (x == INFINITY) high[e] = max(high[e], j);
+          if (x == -INFINITY) low[e] = max(low[e], j);
         }
       }
-      score *= scale;
+      for (unsigned todo = __ballot_sync(0xffffffffu, turn == k0 + k); todo != 0; todo &= todo - 1) {
+        const int r = __ffs(todo) - 1, from_r = __shfl_sync(0xffffffffu, lo, r);
+        __half* out = p.out + __shfl_sync(0xffffffffu, at, r) * D;
+#pragma unroll
+        for (int e = 0; e < D / 32; ++e) {
+          const int d = lane * (D / 32) + e;
+          if (d < d0 || d >= d1 || max(nan[e], max(high[e], low[e])) < from_r) continue;
+          const float x = (nan[e] >= from_r ? NAN : 0.f) + (high[e] >= from_r ? INFINITY : 0.f) +
+                          (low[e] >= from_r ? -INFINITY : 0.f);
+          out[d] = __float2half_rn(__half2float(out[d]) + x);
+        }
+      }
     }
-    float top = fmaxf(score, m);
-#pragma unroll
-    for (int w = 16; w > 0; w >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, w));
-    const float alpha = m == -INFINITY ? 0.f : fast_exp2(m - top);
-    m = top;
-    const float weight = fast_exp2(score - (m == -INFINITY ? 0.f : m));
-    l = l * alpha + weight;
-#pragma unroll
-    for (int e = 0; e < D / 32; ++e) o[e] *= alpha;
-    // Each lane sums D / 32 of the values' dimensions.
-    for (int k = 0; k < min(32, keys - x0); ++k) {
-      const float w = __shfl_sync(0xffffffffu, weight, k);
-      const long long from = __shfl_sync(0xffffffffu, row, k);
-      if (from < 0) continue;
-      const __half* v = p.v_pages + from * D + lane * (D / 32);
-#pragma unroll
-      for (int e = 0; e < D / 32; ++e) o[e] += w * __half2float(v[e]);
-    }
-  }
-#pragma unroll
-  for (int w = 16; w > 0; w >>= 1) l += __shfl_xor_sync(0xffffffffu, l, w);
-  const float inv = l == 0.f ? 0.f : 1.f / l;
-#pragma unroll
-  for (int e = 0; e < D / 32; ++e) {
-    const int d = lane * (D / 32) + e;
-    if (d >= d0 && d < d1) p.out[at * D + d] = __float2half_rn(o[e] * inv);
   }
 }
 
@@ -205,6 +214,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   uint64_t* drain = o_done + 2;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(drain + 1);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+  uint32_t* odd_values = tmem_slot + 2;  // tiles went without some of V's (add_odd_values)
   // Over the ring at the end: O of a CTA that has a share of the keys, [tile][D / 4][row], and
   // its rows' maxima and sums.
   uint4* parts = reinterpret_cast<uint4*>(smem + S::kRing);
@@ -234,6 +244,9 @@ __global__ void __launch_bounds__(kThreads, 1)
     span.len = m_hi > m_lo ? max(0, span.first_pos + m_hi) : 0;
     span.lo = p.window > 0 ? max(0, first - p.window + 1) : 0;
     span.s = min(p.sinks, span.lo);
+    span.all_lo = p.window > 0 ? max(0, span.len - p.window) : 0;
+    span.all_len = first + 1;
+    span.sinks = p.sinks;
     span.units.set(span.lo, span.len, p.sinks);
     if (span.len == 0) span.units.n = 0;
   }
@@ -241,14 +254,14 @@ __global__ void __launch_bounds__(kThreads, 1)
   const long long n_all = (span.units.n + KT / kUnit - 1) / (KT / kUnit);
   const int tile0 = static_cast<int>(n_all * rank / p.splits);
   const int n_tiles = static_cast<int>(n_all * (rank + 1) / p.splits) - tile0;
-  // The key of row `row` of tile j (past the last unit: a hidden one), and whether some query
-  // sees each key of the tile.
+  // The key of row `row` of tile j (past the last unit: a hidden one), and whether all queries
+  // see each key of the tile.
   auto key_of = [&](int j, int row) {
     return span.units.key0((tile0 + j) * (KT / kUnit) + row / kUnit) + row % kUnit;
   };
   auto whole = [&](int j) {
     bool all = true;
-    for (int row = 0; row < KT; row += kUnit) all = all && span.sees_all(key_of(j, row), kUnit);
+    for (int row = 0; row < KT; row += kUnit) all = all && span.seen_by_all(key_of(j, row), kUnit);
     return all;
   };
 
@@ -276,6 +289,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
     mbar_init(drain, 1);
     *abort_flag = 0;
+    *odd_values = 0;
     fence_barrier_init();
   }
   if (warp == 9) {
@@ -300,14 +314,12 @@ __global__ void __launch_bounds__(kThreads, 1)
   // Keys of this row: j <= last and (j >= lo or j < sinks).
   const int last = row_ok && m0 + i < span.q_len ? span.first_pos + m0 + i : -1;
   const int lo = p.window > 0 ? max(0, last - p.window + 1) : 0;
-  // Rows that came out as NaN, by the whole warp; dimensions [d0, d1).
-  auto redo = [&](bool odd, int d0, int d1) {
-    __syncwarp();
-    for (unsigned todo = __ballot_sync(0xffffffffu, odd); todo != 0; todo &= todo - 1) {
-      const int from = __ffs(todo) - 1;
-      row_alone<D>(p, b, hk, __shfl_sync(0xffffffffu, at, from), __shfl_sync(0xffffffffu, last, from),
-                   __shfl_sync(0xffffffffu, lo, from), d0, d1);
-    }
+  // The keys that some queries see and others do not: those before the last one's window, and
+  // those after the first query.
+  auto add_odd = [&](int d0, int d1) {
+    const int from = max(span.lo, p.sinks), keys = min(span.all_lo, span.all_len) - from;
+    add_odd_values<D>(p, b, hk, at, last >= 0 ? keys - 1 : -1, lo, from, keys, d0, d1);
+    add_odd_values<D>(p, b, hk, at, last - span.all_len, lo, span.all_len, span.len - span.all_len, d0, d1);
   };
 
   if (warp == 8) {
@@ -442,20 +454,34 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
   } else if (warp == 10) {
     // ---------------- hidden rows of V ----------------
-    // Rows that no query here sees may hold anything; their weights are 0, but
-    // 0 * NaN is NaN.
+    // Rows that a query does not see may hold anything; its weights for them are 0, but 0 x inf
+    // and 0 x NaN are NaN.  Rows that no query here sees are cleared; what is infinite or NaN in
+    // rows that some see is, and comes back in add_odd_values.
     uint32_t raw_uses = 0;  // bit s: raw[s] was used an odd number of times
     for (int j = 0; j < n_tiles; ++j) {
       const int s = (2 * j + 1) % kStages;
       if (whole(j)) continue;
       if (!__all_sync(0xffffffffu, wait_or_abort(&raw[s], raw_uses >> s & 1, abort_flag))) break;
       raw_uses ^= 1u << s;
-      for (int r = lane; r < KT; r += 32)
-        if (!span.sees(key_of(j, r)))
-          for (int a = 0; a < S::kRegions; ++a)
-            for (int c = 0; c < 128; c += 16)
-              *reinterpret_cast<uint4*>(smem + S::kRing + s * S::kTileBytes + a * S::kRegion +
-                                        r * 128 + c) = make_uint4(0, 0, 0, 0);
+      for (int r = lane; r < KT; r += 32) {
+        const int key = key_of(j, r);
+        if (span.seen_by_all(key, 1)) continue;
+        uint8_t* row = smem + S::kRing + s * S::kTileBytes + r * 128;
+        auto chunk = [&](int x) {  // each lane begins at banks of its own
+          return reinterpret_cast<uint4*>(row + (x >> 3) * S::kRegion + ((x + lane) & 7) * 16);
+        };
+        if (!span.sees(key)) {
+          for (int x = 0; x < D / 8; ++x) *chunk(x) = make_uint4(0, 0, 0, 0);
+          continue;
+        }
+        __half2 sum = __half2half2(__ushort_as_half(0));
+#pragma unroll
+        for (int x = 0; x < D / 8; ++x) sum = times_zero(*chunk(x), sum);
+        if (is_odd(sum)) {
+          for (int x = 0; x < D / 8; ++x) *chunk(x) = without_odd(*chunk(x));
+          *odd_values = 1;
+        }
+      }
       fence_proxy_async_smem();
       __syncwarp();
       if (lane == 0) mbar_arrive(&full[s]);
@@ -568,7 +594,6 @@ __global__ void __launch_bounds__(kThreads, 1)
       const bool any = n_tiles > 0 && l_run != 0.f;
       const float inv = any ? 1.f / l_run : 0.f;
       uint4* row = reinterpret_cast<uint4*>(p.out + at * D);
-      bool odd = false;  // not a number
       uint32_t o[D];
       if (n_tiles > 0) {
 #pragma unroll
@@ -580,15 +605,12 @@ __global__ void __launch_bounds__(kThreads, 1)
         for (int c = 0; c < D; c += 8) {
           float f[8];
 #pragma unroll
-          for (int e = 0; e < 8; ++e) {
-            f[e] = any ? __uint_as_float(o[c + e]) * inv : 0.f;
-            odd |= f[e] != f[e];
-          }
+          for (int e = 0; e < 8; ++e) f[e] = any ? __uint_as_float(o[c + e]) * inv : 0.f;
           row[c / 8] = make_uint4(pack_half2(f[0], f[1]), pack_half2(f[2], f[3]), pack_half2(f[4], f[5]),
                                   pack_half2(f[6], f[7]));
         }
       }
-      redo(odd, 0, D);
+      if (n_tiles > 0 && *odd_values != 0) add_odd(0, D);
     }
   }
 
@@ -618,7 +640,6 @@ __global__ void __launch_bounds__(kThreads, 1)
       }
       const float inv = sum != 0.f ? 1.f / sum : 0.f;
       const int each = D / 4 / p.splits;  // groups of four dimensions
-      bool odd = false;
 #pragma unroll 1
       for (int q = rank * each; q < (rank + 1) * each; q += 2) {
         float f[8] = {};
@@ -632,14 +653,14 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
         if (!row_ok) continue;
 #pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          f[e] *= inv;
-          odd |= f[e] != f[e];
-        }
+        for (int e = 0; e < 8; ++e) f[e] = sum != 0.f ? f[e] * inv : 0.f;
         *reinterpret_cast<uint4*>(p.out + at * D + q * 4) = make_uint4(
             pack_half2(f[0], f[1]), pack_half2(f[2], f[3]), pack_half2(f[4], f[5]), pack_half2(f[6], f[7]));
       }
-      redo(odd, rank * each * 4, (rank + 1) * each * 4);
+      bool odd = false;
+      for (int c = 0; c < p.splits; ++c)
+        odd |= __float_as_uint(ld_cluster_f32(cluster_map(smem_u32(odd_values), c))) != 0;
+      if (odd) add_odd(rank * each * 4, (rank + 1) * each * 4);
     }
     cluster_sync_all();  // nobody reads this CTA's parts any more
   }
@@ -709,8 +730,6 @@ extern "C" int npu_b200_paged_prefill(const void* d_q, const void* d_k_pages, co
   NPU_REQUIRE(aligned16(d_q) && aligned16(d_k_pages) && aligned16(d_v_pages) && aligned16(d_out),
               "paged_prefill: q, pages and out must be 16-byte aligned");
   PpParams p;
-  p.q = static_cast<const __half*>(d_q);
-  p.k_pages = static_cast<const __half*>(d_k_pages);
   p.v_pages = static_cast<const __half*>(d_v_pages);
   p.table = d_page_table;
   p.seq_lens = d_seq_lens;

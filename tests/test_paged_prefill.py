@@ -314,3 +314,65 @@ def test_queries_and_keys_that_are_no_numbers(cuda, dim, queries, copies):
             assert torch.equal(got[c:c + 4].isnan(), want.isnan())
         else:
             check_with_nan(got[:4], want, bound)
+
+
+@pytest.mark.gpu
+def test_numbers_that_are_none_cost_no_second_pass(cuda):
+    """A prompt with NaN in all queries, in one key, in one early or late value or in all values
+    takes about what it takes without (rows done again one by one took 400 times as long)."""
+    from llm_compiler_3_b200 import ops
+    n = 2048
+    k, v, table = paged_cache([n], 2, 128, 64, seed=3)
+    q = seeded((1, 8, n, 128), 5)
+
+    def took(q, k, v):
+        state = [t.cuda() for t in (q, k, v, table, ints([n]))]
+        ops.paged_prefill(*state)
+        times = []
+        for _ in range(5):
+            start, end = (torch.cuda.Event(enable_timing=True) for _ in range(2))
+            start.record()
+            ops.paged_prefill(*state)
+            end.record()
+            end.synchronize()
+            times.append(start.elapsed_time(end))
+        return sorted(times)[2]
+
+    bad_q, bad_k, bad_v, late_v, all_v = q.clone(), k.clone(), v.clone(), v.clone(), v.clone()
+    bad_q[..., 3] = NAN
+    bad_k[int(table[0, 0]), :, 0, 3] = NAN
+    bad_v[int(table[0, 0]), :, 0, 3] = NAN
+    late_v[int(table[0, -1]), :, 40] = NAN
+    all_v[:, :, :, 3] = NAN
+    plain = took(q, k, v)
+    for case in ((bad_q, k, v), (q, bad_k, v), (q, k, bad_v), (q, k, late_v), (q, k, all_v)):
+        assert took(*case) < 4 * plain + 0.1, (took(*case), plain)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("heads,dim,window,sinks", [(2, 64, 0, 0), (8, 128, 0, 0), (2, 128, 100, 0), (8, 64, 300, 9),
+                                                    (1, 64, 40, 600), (4, 128, 1, 0), (4, 64, 64, 32)])
+@pytest.mark.parametrize("batch,queries", [(1, 7), (3, 70), (16, 150), (2, 333)])
+def test_values_that_are_no_numbers_behind_long_prefixes(cuda, heads, dim, window, sinks, batch, queries):
+    """The same where clusters share the keys and where one CTA has them: single tokens with infinite
+    or NaN values in the prefix, in the chunk, beside one another in one dimension; chunks that are
+    shorter than the call's."""
+    lens, q_lens = ([900, 450, 641, 70] * 4)[:batch], [queries, 65, 1, 70] * 4
+    q_lens = [min(a, b, queries) for a, b in zip(lens, q_lens)]
+    k, v, table = paged_cache(lens, 1, dim, 16, seed=dim + window)
+    for b, (n, m) in enumerate(zip(lens, q_lens)):
+        for j, d, x in ((n - 1, 0, NAN), (n - m, 9, INF), (n - m + 3, 9, -INF), (n - m + 5, 17, INF), (n // 2, 33, -INF),
+                        (n - 40, 63, NAN), (max(0, n - m - 20), 40, INF), (3, 41, NAN)):
+            if 0 <= j < n:
+                v[int(table[b, j // 16]), :, j % 16, d] = x
+    q = seeded((batch, heads, queries, dim), 6)
+    got = _prefill(q, k, v, table, lens, q_lens, window=window, sinks=sinks)
+    rows = slice(0, 3)  # of 64 bits; the others are as many more of the same
+    args = (q[rows], k, v, table[rows], lens[rows], q_lens[rows])
+    want = oracle.attention_paged(*args, window=window, sinks=sinks)[0]
+    odd = ~want.isfinite()
+    some = got[rows].double()
+    assert odd.any() and torch.equal(some.nan_to_num(1e9, 2e9, 3e9)[odd], want.nan_to_num(1e9, 2e9, 3e9)[odd])
+    args = (q[rows], k, v.nan_to_num(0, 0, 0), *args[3:])
+    want, bound = oracle.attention_paged(*args, window=window, sinks=sinks)
+    check(torch.where(odd, want.half(), got[rows]), want, torch.where(odd, want.abs(), bound))
