@@ -536,15 +536,16 @@ __global__ void __launch_bounds__(PdShape<D, NB>::kThreads, 1)
     for (int x = rank * S::kThreads + threadIdx.x; x < heads * D / 4; x += p.shares * S::kThreads) {
       const int head = x * 4 / D, dim = x * 4 - head * D;
       float m[kMaxShares], l[kMaxShares], mx = -INFINITY, L = 0.f;
-      float4 O = make_float4(0.f, 0.f, 0.f, 0.f);
+      float4 v[kMaxShares], O = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
-      for (int c = 0; c < kMaxShares; ++c) {
+      for (int c = 0; c < kMaxShares; ++c) {  // all loads in flight together
         m[c] = -INFINITY;
         l[c] = -1.f;
         if (c >= p.shares) continue;
         const uint32_t ml = cluster_map(smem_u32(share + S::kHeads * D + head), c);
         m[c] = ld_cluster_f32(ml);
         l[c] = ld_cluster_f32(ml + S::kHeads * 4);
+        v[c] = ld_cluster_v4(cluster_map(smem_u32(share + head * D + dim), c));
         mx = fmaxf(mx, m[c]);
       }
 #pragma unroll
@@ -554,11 +555,10 @@ __global__ void __launch_bounds__(PdShape<D, NB>::kThreads, 1)
         // maximum either, and its sum and O are NaN.
         const float wt = m[c] == -INFINITY ? 0.f : fast_exp2(m[c] - mx);
         L += wt * l[c];
-        const float4 v = ld_cluster_v4(cluster_map(smem_u32(share + head * D + dim), c));
-        O.x += v.x * wt;
-        O.y += v.y * wt;
-        O.z += v.z * wt;
-        O.w += v.w * wt;
+        O.x += v[c].x * wt;
+        O.y += v[c].y * wt;
+        O.z += v[c].z * wt;
+        O.w += v[c].w * wt;
       }
       const float inv = L == 0.f ? 0.f : 1.f / L;
       *reinterpret_cast<uint2*>(p.out + (q_row + head) * D + dim) =
