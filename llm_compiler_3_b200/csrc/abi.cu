@@ -36,16 +36,14 @@ int check_cuda(cudaError_t e, const char* what) {
 }
 
 int sm_count() {
-  static int cached[64] = {0};
+  static AskedOnce asked[64];
   int dev = 0;
   if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return 148;
-  if (cached[dev] == 0) {
+  return asked[dev].get([&] {
     int n = 0;
-    if (cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess || n <= 0)
-      n = 148;
-    cached[dev] = n;
-  }
-  return cached[dev];
+    const bool ok = cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev) == cudaSuccess;
+    return ok && n > 0 ? n : 148;
+  });
 }
 
 namespace {

@@ -5,6 +5,7 @@
 #include <cuda_runtime.h>
 #include <stdint.h>
 
+#include <atomic>
 #include <string>
 
 #include "../../include/npu_b200.h"
@@ -95,14 +96,30 @@ int launch(const LaunchCfg& c, void (*kernel)(KArgs...), Args&&... args) {
                     "cudaLaunchKernelEx");
 }
 
+// A number that one device answers the same to every asker (not 0), kept from its first answer on;
+// host threads may ask at once.  A question that failed (0) is asked again by the next call.
+class AskedOnce {
+ public:
+  template <typename Ask>
+  int get(Ask ask) {
+    int n = answer_.load(std::memory_order_relaxed);
+    if (n == 0 && (n = ask()) != 0) answer_.store(n, std::memory_order_relaxed);
+    return n;
+  }
+
+ private:
+  std::atomic<int> answer_{0};
+};
+
 // How many clusters of `size` CTAs (2, 4 or 8; `size` 1: CTAs) of KERNEL run at once on the
-// current device, asked once: clusters of 8 that fill an SM each leave 28 of 148 SMs idle.
+// current device: clusters of 8 that fill an SM each leave 28 of 148 SMs idle.  None, if that
+// cannot be told.
 template <auto KERNEL>
 int clusters_at_once(int size, dim3 block, size_t smem) {
-  static int cached[64][9] = {};
+  static AskedOnce asked[64][9];
   int dev = 0;
   if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64 || size > 8) return 0;
-  if (cached[dev][size] == 0) {
+  const int n = asked[dev][size].get([&] {
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(size);
     cfg.blockDim = block;
@@ -113,14 +130,14 @@ int clusters_at_once(int size, dim3 block, size_t smem) {
     attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
     cfg.attrs = &attr;
     cfg.numAttrs = 1;
-    int n = 0;
-    if (cudaOccupancyMaxActiveClusters(&n, KERNEL, &cfg) != cudaSuccess) {
+    int clusters = 0;
+    if (cudaOccupancyMaxActiveClusters(&clusters, KERNEL, &cfg) != cudaSuccess) {
       cudaGetLastError();
-      n = 0;
+      return 0;
     }
-    cached[dev][size] = n > 0 ? n : -1;
-  }
-  return cached[dev][size];
+    return clusters > 0 ? clusters : -1;
+  });
+  return n > 0 ? n : 0;
 }
 
 }  // namespace npu_b200

@@ -73,3 +73,41 @@ def test_flash_decode_split_choice(batch, kv_heads, keys, splits):
     per_split = batch * kv_heads * (8 * 128 + 16) * 4
     assert (size - 16384 * 4) % per_split == 0
     assert (size - 16384 * 4) // per_split == splits
+
+
+def test_answers_kept_for_all_host_threads(tmp_path):
+    """AskedOnce (csrc/host.hpp), which keeps the SM count and the cluster counts: threads that ask at
+    once get the answer, and a question that failed is asked again."""
+    from llm_compiler_3_b200 import build
+    source = tmp_path / "asked.cpp"
+    source.write_text("""
+#include "host.hpp"
+#include <thread>
+#include <vector>
+int main() {
+  npu_b200::AskedOnce once;
+  int asked = 0;
+  if (once.get([&] { ++asked; return 0; }) != 0) return 1;   // failed
+  if (once.get([&] { ++asked; return 7; }) != 7) return 2;   // asked again
+  if (once.get([&] { ++asked; return 9; }) != 7) return 3;   // kept
+  if (asked != 2) return 4;
+  npu_b200::AskedOnce shared[3];
+  std::atomic<int> wrong{0};
+  std::vector<std::thread> threads;
+  for (int t = 0; t < 8; ++t)
+    threads.emplace_back([&] {
+      for (int i = 0; i < 3000; ++i)
+        if (shared[i % 3].get([&] { return i % 3 + 1; }) != i % 3 + 1) ++wrong;
+    });
+  for (auto& t : threads) t.join();
+  return wrong ? 5 : 0;
+}
+""")
+    from pathlib import Path
+    cuda = Path(build.nvcc()).resolve().parent.parent / "include"
+    program = tmp_path / "asked"
+    done = subprocess.run(["g++", "-std=c++17", "-O1", "-pthread", "-fsanitize=thread", "-I", str(build.CSRC),
+                           "-isystem", str(cuda), str(source), "-o", str(program)], capture_output=True, text=True)
+    assert done.returncode == 0, done.stderr
+    ran = subprocess.run([str(program)], capture_output=True, text=True)
+    assert ran.returncode == 0, ran.stderr
