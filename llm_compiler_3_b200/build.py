@@ -60,11 +60,16 @@ def _compile(src: Path, force: bool, hdr_mtime: float, extra: list[str]) -> Path
 
 def _build_bindings(force: bool, hdr_mtime: float) -> None:
     """The Python binding of the paged-cache and beam operators (csrc/bindings.cpp): C++ against
-    torch's headers, calling the library next to it."""
+    torch's headers, calling the library next to it.  Without torch there is none, and the library
+    serves its C ABI alone."""
     import sysconfig
 
-    import torch
-    from torch.utils.cpp_extension import include_paths, library_paths
+    try:
+        import torch
+        from torch.utils.cpp_extension import include_paths, library_paths
+    except ImportError as exc:
+        print(f"no Python binding of the paged-cache and beam operators without torch ({exc})", file=sys.stderr)
+        return
     src = CSRC / "bindings.cpp"
     if (not force and BINDINGS.exists()
             and BINDINGS.stat().st_mtime >= max(src.stat().st_mtime, hdr_mtime)):
@@ -87,7 +92,7 @@ def _build_bindings(force: bool, hdr_mtime: float) -> None:
 
 def build(force: bool = False, jobs: int | None = None, verbose_ptxas: bool = False) -> Path:
     """Compile every csrc/*.cu for sm_100a, link libnpu_b200.so, build the Python binding that
-    calls it; return the library's path."""
+    calls it (where there is torch); return the library's path."""
     BUILD.mkdir(exist_ok=True)
     LIBDIR.mkdir(exist_ok=True)
     sources = sorted(CSRC.glob("*.cu"))

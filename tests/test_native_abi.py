@@ -111,3 +111,17 @@ int main() {
     assert done.returncode == 0, done.stderr
     ran = subprocess.run([str(program)], capture_output=True, text=True)
     assert ran.returncode == 0, ran.stderr
+
+
+def test_library_builds_without_torch():
+    """A program of the C ABI needs nvcc alone: without torch the build leaves the Python binding out."""
+    import sys
+    from llm_compiler_3_b200 import build
+    build.build()
+    before = build.BINDINGS.read_bytes()
+    done = subprocess.run([sys.executable, "-c", "import sys; sys.modules['torch'] = None\n"
+                           "from llm_compiler_3_b200 import build; print(build.build())"],
+                          capture_output=True, text=True, cwd=build.ROOT)
+    assert done.returncode == 0, done.stderr
+    assert done.stdout.strip() == str(build.LIBRARY) and "without torch" in done.stderr
+    assert build.BINDINGS.read_bytes() == before
