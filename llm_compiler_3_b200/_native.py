@@ -144,6 +144,11 @@ def bindings():
             raise NativeUnavailable(
                 f"cannot load llm_compiler_3_b200/_bindings.so ({exc}): run "
                 "`python -m llm_compiler_3_b200.build`") from exc
+        import torch
+        if _bindings.built_for != torch.__version__:
+            raise NativeUnavailable(
+                f"llm_compiler_3_b200/_bindings.so was built for torch {_bindings.built_for}, not for "
+                f"{torch.__version__}: run `python -m llm_compiler_3_b200.build`")
         _bound = _bindings
     return _bound
 

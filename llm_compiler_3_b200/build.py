@@ -60,8 +60,8 @@ def _compile(src: Path, force: bool, hdr_mtime: float, extra: list[str]) -> Path
 
 def _build_bindings(force: bool, hdr_mtime: float) -> None:
     """The Python binding of the paged-cache and beam operators (csrc/bindings.cpp): C++ against
-    torch's headers, calling the library next to it.  Without torch there is none, and the library
-    serves its C ABI alone."""
+    torch's headers, calling the library next to it; built for one torch and one Python.  Without
+    torch there is none, and the library serves its C ABI alone."""
     import sysconfig
 
     try:
@@ -71,13 +71,16 @@ def _build_bindings(force: bool, hdr_mtime: float) -> None:
         print(f"no Python binding of the paged-cache and beam operators without torch ({exc})", file=sys.stderr)
         return
     src = CSRC / "bindings.cpp"
-    if (not force and BINDINGS.exists()
+    stamp = BUILD / "bindings.stamp"
+    built_for = f"torch {torch.__version__}, Python {sys.version_info.major}.{sys.version_info.minor}"
+    if (not force and BINDINGS.exists() and stamp.exists() and stamp.read_text() == built_for
             and BINDINGS.stat().st_mtime >= max(src.stat().st_mtime, hdr_mtime)):
         return
     cuda = Path(nvcc()).resolve().parent.parent
     tmp = BINDINGS.with_suffix(".so.tmp")
     cmd = ["g++", "-O2", "-std=c++17", "-shared", "-fPIC", "-fvisibility=hidden",
            f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
+           f'-DNPU_B200_BUILT_FOR="{torch.__version__}"',
            "-I", str(INCLUDE), "-isystem", str(cuda / "include"),
            *[x for p in include_paths() for x in ("-isystem", p)],
            "-isystem", sysconfig.get_path("include"), str(src), "-o", str(tmp),
@@ -88,6 +91,7 @@ def _build_bindings(force: bool, hdr_mtime: float) -> None:
     if done.returncode:
         raise RuntimeError(f"g++ failed on {src.name}:\n{done.stdout}\n{done.stderr}")
     os.replace(tmp, BINDINGS)
+    stamp.write_text(built_for)
 
 
 def build(force: bool = False, jobs: int | None = None, verbose_ptxas: bool = False) -> Path:

@@ -289,6 +289,7 @@ PYBIND11_MODULE(_bindings, m) {
       PyErr_SetString(py::module_::import("torch").attr("OutOfMemoryError").ptr(), e.what_without_backtrace());
     }
   });
+  m.attr("built_for") = NPU_B200_BUILT_FOR;  // the version of torch
   m.def("paged_decode", &paged_decode);
   m.def("paged_prefill", &paged_prefill);
   m.def("paged_append", &paged_append);

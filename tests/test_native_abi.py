@@ -125,3 +125,33 @@ def test_library_builds_without_torch():
     assert done.returncode == 0, done.stderr
     assert done.stdout.strip() == str(build.LIBRARY) and "without torch" in done.stderr
     assert build.BINDINGS.read_bytes() == before
+
+
+def test_binding_is_built_for_the_torch_that_loads_it(tmp_path, monkeypatch):
+    """Built again for another version of torch, and refused by name where it was not."""
+    import types
+    import torch
+    from llm_compiler_3_b200 import _native, build
+    built = []
+
+    def run(cmd, **kw):
+        built.append(cmd)
+        tmp_path.joinpath("_bindings.so.tmp").write_bytes(b"")
+        return subprocess.CompletedProcess(cmd, 0, "", "")
+
+    monkeypatch.setattr(build, "BINDINGS", tmp_path / "_bindings.so")
+    monkeypatch.setattr(build, "BUILD", tmp_path)
+    monkeypatch.setattr(build.subprocess, "run", run)
+    for version, times in ((torch.__version__, 1), (torch.__version__, 1), ("9.9.0", 2), ("9.9.0", 2)):
+        monkeypatch.setattr(torch, "__version__", version)
+        build._build_bindings(False, 0.0)
+        assert len(built) == times
+    assert any("9.9.0" in word for word in built[1])
+    monkeypatch.undo()
+
+    import llm_compiler_3_b200
+    _native.lib()
+    monkeypatch.setattr(_native, "_bound", None)
+    monkeypatch.setattr(llm_compiler_3_b200, "_bindings", types.SimpleNamespace(built_for="9.9.0"), raising=False)
+    with pytest.raises(_native.NativeUnavailable, match="built for torch 9.9.0"):
+        _native.bindings()
