@@ -799,8 +799,9 @@ extern "C" int npu_b200_beam_reorder(const void* d_state, const int32_t* d_paren
   NPU_REQUIRE(rows >= 1 && new_rows >= 1 && row_bytes >= 1 && row_bytes < size_t(1) << 40,
               "beam_reorder: %d rows to %d of %zu bytes", rows, new_rows, row_bytes);
   const uintptr_t a = reinterpret_cast<uintptr_t>(d_state), b = reinterpret_cast<uintptr_t>(d_out);
-  NPU_REQUIRE(!overlap(d_state, row_bytes * rows, d_out, row_bytes * new_rows),
-              "beam_reorder: the output must not overlap the state");
+  NPU_REQUIRE(!overlap(d_state, row_bytes * rows, d_out, row_bytes * new_rows) &&
+                  !overlap(d_parents, new_rows * size_t(4), d_out, row_bytes * new_rows),
+              "beam_reorder: the output must not overlap the state or the parents");
   ReorderParams p = {d_state, d_out, d_parents, 0, rows, new_rows};
   const cudaStream_t s = static_cast<cudaStream_t>(stream);
   const uintptr_t all = a | b | row_bytes;

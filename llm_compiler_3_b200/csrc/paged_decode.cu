@@ -688,9 +688,12 @@ extern "C" int npu_b200_paged_decode(const void* d_q, const void* d_k_pages, con
               "paged_decode: workspace of %zu bytes needed, %zu given", need, workspace_bytes);
 
   const size_t q_bytes = static_cast<size_t>(batch) * q_heads * head_dim * 2;
-  NPU_REQUIRE(!overlap(d_q, q_bytes, d_out, q_bytes), "paged_decode: out must not overlap q");
-
   const uint64_t rows = static_cast<uint64_t>(num_pages) * kv_heads * page_size;
+  const size_t pool = rows * head_dim * 2;
+  NPU_REQUIRE(!overlap(d_q, q_bytes, d_out, q_bytes) && !overlap(d_k_pages, pool, d_out, q_bytes) &&
+                  !overlap(d_v_pages, pool, d_out, q_bytes),
+              "paged_decode: out must not overlap q or the pages");
+
   const int tile = head_dim == 128 ? PdShape<128, 1>::kTile : PdShape<64, 1>::kTile;
   const int box = page_box(page_size, tile);
   CUtensorMap km, vm;

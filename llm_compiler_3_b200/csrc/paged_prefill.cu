@@ -764,7 +764,10 @@ extern "C" int npu_b200_paged_prefill(const void* d_q, const void* d_k_pages, co
   p.scale_log2 = std::max(std::fabs(scale) * 1.4426950408889634f, 1e-30f);
 
   const size_t q_bytes = static_cast<size_t>(batch) * q_heads * queries * head_dim * 2;
-  NPU_REQUIRE(!overlap(d_q, q_bytes, d_out, q_bytes), "paged_prefill: out must not overlap q");
+  const size_t pool = rows * head_dim * 2;
+  NPU_REQUIRE(!overlap(d_q, q_bytes, d_out, q_bytes) && !overlap(d_k_pages, pool, d_out, q_bytes) &&
+                  !overlap(d_v_pages, pool, d_out, q_bytes),
+              "paged_prefill: out must not overlap q or the pages");
   CUtensorMap qm, km, vm;
   rc = make_tensor_map_3d(&qm, d_q, head_dim, queries, static_cast<uint64_t>(batch) * q_heads,
                           static_cast<uint64_t>(queries) * head_dim * 2, p.bm, 64);

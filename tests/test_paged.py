@@ -167,6 +167,25 @@ def test_outputs_over_inputs_are_refused():
                                                 1 << 26, None))
 
 
+def test_outputs_over_pages_are_refused():
+    """An output in the pool that the call reads, or over the parents it goes by."""
+    from llm_compiler_3_b200 import _native
+    lib = _native.lib()
+    p = [(i + 1) << 28 for i in range(7)]
+    pool = 9 * 2 * 16 * 128 * 2
+    for pages in p[1:3]:
+        for shift in (0, 16, pool - 16):
+            assert lib.npu_b200_paged_decode(*p[:5], pages + shift, 3, 8, 2, 128, 9, 16, 4, 0, 0, 0.1, p[6], 1 << 26,
+                                             None) == -1
+            assert b"overlap" in lib.npu_b200_last_error()
+            assert lib.npu_b200_paged_prefill(*p[:5], None, pages + shift, 3, 8, 2, 128, 5, 9, 16, 4, 0, 0, 0.1,
+                                              None) == -1
+            assert b"overlap" in lib.npu_b200_last_error()
+    for out in (p[1], p[1] + 12, p[1] - 60):
+        assert lib.npu_b200_beam_reorder(p[0], p[1], out, 3, 4, 16, None) == -1
+        assert b"overlap" in lib.npu_b200_last_error()
+
+
 def test_operators_refuse_cpu_tensors():
     from llm_compiler_3_b200 import ops
     k, v, table = paged_cache([5], 1, 64, 8)
