@@ -143,9 +143,49 @@ NPU_B200_API int npu_b200_flash_decode_noalloc(const void* d_q, const void* d_k,
  * accumulation; the softmax weights are rounded to FP16 as the second MMA's
  * operand; the output is rounded once.  A row that sees no key is zero.
  *
- *   d_q, d_out [batch, q_heads, queries, head_dim] FP16, 16-byte aligned, apart,
- *              d_out apart from the pages too.  Rows past d_q_lens[b], at a
- *              negative position, or without a visible key, are zero
+ *   d_q, d_out [batch, q_heads, queries, head_dim]
+ *   d_k, d_v   [batch, kv_heads, max_seq, head_dim]   (the KV-cache layout)
+ *   d_q_start  [batch] int32 or NULL
+ *   head_dim in {32, 64, 128}; keys in [0, max_seq]; batch x kv_heads <= 65535;
+ *   every pointer 16-byte aligned.  No workspace; calls may overlap. */
+NPU_B200_API int npu_b200_prefill_attention(const void* d_q, const void* d_k, const void* d_v,
+                                            const int32_t* d_q_start, void* d_out, int batch,
+                                            int q_heads, int kv_heads, int head_dim, int queries,
+                                            int keys, int max_seq, float scale, int causal,
+                                            void* stream);
+
+/* ---------------------------------------------------------------------------
+ * Paged key-value cache.
+ *
+ * Keys (and values) of any number of sequences in a pool of fixed-size pages, so
+ * that a cache grows page by page and sequences share what they have in common
+ * (no counterpart in the reference, whose compiled programs hold one flat cache
+ * per sequence):
+ *
+ *   d_k_pages, d_v_pages [num_pages, kv_heads, page_size, head_dim] FP16, 16-byte
+ *                aligned; head_dim in {64, 128}; page_size a multiple of 8 in
+ *                [8, 65536]; num_pages x kv_heads x page_size < 2^31
+ *   d_page_table [batch, table_entries] int32: position j of sequence b is row
+ *                j % page_size of page d_page_table[b][j / page_size].  Entries of
+ *                positions that a call does not touch may hold anything (-1 where
+ *                npu_b200_page_update has none).
+ *
+ * An entry outside [0, num_pages) that a call does need sets the bounds bit of
+ * npu_b200_device_status, and the access is skipped (keys and values read as
+ * zero, new rows are dropped).
+ *
+ * window and sinks: with window > 0 the token at position p sees key j iff
+ * j <= p and (j > p - window or j < sinks): the last `window` keys, itself
+ * included, and the first `sinks`.  window == 0: every key up to p.  Pages that
+ * hold no visible key are not read; their entries may be -1.
+ * ------------------------------------------------------------------------- */
+
+/* Attention of one new token per sequence, at position d_seq_lens[b] - 1 (its
+ * own key and value are in the pages already: npu_b200_paged_append), head h with
+ * KV head h / (q_heads / kv_heads); the counterpart of npu_b200_flash_decode:
+ *
+ *   d_q, d_out [batch, q_heads, head_dim] FP16, 16-byte aligned, apart, d_out apart
+ *              from the pages too; any group
  *   d_seq_lens [batch] int32 keys per sequence, clamped to [0, table_entries x
  *              page_size]; 0 keys gives a zero row
  *   d_workspace npu_b200_paged_decode_workspace_size() bytes, 16-byte aligned, on
@@ -173,8 +213,8 @@ NPU_B200_API int npu_b200_paged_decode(const void* d_q, const void* d_k_pages,
  * of every query's own position.
  *
  *   d_q, d_out [batch, q_heads, queries, head_dim] FP16, 16-byte aligned, apart,
- *              d_out apart from the pages too.  Rows past d_q_lens[b], at a negative position, or without a visible
- *              key, are zero
+ *              d_out apart from the pages too.  Rows past d_q_lens[b], at a
+ *              negative position, or without a visible key, are zero
  *   d_seq_lens [batch] int32 keys per sequence, the chunk included, clamped to
  *              [0, table_entries x page_size]; d_q_lens [batch] int32, clamped to
  *              [0, queries]
