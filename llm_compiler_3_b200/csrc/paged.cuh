@@ -44,6 +44,13 @@ struct Divisor {
   }
 };
 
+// Softmax weights, FP16 as the second product's operand, are relative to a reference 2^7 below
+// the maximum that set it.  It moves once a weight would pass 2^15, so weights fit FP16, and
+// those far below the maximum keep their bits down to 2^-21 of it (relative to the maximum
+// itself they were gone at 2^-25, and with them all that thousands of such keys add up to).
+constexpr float kBelowMax = 7.f;
+constexpr float kMostLog2 = 15.f;
+
 // Rows of the largest TMA box that never crosses a page: the largest power of
 // two that divides P, at most `tile`.
 inline int page_box(int page_size, int tile) {

@@ -2,7 +2,7 @@
 //
 // Per query head h with KV head h / group and n = seq_lens[b] keys:
 //   out[b, h] = softmax_j(scale * q[b, h] . k[j]) v[j]  over the visible keys j
-// (paged.cuh), with a running max m, sum l and output O in FP32 per pass over
+// (paged.cuh), with a running reference m, sum l and output O in FP32 per pass over
 // the keys, joined as m = max m_i, l = sum l_i 2^(m_i - m), O = sum O_i 2^(m_i - m).
 // The weights are rounded to FP16 as the second MMA's operand (the values are
 // FP16 too); the output is rounded once.
@@ -41,7 +41,6 @@
 namespace npu_b200 {
 namespace {
 
-constexpr float kRescaleLog2 = 8.f;
 constexpr int kMaxShares = 8;  // CTAs of a cluster
 constexpr int kFewTiles = 8;   // tiles of a warp, at most, where clusters take the units
 
@@ -365,10 +364,18 @@ __global__ void __launch_bounds__(PdShape<D, NB>::kThreads, 1)
             mma_16816(sv[mt][nb], a[0], a[1], a[2], a[3], qf[nb][s][0], qf[nb][s][1]);
         });
       });
-      // Online softmax, in the base-2 logarithm's domain.  A column's maximum moves only
-      // when a score exceeds it by 2^8 (weights stay below 256, exact enough in FP16):
-      // then, and only then, the lanes of a column compare notes and O is rescaled.
+      // Online softmax, in the base-2 logarithm's domain.  A column's reference moves only
+      // when a weight would pass 2^15: then, and only then, the lanes of a column compare notes
+      // and O is rescaled.
       bool grows = false;
+      float most[NB][2];  // scores that need no other reference
+#pragma unroll
+      for (int nb = 0; nb < NB; ++nb)
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+          most[nb][j] = m_run[nb][j] + kMostLog2;
+          if (most[nb][j] - m_run[nb][j] > kMostLog2) most[nb][j] = m_run[nb][j];  // rounded up
+        }
 #pragma unroll
       for (int mt = 0; mt < MT; ++mt)
 #pragma unroll
@@ -378,7 +385,7 @@ __global__ void __launch_bounds__(PdShape<D, NB>::kThreads, 1)
             float v = sv[mt][nb][r] * p.scale_log2;
             if (!whole && !at.keys.sees(key0 + mt * 16 + g + ((r & 2) ? 8 : 0))) v = -INFINITY;
             sv[mt][nb][r] = v;
-            grows |= v > m_run[nb][r & 1] + kRescaleLog2;
+            grows |= v > most[nb][r & 1];
           }
       if (__any_sync(0xffffffffu, grows)) {
 #pragma unroll
@@ -393,7 +400,8 @@ __global__ void __launch_bounds__(PdShape<D, NB>::kThreads, 1)
             top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 8));
             top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 16));
             alpha[j] = 1.f;
-            if (top > m_run[nb][j] + kRescaleLog2) {
+            if (top > most[nb][j]) {
+              top -= kBelowMax;
               alpha[j] = m_run[nb][j] == -INFINITY ? 0.f : fast_exp2(m_run[nb][j] - top);
               m_run[nb][j] = top;
               l_run[nb][j] *= alpha[j];

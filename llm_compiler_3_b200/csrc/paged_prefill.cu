@@ -3,7 +3,7 @@
 // Query i < q_lens[b] of sequence b sits at position p = seq_lens[b] - q_lens[b] + i
 // and sees the keys of paged.cuh: causal, with an optional window and sinks.
 //   out[b, h, i] = sum_j softmax_j(scale q[b, h, i] . k[j]) v[j]
-// in one pass over the keys with a running maximum m, sum l and output O (FP32).
+// in one pass over the keys with a running reference m, sum l and output O (FP32).
 // The weights are rounded to FP16 as the second product's operand (the values are
 // FP16 too), the output is rounded once.  Rows that see no key, and rows past
 // q_lens[b], are zero.
@@ -27,8 +27,8 @@
 // TMEM: S0, S1 (128 columns each), O0, O1 (D each); P_t, FP16, lies over the first
 // half of S_t.  The tensor pipe works in order, so S_t(j + 1), issued after
 // P_t(j) V, cannot overwrite weights that are still read, and its completion says
-// that O_t is up to date.  A row's maximum moves, and its O row is rescaled, only
-// when a tile's exceeds it by 2^8: weights stay below 256, exact enough in FP16.
+// that O_t is up to date.  A row's reference moves, and its O row is rescaled,
+// only when a weight would pass 2^15 (paged.cuh).
 #include <limits.h>
 #include <math.h>
 
@@ -50,7 +50,6 @@ constexpr int KT = 128;           // keys per tile
 constexpr int kUnit = 32;
 constexpr int kThreads = 352;
 constexpr uint32_t kTmemCols = 512;
-constexpr float kRescaleLog2 = 8.f;
 constexpr int kMaxSplits = 8;     // CTAs that share a tile pair's keys
 
 template <int D>
@@ -527,11 +526,11 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll
       for (int e = 0; e < 4; ++e) top[e] = fmaxf(top[e], __uint_as_float(sr[KT - 4 + e]));
       const float mx = fmaxf(max3(top[0], top[1], top[2]), top[3]);
-      const float m_tile = mx * p.scale_log2;
-      const bool grow = m_tile > m_run + kRescaleLog2;
+      const bool grow = __fmaf_rn(mx, p.scale_log2, -m_run) > kMostLog2;
       if (__any_sync(0xffffffffu, grow)) {
         float alpha = 1.f;
         if (grow) {
+          const float m_tile = __fmaf_rn(mx, p.scale_log2, -kBelowMax);
           alpha = m_run == -INFINITY ? 0.f : fast_exp2(m_run - m_tile);
           l_run *= alpha;
           m_run = m_tile;

@@ -5,8 +5,9 @@ from their pages one by one, every key is shown or hidden by the written rule,
 and softmax is taken in FP64.  ``attention_paged`` also returns, per output
 element, how far a kernel may be off that rounds only where the kernels do:
 
-  * each softmax weight to FP16 before the second product: a relative 2^-11
-    (below 2^-14, FP16's smallest normal number, an absolute 2^-25);
+  * each softmax weight to FP16 before the second product, relative to a number
+    2^7 or more below the largest weight: a relative 2^-11 (below 2^-21 of the
+    largest, where FP16 is subnormal, an absolute 2^-32 of it);
   * scores in FP32: a dot product of D terms is off by at most (D + 4) 2^-23
     times the sum of the terms' magnitudes (tensor cores may cut instead of
     round, hence 2^-23), which moves each weight by that relative amount, and
@@ -66,7 +67,7 @@ def attention_paged(q, k_pages, v_pages, table, seq_lens, q_lens=None, window=0,
                 off = float((kk.abs() @ qq.abs()).max()) * abs(scale) * (dim + 4) * 2.0 ** -23
                 rel = 2.0 ** -11 + 2 * off + 2.0 ** -20 + 2 * len(see) * 2.0 ** -23
                 bound[b, h, i] = (2.0 ** -11 * out[b, h, i].abs() + 2.0 ** -25 + rel * mass
-                                  + len(see) * 2.0 ** -25 * vv.abs().max())
+                                  + len(see) * 2.0 ** -32 * vv.abs().max())
     return out, bound
 
 

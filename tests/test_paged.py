@@ -492,3 +492,59 @@ def test_decode_of_queries_and_keys_that_are_no_numbers(cuda, dim, heads, kv_hea
     got = _decode(q, k, v, wide, lens)
     want, bound = oracle.attention_paged(q[:, :, None], k, v, wide, lens, q_lens=[1] * len(lens))
     check_with_nan(got, want[:, :, 0], bound[:, :, 0])
+
+
+def far_below(dim, page, n):
+    """(q [1, 2, D], k, v, table): one key whose weight is 2^25 times that of each of the others, whose
+    values alone are not 0."""
+    k, v, table = paged_cache([n], 1, dim, page, seed=n)
+    for j in range(n):
+        at = int(table[0, j // page]), 0, j % page
+        k[at], v[at] = 0.0, 64.0
+    k[int(table[0, 0]), 0, 0] = 17.68 / dim
+    v[int(table[0, 0]), 0, 0] = 0.0
+    return torch.ones(1, 2, dim).half(), k, v, table
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("n,reach", [(20, 20), (900, 900), (3000, 80000)])
+def test_decode_keeps_weights_far_below_the_largest(cuda, dim, n, reach):
+    """Weights of 2^-25 of the largest: each is rounded by 2^-11 of itself (2^-32 of the largest), like
+    the output (by 2^-25 at least), and the sums by less than 2^-11 together."""
+    q, k, v, table = far_below(dim, 16, n)
+    wide = torch.full((1, (reach + 15) // 16), -1, dtype=torch.int32)
+    wide[:, :table.shape[1]] = table
+    got = _decode(q, k, v, wide, [n], scale=1.0)
+    want, _ = oracle.attention_paged(q[:, :, None], k, v, wide, [n], [1], scale=1.0)
+    bound = 3 * 2.0 ** -11 * want + 2.0 ** -25 + 64 * n * 2.0 ** -32
+    check(got, want[:, :, 0], bound[:, :, 0])
+
+
+def steep(dim, page, n, base):
+    """(q [1, 2, D], k, v, table): scores of `base` and up to 40 more, rising and falling, and values of 1,
+    so that attention is 1 whatever the weights are."""
+    k, v, table = paged_cache([n], 1, dim, page, seed=n)
+    r = torch.Generator().manual_seed(n)
+    step = torch.rand(n, generator=r) * 40
+    step[:n // 3] = torch.linspace(0, 40, n // 3)
+    q = torch.zeros(1, 2, dim).half()
+    q[..., 0] = 2.0 ** (base // 2)
+    q[..., 1] = 1.0
+    for j in range(n):
+        at = int(table[0, j // page]), 0, j % page
+        k[at], v[at] = 0.0, 1.0
+        k[at][0], k[at][1] = 2.0 ** (base - base // 2), step[j]
+    return q, k, v, table
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("base", [0, 10, 20, 23, 24, 25, 26])
+def test_decode_of_steep_and_large_scores(cuda, dim, base):
+    """No weight passes FP16's range, however large the scores and their steps: the output is the sum of
+    rounded weights over the sum of the weights, 2^-11 and the output's own rounding off 1."""
+    for n, scale in ((300, 1.0), (700, -1.0), (5000, 1.0)):
+        q, k, v, table = steep(dim, 16, n, base)
+        got = _decode(q * scale, k, v, table, [n], scale=scale)
+        assert float((got.double() - 1).abs().max()) <= 2.0 ** -10 + n * 2.0 ** -23

@@ -7,7 +7,7 @@ import torch
 
 import oracle
 from conftest import seeded
-from test_paged import INF, NAN, check, check_with_nan, ints, paged_cache
+from test_paged import INF, NAN, check, check_with_nan, far_below, ints, paged_cache, steep
 
 
 def _prefill(q, k, v, table, lens, q_lens=None, **kw):
@@ -376,3 +376,27 @@ def test_values_that_are_no_numbers_behind_long_prefixes(cuda, heads, dim, windo
     args = (q[rows], k, v.nan_to_num(0, 0, 0), *args[3:])
     want, bound = oracle.attention_paged(*args, window=window, sinks=sinks)
     check(torch.where(odd, want.half(), got[rows]), want, torch.where(odd, want.abs(), bound))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("n,queries", [(20, 3), (900, 7), (900, 300)])
+def test_keeps_weights_far_below_the_largest(cuda, dim, n, queries):
+    """As in decode, for every query that sees some of them."""
+    q, k, v, table = far_below(dim, 16, n)
+    q = q[:, :, None].expand(1, 2, queries, dim).contiguous()
+    got = _prefill(q, k, v, table, [n], scale=1.0)
+    want, _ = oracle.attention_paged(q, k, v, table, [n], scale=1.0)
+    check(got, want, 3 * 2.0 ** -11 * want + 2.0 ** -25 + 64 * n * 2.0 ** -32)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("base", [0, 10, 20, 23, 24, 25, 26])
+def test_steep_and_large_scores(cuda, dim, base):
+    """As in decode."""
+    for n, queries, scale in ((300, 300, 1.0), (700, 5, -1.0), (3000, 130, 1.0)):
+        q, k, v, table = steep(dim, 16, n, base)
+        q = q[:, :, None].expand(1, 2, queries, dim).contiguous() * scale
+        got = _prefill(q, k, v, table, [n], scale=scale)
+        assert float((got.double() - 1).abs().max()) <= 2.0 ** -10 + n * 2.0 ** -23
