@@ -219,7 +219,8 @@ NPU_B200_API int npu_b200_paged_decode(const void* d_q, const void* d_k_pages,
  *              [0, table_entries x page_size]; d_q_lens [batch] int32, clamped to
  *              [0, queries]
  * Arithmetic as in npu_b200_paged_decode.  Infinite and NaN keys and values reach the
- * queries that see them and no others.  No workspace; calls may overlap. */
+ * queries that see them and no others (an infinite value whose weight is below 2^-32 of
+ * the largest may come as NaN).  No workspace; calls may overlap. */
 NPU_B200_API int npu_b200_paged_prefill(const void* d_q, const void* d_k_pages,
                                         const void* d_v_pages, const int32_t* d_page_table,
                                         const int32_t* d_seq_lens, const int32_t* d_q_lens,

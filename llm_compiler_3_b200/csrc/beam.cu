@@ -14,7 +14,8 @@
 // its lanes' maxima over their first words, then, each time twice as much has been
 // read, the width-th best candidate.  That leaves some width x log2(length / 4096)
 // candidates of a stretch, so the selection costs one comparison per 8 logits (sorted
-// lists that each warp kept for itself cost twice the rest).  A warp whose list runs
+// lists that each warp kept for itself cost twice the rest; rows whose logits nearly all equal
+// the floor, as under a mask of the type's lowest number, cost 17 times as much).  A warp whose list runs
 // full, on rising logits, keeps its `width` best and raises the floor.  A second,
 // dependent launch joins the stretches.
 //
@@ -781,7 +782,8 @@ extern "C" int npu_b200_beam_select(const void* d_logits, int logits_f32, const 
   // Where three CTAs an SM do not hold all rows at once, four do with some spilled registers
   // (64 x 8 rows of 128256 tokens 57 -> 46 us; 100 x 4 of 32000, which three hold, 15.9 ->
   // 18).  Not with finished beams, whose CTAs end at once: the places they leave go to the
-  // rows that wait (a fifth of them finished: 43 us, with four 49).
+  // rows that wait (a fifth of them finished: 43 us, with four 49); flags of which few are set
+  // pay for it (none of them: 68 us instead of 53, cold caches).
   const bool four = rows * p.splits > 3ll * sm_count() && d_done == nullptr;
   const auto stretch = logits_f32 ? (four ? beam_stretch_kernel<float, 4> : beam_stretch_kernel<float, 3>)
                                   : (four ? beam_stretch_kernel<__half, 4> : beam_stretch_kernel<__half, 3>);

@@ -21,9 +21,10 @@
 //   warp 8          TMA: both Q tiles, then K and V tiles in one ring (K0 V0 K1 V1
 //                   ...), one box per piece of a page, each lane one
 //   warp 9          MMA issue: O_t += P_t V, then the next S_t = Q_t K^T
-//   warp 10         clears the hidden rows of V tiles on a border
+//   warp 10         V tiles with keys that not all of the CTA's queries see: clears the rows that
+//                   none sees, takes infinite and NaN numbers out of the others
 // When there are few query tiles, a cluster of up to 8 CTAs shares the keys of each pair;
-// their O, maxima and sums meet in shared memory, each CTA joining a share of the dimensions.
+// their O, references and sums meet in shared memory, each CTA joining a share of the dimensions.
 // TMEM: S0, S1 (128 columns each), O0, O1 (D each); P_t, FP16, lies over the first
 // half of S_t.  The tensor pipe works in order, so S_t(j + 1), issued after
 // P_t(j) V, cannot overwrite weights that are still read, and its completion says

@@ -3,8 +3,9 @@
 //
 // page_update and page_compact work on whole numbers only: tables and reference
 // counts of a few thousand to a few hundred thousand words, in phases that each
-// need the previous one finished everywhere.  They are bound by latency, so one
-// launch does it all: a single cluster of 8 CTAs, whose hardware barrier orders
+// need the previous one finished everywhere.  They are bound by latency (256 rows of 96
+// entries and 12000 pages: 14 us; 8192 rows of 64 and 600000 pages, 227 us, are bound by what 8
+// SMs read), so one launch does it all: a single cluster of 8 CTAs, whose hardware barrier orders
 // the phases (and their global writes) without flags or further launches, and
 // whose distributed shared memory carries the counts of the prefix sums.  Every
 // result is a count, a rank or a lowest index, so no order of atomics shows.
